@@ -187,6 +187,14 @@ int rlu_gemm_fp8blk_m16(const void* qx, const float* xs, const void* w, const fl
 int rlu_gemm_fp8blk_m64(const void* qx, const float* xs, const void* w, const float* ws,
                         void* y, int M, int N, int K, hipStream_t stream);
 
+/* No counterpart in the reference (its head kernel takes decode rows only, kernels/
+ * fp8_target_lmhead.py:31): y [M, n] bf16 (rows ldy elements apart) = qx [M, K] e4m3 (xs [M, K/128])
+ * x w [n_pad, K]^T (ws [n_pad/128, K/128]), n_pad = n up to the next multiple of 128, w in fragment
+ * order, for any M and n: one weight read per tile of rows. Elements outside [M, n] are not
+ * written. M = 0 launches nothing. Returns -1 (bad sizes, ldy < n or a NULL pointer), -2 (K % 128). */
+int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void* w, const float* ws, void* y,
+                          long long ldy, int M, int n, int K, hipStream_t stream);
+
 /* Replaces shuffle_weight_gfx1201 (the load-time weight shuffle behind pack_fp8_block,
  * kernels/fp8_target_lmhead.py:44-66) for gfx950: row-major e4m3 [rows, K] -> MFMA fragment
  * order, the layout every GEMM above reads. Byte (n, k), n = 16 nt + r,

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from dataclasses import dataclass
 
 import torch
 
@@ -341,6 +342,65 @@ def pack_fp8_block(w: torch.Tensor, rows: int = 4096) -> tuple[torch.Tensor, tor
         ws[r0 // 128:r1 // 128] = scale.view((r1 - r0) // 128, K // 128)
         del wf, q
     return out, ws
+
+
+@dataclass(frozen=True)
+class PackedFp8:
+    """A weight as gemm_fp8_dense reads it; hold this on the layer."""
+    wq: torch.Tensor     # e4m3 [n_pad, k] in fragment order, rows n.. zero
+    ws: torch.Tensor     # f32 [n_pad/128, k/128]
+    n: int               # output features
+    k: int
+
+    @property
+    def n_pad(self) -> int:
+        return self.wq.shape[0]
+
+
+@torch.no_grad()
+def pack_fp8_dense(w: torch.Tensor, ws: torch.Tensor) -> PackedFp8:
+    """Row-major e4m3 [N, K] with its float32 block scales [ceil(N/128), K/128] -> PackedFp8: rows
+    padded with zeros to a multiple of 128 and laid out in fragment order. Runs once, at load."""
+    if w.ndim != 2 or w.dtype != FP8 or not w.is_cuda:
+        raise ValueError("pack_fp8_dense takes an e4m3 [N, K] weight on the GPU")
+    n, k = w.shape
+    if n < 1 or k < 1 or k % GROUP:
+        raise ValueError(f"pack_fp8_dense: [{n}, {k}], K must be a multiple of {GROUP}")
+    nb = -(-n // GROUP)
+    if ws.shape != (nb, k // GROUP) or ws.dtype != torch.float32 or ws.device != w.device:
+        raise ValueError(f"pack_fp8_dense: block scales must be float32 [{nb}, {k // GROUP}] "
+                         "beside the weight")
+    rows = torch.zeros((nb * GROUP, k), dtype=torch.uint8, device=w.device)
+    rows[:n] = w.view(torch.uint8)
+    with torch.cuda.device(w.device):
+        wq = shuffle_fp8_weight(rows.view(FP8))
+    return PackedFp8(wq=wq, ws=ws.contiguous(), n=n, k=k)
+
+
+def gemm_fp8_dense(qx: torch.Tensor, xs: torch.Tensor, w: PackedFp8,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """e4m3 [M, K] (xs [M, K/128], as fp8_quant_group gives them) x w^T -> bf16 [M, n], any M and n.
+    out may have padded rows (stride(0) >= n); only its [M, n] elements are written."""
+    if qx.ndim != 2 or qx.dtype != FP8 or not qx.is_cuda or not qx.is_contiguous():
+        raise ValueError("gemm_fp8_dense takes contiguous e4m3 [M, K] rows on the GPU")
+    M, K = qx.shape
+    if K != w.k:
+        raise ValueError(f"gemm_fp8_dense: rows of {K}, weight of {w.k}")
+    if xs.shape != (M, K // GROUP) or xs.dtype != torch.float32 or not xs.is_contiguous():
+        raise ValueError(f"gemm_fp8_dense: scales must be contiguous float32 [{M}, {K // GROUP}]")
+    if out is None:
+        out = torch.empty((M, w.n), dtype=torch.bfloat16, device=qx.device)
+    elif out.shape != (M, w.n) or out.dtype != torch.bfloat16 or \
+            (w.n > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < w.n):
+        raise ValueError(f"gemm_fp8_dense: out must be bf16 [{M}, {w.n}] with rows apart")
+    if not xs.device == w.wq.device == w.ws.device == out.device == qx.device:
+        raise ValueError("gemm_fp8_dense: operands on different devices")
+    ldy = out.stride(0) if M > 1 else w.n
+    with torch.cuda.device(qx.device):
+        rc = lib().rlu_gemm_fp8blk_dense(_p(qx), _p(xs), _p(w.wq), _p(w.ws), _p(out), ldy, M, w.n,
+                                         K, _P(stream_ptr()))
+    check(rc, "rlu_gemm_fp8blk_dense")
+    return out
 
 
 def moe_gemm_tiles(expert_ids: torch.Tensor, num_post_pad: torch.Tensor,
