@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "gemm_common.h"
+#include "head.h"
 #include "numerics.h"
 #include "rlu.h"
 #include "wave.h"
@@ -14,11 +15,11 @@ namespace dense {
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr int GROUP = 8;               // row tiles walked together
+constexpr int GROUP = 4;               // row tiles walked together
 constexpr int SC = 8;                  // steps of row scales staged at a time
 
 __device__ __forceinline__ v16f mfma32(v8i a, v8i b, v16f c) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 127, 0, 127);
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -34,21 +35,24 @@ __device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t b, int voff, int 
 
 // Barrier behind which every wave's loads to LDS so far have arrived (the fence of a barrier alone
 // does not wait for them).
+template <int LEFT = 0>
 __device__ __forceinline__ void staged_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0)
-  __syncthreads();
+  static_assert(LEFT < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4) << 14);        // vmcnt(LEFT)
+  lds_barrier();
 }
 
 // A wave has WM x WN tiles of 32 rows x 32 columns, a workgroup GM x GN waves.
-template <int WM_, int WN_, int GM_, int GN_>
+template <int WM_, int WN_, int GM_, int GN_, int ST_>
 struct Cfg {
-  static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_;
+  static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_, ST = ST_;
   static constexpr int BM = 32 * WM * GM, BN = 32 * WN * GN, NW = GM * GN;
   static constexpr int X = BM * 128, W = BN * 128;              // bytes of a step
   static constexpr int S = BM * SC * 4;                         // bytes of SC steps' row scales
   static constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW;      // loads of a wave
   static_assert(XI * 8 * NW == BM && WI * 8 * NW == BN, "the waves share the loads evenly");
-  static constexpr int LDS = 2 * (X + W + S);
+  static constexpr int SLOTS = WM % 2 ? WM : 2;                 // row tiles' operands held
+  static constexpr int LDS = ST * (X + W) + 2 * S;
 };
 
 template <class C>
@@ -60,8 +64,8 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
                                                            long long ldy, int M, int n, int K) {
   extern __shared__ __align__(16) uint8_t lds[];
   uint8_t* lx = lds;                                  // [2][BM rows][8 chunks of 16 B, swizzled]
-  uint8_t* lw = lds + 2 * C::X;                       // [2][BN / 16 strips][2][64 lanes][16 B]
-  uint8_t* ls = lw + 2 * C::W;                        // [2][BM / 8][8 rows][SC, swizzled] floats
+  uint8_t* lw = lds + C::ST * C::X;                       // [2][BN / 16 strips][2][64 lanes][16 B]
+  uint8_t* ls = lw + C::ST * C::W;                        // [2][BM / 8][8 rows][SC, swizzled] floats
   const int lane = lane_id();
   const int w = uniform((int)threadIdx.x / WAVE);
   const int nkg = K / 128;
@@ -71,8 +75,8 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
   const int tiles = (int)gridDim.x, tn = tiles / tm;
   const int xcd = (int)blockIdx.x & 7, per = tiles / 8, more = tiles % 8;
   const int id = xcd * per + min(xcd, more) + (int)blockIdx.x / 8;
-  const int grp = id / (GROUP * tn), gm = min(GROUP, tm - grp * GROUP), at = id - grp * GROUP * tn;
-  const int m0 = (grp * GROUP + at % gm) * C::BM, n0 = at / gm * C::BN;
+  const int band = id / (GROUP * tn), gm = min(GROUP, tm - band * GROUP), at = id - band * GROUP * tn;
+  const int m0 = (band * GROUP + at % gm) * C::BM, n0 = at / gm * C::BN;
   const int strips = (n + 127) / 128 * 8;
   const int rows = min(C::BM, M - m0), cols = min(C::BN, strips * 16 - n0);
   const uint8_t* gx = qx + (size_t)m0 * K;
@@ -82,36 +86,40 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
   auto buf = [&](const void* p, int bytes, bool live) __attribute__((always_inline)) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, live ? bytes : 0, BUF_WORD3);
   };
-  // a wave's loads take 8 rows, 8 lanes a row; a row's chunk q lies at q ^ (row & 7)
-  const int vx = lane / 8 * K + ((lane ^ (lane / 8)) & 7) * 16;
+  // a wave's loads take 8 rows, 8 lanes a row; a row's chunk q lies at q ^ (row / 2 & 7), so that 16
+  // rows' reads of one chunk meet all 64 banks (by row & 7, row r and r + 8 shared theirs)
+  const int vx = lane / 8 * K + ((lane ^ (lane / 16 + (w * C::XI & 1) * 4)) & 7) * 16;
   const int vw = lane * 16;
-  auto stage = [&](int b, int kb) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t bx = buf(gx, rows * K, kb < nkg);
-    const __amdgpu_buffer_rsrc_t bw = buf(gw, cols * K, kb < nkg);
-#pragma unroll
-    for (int i = 0; i < C::XI; ++i)
-      to_lds16(bx, vx, (w * C::XI + i) * 8 * K + kb * 128,
-               lx + b * C::X + (w * C::XI + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < C::WI; ++i) {
-      const int s = w * C::WI + i;                     // half a strip's step
-      to_lds16(bw, vw, (s / 2) * nkg * 2048 + kb * 2048 + (s & 1) * 1024,
-               lw + b * C::W + s * 1024);
-    }
-  };
-  // a wave's i-th load of the row scales of steps kb .. kb + SC
+  // A step's loads, one at a time: XI of rows, WI of half strips, and a part of the row scales that the
+  // steps from the next multiple of SC on read (the last part again once all are on their way).
+  constexpr int PIECES = C::XI + C::WI + 1;
   auto scales = [&](int b, int kb, int i) __attribute__((always_inline)) {
     const int e = w * C::XI + i;
     const int j = (lane ^ (lane / 8 + 2 * e)) & 7;
     to_lds4(buf(gs, rows * nkg * 4, kb < nkg), (lane / 8 * nkg + j) * 4, (e * 8 * nkg + kb) * 4,
             ls + b * C::S + e * 256);
   };
+  auto piece = [&](int b, int kb, int j) __attribute__((always_inline)) {
+    if (j < C::XI) {
+      const int e = w * C::XI + j;
+      to_lds16(buf(gx, rows * K, kb < nkg), vx ^ (j % 2 * 64), e * 8 * K + kb * 128,
+               lx + b * C::X + e * 1024);
+    } else if (j < C::XI + C::WI) {
+      const int e = w * C::WI + j - C::XI;             // half a strip's step
+      to_lds16(buf(gw, cols * K, kb < nkg), vw,
+               (e / 2) * nkg * 2048 + kb * 2048 + (e & 1) * 1024, lw + b * C::W + e * 1024);
+    } else {
+      const int s = kb - C::ST, c = (s >> 3) + 1;
+      static_assert(SC == 8, "s >> 3");
+      scales(c & 1, c * SC, min(s & 7, C::XI - 1));
+    }
+  };
 
   const int wm = w % C::GM, wn = w / C::GM;
   const int r = lane & 31, g = lane >> 5;
   const int nb = uniform((n0 + wn * 32 * C::WN) / 128);
   const float* wsr = ws + (size_t)min(nb, strips / 8 - 1) * nkg;
-  float acc[C::WM][C::WN][16];
+  v16f acc[C::WM][C::WN];
 #pragma unroll
   for (int t = 0; t < C::WM; ++t)
 #pragma unroll
@@ -119,88 +127,102 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[t][u][i] = 0.f;
   const uint8_t* pw = lw + wn * C::WN * 4096 + (r / 16) * 2048 + (32 * g + (r & 15)) * 16;
-  const uint8_t* px[4];                                // chunk 4 h + 2 g + i at [2 h + i]
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    px[c] = lx + wm * C::WM * 4096 + r * 128 + (((4 * (c / 2) + 2 * g + c % 2) ^ r) & 7) * 16;
+  // chunk 4 h + 2 g + i of a row lies at (that of h = i = 0) ^ (4 h + i)
+  const int ox = wm * C::WM * 4096 + r * 128 + ((2 * g ^ (r / 2)) & 7) * 16;
   const uint8_t* ps = ls + wm * C::WM * 1024 + (r / 8) * 256 + (r & 7) * 32;
 
-  v8i a[C::WN][2], x[2][2];
+  v8i a[C::WN][2], x0[C::SLOTS], x1;
   v16f d[2];
-  float f[2], sx[2], wsc;
-  auto read_w = [&](int b, int u) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t* p = pw + b * C::W + u * 4096 + h * 1024;
-      a[u][h] = pack8(*reinterpret_cast<const v4u*>(p), *reinterpret_cast<const v4u*>(p + 256));
-    }
+  float f[C::SLOTS], sx, wsc = wsr[0], wsn;
+  auto read_w = [&](int b, int u, int h) __attribute__((always_inline)) {
+    const uint8_t* p = pw + b * C::W + u * 4096 + h * 1024;
+    a[u][h] = pack8(*reinterpret_cast<const v4u*>(p), *reinterpret_cast<const v4u*>(p + 256));
   };
-  auto read_x = [&](int b, int kb, int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      x[t & 1][h] = pack8(*reinterpret_cast<const v4u*>(px[2 * h] + b * C::X + t * 4096),
-                          *reinterpret_cast<const v4u*>(px[2 * h + 1] + b * C::X + t * 4096));
-    sx[t & 1] = *reinterpret_cast<const float*>(ps + t * 1024 + (kb / SC & 1) * C::S +
+  auto read_x = [&](int b, int t, int h) __attribute__((always_inline)) {
+    const uint8_t* p = lx + b * C::X + t * 4096;
+    (h ? x1 : x0[t % C::SLOTS]) = pack8(*reinterpret_cast<const v4u*>(p + (ox ^ (64 * h))),
+                                 *reinterpret_cast<const v4u*>(p + (ox ^ (64 * h + 16))));
+  };
+  auto read_s = [&](int kb, int t) __attribute__((always_inline)) {
+    sx = *reinterpret_cast<const float*>(ps + t * 1024 + (kb / SC & 1) * C::S +
                                                 ((kb ^ (r + 2 * (r / 8))) & 7) * 4);
   };
-  // tile i = t WN + u of a step: its products, and the scaling of the tile before it
-  auto tile = [&](int i) __attribute__((always_inline)) {
-    const int t = i / C::WN, u = i % C::WN;
-    v16f z;
+  constexpr int T = C::WM * C::WN;
+  // (a part staged behind step s's barrier has arrived at that of step s + ST - 1, before the reads for s + ST)
+  static_assert(C::XI <= SC - C::ST + 1, "all parts are there when the next SC steps begin");
+  // Behind a step's barrier its buffer is free for step kb + ST, whose loads go out a few in each of the
+  // WINDOW tiles from there on: in one go they kept every wave from its products.
+  constexpr int WINDOW = T - 3 > C::WN ? T - 3 : C::WN, PER = (PIECES + WINDOW - 1) / WINDOW;
+  // the step whose operands are in buffer b; bp, bn: the buffers of the steps before and after it
+  auto step = [&](int bp, int b, int bn, int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) z[k] = 0.f;
-    d[i & 1] = mfma32(a[u][0], x[t & 1][0], z);
-    d[i & 1] = mfma32(a[u][1], x[t & 1][1], d[i & 1]);
-    constexpr int T = C::WM * C::WN;
-    const int p = (i + T - 1) % T;
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      acc[p / C::WN][p % C::WN][k] =
-          fmaf(d[(i + 1) & 1][k], f[p / C::WN & 1], acc[p / C::WN][p % C::WN][k]);
-    if (u == 0) f[t & 1] = wsc * sx[t & 1];
-  };
-  static_assert(C::XI <= SC, "a step stages at most one part of the scales");
-  auto step = [&](const int b, int kb) __attribute__((always_inline)) {
-#pragma unroll
-    for (int t = 0; t < C::WM; ++t) {
-      if (t == C::WM - 1) {
-        staged_barrier();
-        stage(b, kb + 2);
-        // of the next SC steps' scales the part that this step stages
-        scales((kb / SC + 1) & 1, (kb / SC + 1) * SC, kb % SC * C::XI / SC);
+    for (int i = 0; i < T; ++i) {
+      const int t = i / C::WN, u = i % C::WN;          // a tile, and in p the one before it
+      const int p = (i + T - 1) % T;
+      const bool last = t + 1 == C::WM;
+      if (last && u == 0) {
+        staged_barrier<(C::ST - 2) * PIECES>();
         __builtin_amdgcn_sched_barrier(0);
       }
+      // the next row tile's operands are read between the products, a few at a time
+      v16f z;
 #pragma unroll
-      for (int u = 0; u < C::WN; ++u) {
-        tile(t * C::WN + u);
-        if (t + 1 == C::WM) read_w(b ^ 1, u);
-        if (u == 0) {
-          if (t + 1 < C::WM) read_x(b, kb, t + 1);
-          else read_x(b ^ 1, kb + 1, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+      for (int k = 0; k < 16; ++k) z[k] = 0.f;
+      // the depth's second half goes first in every other tile: x1 is free again one product sooner
+      const int h0 = u & 1, h1 = 1 - h0;
+      d[i & 1] = mfma32(a[u][h0], h0 ? x1 : x0[t % C::SLOTS], z);
+      // (the loop's first product waits for every read before it: none of the new ones)
+      if (i == 0) __builtin_amdgcn_sched_barrier(0);
+      if (last) read_w(bn, u, h0);
+      if (u == 0) read_x(last ? bn : b, last ? 0 : t + 1, 0);
+      else read_x(last ? bn : b, last ? 0 : t + 1, 1);
+      // just ahead of the barrier, which waits for it: a scalar load's wait is one for all LDS reads
+      if (i == T - C::WN - 1) wsn = wsr[min(kb + 1, nkg - 1)];
+      __builtin_amdgcn_sched_barrier(0);
+      d[i & 1] = mfma32(a[u][h1], h1 ? x1 : x0[t % C::SLOTS], d[i & 1]);
+      if (last) read_w(bn, u, h1);
+      if (u == 0) {
+        f[t % C::SLOTS] = wsc * sx;
+        read_s(last ? kb + 1 : kb, last ? 0 : t + 1);
       }
+      const int q = (i + C::WN) % T;                   // tiles since the barrier
+#pragma unroll
+      for (int j = q * PER; j < (q + 1) * PER && j < PIECES; ++j)
+        piece(last ? b : bp, last ? kb + C::ST : kb - 1 + C::ST, j);
+      __builtin_amdgcn_sched_barrier(0x3f4);
+      acc[p / C::WN][p % C::WN] = __builtin_elementwise_fma(
+          d[(i + 1) & 1], (v16f)(f[p / C::WN % C::SLOTS]), acc[p / C::WN][p % C::WN]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    wsc = wsr[min(kb + 1, nkg - 1)];
+    wsc = wsn;
   };
-  static_assert(C::WM % 2 == 0, "x alternates over a step's row tiles");
+  static_assert(C::WM > 1 && C::WN == 2, "a row tile's operands are read while the one before is used");
 #pragma unroll
   for (int i = 0; i < C::XI; ++i) scales(0, 0, i);
-  stage(0, 0);
-  stage(1, 1);
-  staged_barrier();
-  wsc = wsr[0];
 #pragma unroll
-  for (int u = 0; u < C::WN; ++u) read_w(0, u);
-  read_x(0, 0, 0);
+  for (int i = 0; i < C::ST; ++i)
+#pragma unroll
+    for (int j = 0; j < PIECES - 1; ++j)
+      if (i + 1 < C::ST || j < C::WN * PER) piece(i, i, j);
+  staged_barrier();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int u = 0; u < C::WN; ++u) read_w(0, u, h);
+    read_x(0, 0, h);
+  }
+  read_s(0, 0);
 #pragma unroll
   for (int k = 0; k < 16; ++k) d[1][k] = 0.f;
-  f[0] = f[1] = 0.f;
-  for (int kb = 0; kb < nkg; ++kb) step(kb & 1, kb);
-#pragma unroll
-  for (int k = 0; k < 16; ++k)
-    acc[C::WM - 1][C::WN - 1][k] =
-        fmaf(d[(C::WM * C::WN - 1) & 1][k], f[(C::WM - 1) & 1], acc[C::WM - 1][C::WN - 1][k]);
+  f[(C::WM - 1) % C::SLOTS] = 0.f;
+  for (int kb = 0, bp = C::ST - 1, b = 0; kb < nkg; ++kb) {
+    const int bn = b + 1 == C::ST ? 0 : b + 1;
+    step(bp, b, bn, kb);
+    bp = b;
+    b = bn;
+  }
+  acc[C::WM - 1][C::WN - 1] = __builtin_elementwise_fma(
+      d[(T - 1) & 1], (v16f)(f[(C::WM - 1) % C::SLOTS]), acc[C::WM - 1][C::WN - 1]);
   // lane: row r of a tile, columns 8 (i / 4) + 4 g + i % 4. Through LDS (each wave its own part) to
   // whole 16-byte pieces of a row; a row's piece q lies at q ^ (row % CH)
   constexpr int CH = 4 * C::WN;
@@ -212,14 +234,15 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
     for (int u = 0; u < C::WN; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float* v = &acc[t][u][4 * i];
-        const uint2 p = {f32_to_bf16(v[0]) | (uint32_t)f32_to_bf16(v[1]) << 16,
-                         f32_to_bf16(v[2]) | (uint32_t)f32_to_bf16(v[3]) << 16};
+        const v16f& v = acc[t][u];
+        const uint2 p = {f32_to_bf16(v[4 * i]) | (uint32_t)f32_to_bf16(v[4 * i + 1]) << 16,
+                         f32_to_bf16(v[4 * i + 2]) | (uint32_t)f32_to_bf16(v[4 * i + 3]) << 16};
         *reinterpret_cast<uint2*>(le + (t * 32 + r) * (CH * 16) +
                                   (((u * 4 + i) ^ r) & (CH - 1)) * 16 + g * 8) = p;
       }
   wave_lds_sync();
-  const int row0 = m0 + wm * C::WM * 32, col0 = n0 + wn * C::WN * 32;
+  const long long row0 = m0 + wm * C::WM * 32;
+  const int col0 = n0 + wn * C::WN * 32;
   if (ldy % 8 == 0 && (uintptr_t)y % 16 == 0) {
 #pragma unroll
     for (int i = 0; i < C::WM * 32 * CH / WAVE; ++i) {
@@ -228,22 +251,28 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
       uint16_t* o = y + (row0 + row) * ldy + col0 + q * 8;
       if (row0 + row < M) {
         if (col0 + q * 8 + 8 <= n) {
-          *reinterpret_cast<v4u*>(o) = p;
+          __builtin_nontemporal_store(p, reinterpret_cast<v4u*>(o));
         } else {
           for (int k = 0; col0 + q * 8 + k < n; ++k) o[k] = (uint16_t)(p[k / 2] >> (k % 2 * 16));
         }
       }
     }
   } else {
-    constexpr int RW = WAVE / (CH * 8) > 0 ? WAVE / (CH * 8) : 1;   // rows a pass
-    for (int i = 0; i < C::WM * 32 / RW; ++i)
+    // rows at odd addresses: a lane a column, so that a row's part is still one piece
+    static_assert(CH * 8 == WAVE, "a column a lane");
+    const bool in = col0 + lane < n;
+    uint16_t* o = y + row0 * ldy + col0 + lane;
 #pragma unroll
-      for (int c = lane % (CH * 8); c < CH * 8; c += WAVE) {
-        const int row = i * RW + lane / (CH * 8);
-        const uint16_t v = *reinterpret_cast<const uint16_t*>(
-            le + row * (CH * 16) + (((c / 8) ^ row) & (CH - 1)) * 16 + c % 8 * 2);
-        if (row0 + row < M && col0 + c < n) y[(row0 + row) * ldy + col0 + c] = v;
-      }
+    for (int i = 0; i < C::WM * 32; i += 16) {
+      uint16_t v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        v[k] = *reinterpret_cast<const uint16_t*>(
+            le + (i + k) * (CH * 16) + (((lane / 8) ^ (i + k)) & (CH - 1)) * 16 + lane % 8 * 2);
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (in && row0 + i + k < M) o[(i + k) * ldy] = v[k];
+    }
   }
 }
 
@@ -258,6 +287,17 @@ static int launch(hipStream_t st, const uint8_t* qx, const float* xs, const uint
   return (int)hipGetLastError();
 }
 
+typedef Cfg<4, 2, 2, 4, 2> Big;        // 256 x 256, one workgroup a CU
+typedef Cfg<3, 2, 2, 4, 2> Mid;        // 192 x 256, one
+typedef Cfg<2, 2, 2, 2, 2> Small;      // 128 x 128, two
+
+// tiles of a shape that the fullest CU gets
+template <class C>
+static long long per_cu(int M, int n) {
+  const long long t = (long long)((M + C::BM - 1) / C::BM) * ((n + C::BN - 1) / C::BN);
+  return (t + device_cus() - 1) / device_cus();
+}
+
 }  // namespace dense
 }  // namespace rlu
 
@@ -265,11 +305,37 @@ extern "C" int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void
                                      const float* ws, void* y, long long ldy, int M, int n,
                                      int K, hipStream_t stream) {
   using namespace rlu;
-  if (M < 0 || n < 1 || K < 1 || ldy < n) return -1;
-  if (K % 128) return -2;
+  if (M < 0 || n < 1 || K < 1 || ldy < n || n > INT32_MAX - 256 || M > INT32_MAX - 256) return -1;
+  if (K % 128 || K > (1 << 22)) return -2;
   if (M == 0) return 0;
   if (!qx || !xs || !w || !ws || !y) return -1;
   const auto* q = (const uint8_t*)qx;
   const auto* p = (const uint8_t*)w;
-  return dense::launch<dense::Cfg<4, 2, 2, 4>>(stream, q, xs, p, ws, (uint16_t*)y, ldy, M, n, K);
+  auto* o = (uint16_t*)y;
+  // Which kernel: the least of these estimates in us, each of a round of the CUs (fixed part, a 128-deep
+  // step's) as measured. Tiles, with every CU busy: Big 8 + 1.6, Mid 6.5 + 1.22, Small 4 + 0.55 alone
+  // on its CU and 6 + 0.95 for two. The head's kernel, 64 rows x 64 columns and a K split over its waves:
+  // 3.7 + 1.35 for a wave's steps.
+  //   rows x n x K           head / Big / Mid / Small (us)
+  //   256 x 2560 x 2560      10.5 / 28.5 / 24.9 / 15.2    1024 x 2560     24 / 29 / 25.6 / 16
+  //   4096 x 2560 x 2560     - / 34 / 31 / 39             2048 x 10240    - / 69 / 64 / 70
+  //   128 x 151936 x 2560    192 / 119 / 114 / 104        160 x 151936    270 / 126 / 117 / 141
+  //   256 x 151936 x 2560    373 / 138 / 173 / 158        512 x 32000     118 / 36 / 50 / 43
+  // Up to 64 rows the head's kernel reads the weights once, as it does for gemm_fp8_block.
+  const int steps = K / 128, sk = head::sk_of(K);
+  if (M <= 64 && sk) return head::rows(q, xs, p, ws, o, ldy, M, n, K, stream);
+  const double ns = (double)dense::per_cu<dense::Small>(M, n);
+  const double big = dense::per_cu<dense::Big>(M, n) * (8 + 1.6 * steps);
+  const double mid = dense::per_cu<dense::Mid>(M, n) * (6.5 + 1.22 * steps);
+  const double small = (long long)ns / 2 * (6 + 0.95 * steps) + (long long)ns % 2 * (4 + 0.55 * steps);
+  const double tile = small < mid ? (small < big ? small : big) : mid < big ? mid : big;
+  if (sk && M <= 65535 * 64) {
+    const long long items = (n + 127) / 128 * 2, wgs = (items * sk + 3) / 4 * ((M + 63) / 64);
+    if ((double)((wgs + device_cus() - 1) / device_cus()) * (3.7 + 1.35 * (steps / sk)) < tile)
+      return head::rows(q, xs, p, ws, o, ldy, M, n, K, stream);
+  }
+  if (tile == small)
+    return dense::launch<dense::Small>(stream, q, xs, p, ws, o, ldy, M, n, K);
+  if (tile == mid) return dense::launch<dense::Mid>(stream, q, xs, p, ws, o, ldy, M, n, K);
+  return dense::launch<dense::Big>(stream, q, xs, p, ws, o, ldy, M, n, K);
 }

@@ -21,6 +21,7 @@
 
 #include "gemm_common.h"
 #include "gemm_item.h"
+#include "head.h"
 #include "numerics.h"
 #include "rlu.h"
 #include "wave.h"
@@ -40,14 +41,21 @@ __global__ __launch_bounds__(NW * WAVE, 2) void head_k(const uint8_t* __restrict
                                                     const float* __restrict__ xs,
                                                     const uint8_t* __restrict__ wq,
                                                     const float* __restrict__ ws,
-                                                    uint16_t* __restrict__ y, int M, int K,
-                                                    int N) {
+                                                    uint16_t* __restrict__ y, long long ldy,
+                                                    int M, int n, int K, int N) {
   constexpr int D = ring(MB);
   constexpr int IPG = NW / SK;                      // items per workgroup
   static_assert(NPW % SK == 0 && NW % SK == 0, "strips divide over the K splits");
   constexpr int BP = exchange(MB);
   constexpr int OWN = NPW / SK;                     // strips a wave finishes
   extern __shared__ float lds[];                    // scales [NW][nsteps][MB 16], then partials
+  {                                                 // this launch row's block of 64 rows
+    const int m0 = (int)blockIdx.y * 64;
+    qx += (size_t)m0 * K;
+    xs += (size_t)m0 * (K / 128);
+    y += m0 * ldy;
+    M = min(M - m0, 64);
+  }
   const int lane = lane_id();
   const int w = uniform((int)threadIdx.x / WAVE);
   const int sub = w / SK, ks = w % SK;
@@ -166,8 +174,8 @@ __global__ __launch_bounds__(NW * WAVE, 2) void head_k(const uint8_t* __restrict
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int row = 16 * b + 4 * c4 + i;
-          if (live && row < M) y[(size_t)row * N + n0 + s * 16 + r16] = f32_to_bf16(t[i]);
+          const int row = 16 * b + 4 * c4 + i, col = n0 + s * 16 + r16;
+          if (live && row < M && col < n) y[row * ldy + col] = f32_to_bf16(t[i]);
         }
       }
     }
@@ -176,19 +184,34 @@ __global__ __launch_bounds__(NW * WAVE, 2) void head_k(const uint8_t* __restrict
 
 template <int MB>
 static int launch(int sk, hipStream_t st, const uint8_t* qx, const float* xs, const uint8_t* wq,
-                  const float* ws, uint16_t* y, int M, int K, int N) {
+                  const float* ws, uint16_t* y, long long ldy, int M, int n, int K) {
   constexpr int D = ring(MB);
+  const int N = (n + 127) / 128 * 128;
   const int nsteps = (K / 128 / sk + D - 1) / D * D;
   const int items = N / (16 * NPW), ipg = NW / sk;
   const size_t lds = (size_t)NW * nsteps * MB * 64 + (sk > 1 ? NW * NPW * exchange(MB) * 1024 : 0);
 #define RLU_H(SK)                                                                            \
-  hipLaunchKernelGGL((head_k<MB, SK>), dim3((items + ipg - 1) / ipg), dim3(NW * WAVE), lds, \
-                     st, qx, xs, wq, ws, y, M, K, N)
+  hipLaunchKernelGGL((head_k<MB, SK>), dim3((items + ipg - 1) / ipg, (M + 63) / 64),         \
+                     dim3(NW * WAVE), lds, st, qx, xs, wq, ws, y, ldy, M, n, K, N)
   if (sk == 4) RLU_H(4);
   else if (sk == 2) RLU_H(2);
   else RLU_H(1);
 #undef RLU_H
   return (int)hipGetLastError();
+}
+
+// M rows (MB = 4 above 64: launch rows of 64) x n columns of w [n rounded up to 128, K]; sk_of(K) > 0.
+int sk_of(int K) {
+  const int nkg = K / 128, sk = nkg % 4 == 0 ? 4 : nkg % 2 == 0 ? 2 : 1;
+  return nkg / sk > MAXKPW ? 0 : sk;
+}
+int rows(const uint8_t* qx, const float* xs, const uint8_t* wq, const float* ws, uint16_t* y,
+         long long ldy, int M, int n, int K, hipStream_t st) {
+  const int sk = sk_of(K);
+  if (M <= 16) return launch<1>(sk, st, qx, xs, wq, ws, y, ldy, M, n, K);
+  if (M <= 32) return launch<2>(sk, st, qx, xs, wq, ws, y, ldy, M, n, K);
+  if (M <= 48) return launch<3>(sk, st, qx, xs, wq, ws, y, ldy, M, n, K);
+  return launch<4>(sk, st, qx, xs, wq, ws, y, ldy, M, n, K);
 }
 
 }  // namespace head
@@ -200,14 +223,8 @@ extern "C" int rlu_gemm_fp8blk_m64(const void* qx, const float* xs, const void* 
   using namespace rlu;
   if (M < 1 || M > 64 || K <= 0 || N <= 0) return -1;
   if (K % 128 || N % 128) return -2;
-  const int nkg = K / 128, sk = nkg % 4 == 0 ? 4 : nkg % 2 == 0 ? 2 : 1;
-  if (nkg / sk > MAXKPW) return -4;
+  if (!head::sk_of(K)) return -4;
   if (!qx || !xs || !w || !ws || !y) return -1;
-  const auto* q = (const uint8_t*)qx;
-  const auto* p = (const uint8_t*)w;
-  auto* o = (uint16_t*)y;
-  if (M <= 16) return head::launch<1>(sk, stream, q, xs, p, ws, o, M, K, N);
-  if (M <= 32) return head::launch<2>(sk, stream, q, xs, p, ws, o, M, K, N);
-  if (M <= 48) return head::launch<3>(sk, stream, q, xs, p, ws, o, M, K, N);
-  return head::launch<4>(sk, stream, q, xs, p, ws, o, M, K, N);
+  return head::rows((const uint8_t*)qx, xs, (const uint8_t*)w, ws, (uint16_t*)y, N, M, N, K,
+                    stream);
 }
