@@ -334,6 +334,23 @@ int rlu_moe_gemm_fp8blk_tiled_noalloc(const void* qx, const float* xs, const voi
                                       const float* topk_weights, void* y, int mtk, int top_k,
                                       int K, int N, int wv, hipStream_t stream);
 
+/* ---- scoring -------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose logits go to vLLM's sampler: for each of R rows of logits [R, V]
+ * (dtype 0 bf16, 1 f32, 2 f16; rows ld elements apart, at any element's address) the given token's log
+ * probability and rank (1 = the first), the entropy in nats, and the `top` largest log probabilities with
+ * their ids, ties by the lowest id. tokens int64 (wide 1) or int32 (wide 0).
+ *   -inf logits have probability 0. A row of nothing else: log probabilities -inf, entropy 0.
+ *   A row with a NaN or +inf: NaN, rank 0, ids -1.
+ *   A token below 0 asks for none: logprob 0, rank 0. One >= V: logprob NaN, rank 0.
+ * 1 <= V <= 500000, 0 <= top <= min(32, V). top_logprobs / top_ids [R, top] (NULL where top is 0). ws: what
+ * the first call says, 8-byte aligned, used until the second call's kernels end. R = 0 launches nothing.
+ * Returns -1 (bad sizes or a NULL pointer), -4 (misaligned logits). */
+int rlu_token_logprobs_workspace(int dtype, int R, int V, int top, long long* bytes);
+int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V,
+                       const void* tokens, int wide, int top, float* logprob, int* rank,
+                       float* entropy, float* top_logprobs, int* top_ids, void* ws,
+                       hipStream_t stream);
+
 /* Replaces the closed r4d_gemm_w4a16_nt_m64 behind draft_w4_lmhead_gemm / gemm_w4a16
  * (kernels/draft_w4_lmhead.py:351-403), in this build's gfx950 W4 format:
  *   y [M, N] bf16 = x [M, K] bf16 . (scale * (q - zero))^T, 1 <= M <= 16,

@@ -9,6 +9,7 @@ from . import _lib  # noqa: F401
 from ._lib import LIB_PATH, LibraryMissing, lib  # noqa: F401
 from .lru import (LruCache, _align_sizes, _r4d_lru_fused, _r4d_lru_gather,  # noqa: F401
                   _r4d_lru_manage)
+from . import logprobs  # noqa: F401
 from . import ops  # noqa: F401
 from . import hot_profile  # noqa: F401
 from . import routecap  # noqa: F401

@@ -5,6 +5,7 @@ caller can never silently run anything but the HIP kernels.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -37,6 +38,8 @@ SIGNATURES: dict[str, tuple] = {
     "rlu_shuffle_fp8_weight": (_I, [_P, _P, _LL, _I, _P]),
     "rlu_gemm_fp8blk_m64": (_I, [_P] * 5 + [_I] * 3 + [_P]),
     "rlu_gemm_fp8blk_dense": (_I, [_P] * 5 + [_LL] + [_I] * 3 + [_P]),
+    "rlu_token_logprobs_workspace": (_I, [_I] * 4 + [_P]),
+    "rlu_token_logprobs": (_I, [_P, _I, _LL, _I, _I, _P, _I, _I] + [_P] * 7),
     "rlu_gemm_w4_m16": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _P]),
     "rlu_gemm_w4_m64": (_I, [_P, _I, _I, _P, _P, _P, _I, _P]),
     "rlu_pack_w4": (_I, [_P, _I, _LL, _I, _I, _I, _P, _P, _P]),
@@ -85,6 +88,16 @@ def stream_ptr(stream=None) -> int:
     import torch
     s = torch.cuda.current_stream() if stream is None else stream
     return s.cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which `device` is the current one (nothing to do where it is already: entering
+    torch.cuda.device costs 2 us a call)."""
+    import torch
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def check(rc: int, what: str) -> None:

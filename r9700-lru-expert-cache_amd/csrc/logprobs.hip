@@ -1,0 +1,468 @@
+// Log probabilities of given tokens, with rank, entropy and the n largest alternatives, in one read of
+// the logits. With m = max x, Z = sum e^(x - m):
+//   logprob = x_t - m - ln Z, entropy = ln Z - sum (x - m) e^(x - m) / Z,
+//   rank = 1 + #{x > x_t} + #{j < t: x_j = x_t}, alternatives by value, the lowest index first.
+#include <float.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "rlu.h"
+#include "wave.h"
+
+namespace rlu {
+namespace lp {
+
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+constexpr int NT = 256, NW = NT / WAVE;    // threads and waves of a segment's workgroup
+constexpr int MAX_TOP = 32, MAX_V = 500000;
+constexpr int MAX_SEGS = WAVE;             // a row's segments, one to a lane of the joining wave
+constexpr int CAP = 256;                   // candidates a wave lists
+constexpr float L2E = 1.44269504f;
+constexpr double LN2 = 0.693147180559945309;
+
+// What a segment leaves of a row: its maximum, sum e^(x - m) - 1 (the maximum's own 1 left out: a nearly
+// certain row's small terms would be lost beside it), sum log2(e^(x - m)) e^(x - m), and how many of its logits
+// come before the token's. A segment of nothing: -inf, -1, 0.
+struct Part {
+  float m, rest, t;
+  int before;
+};
+
+template <int DT>
+struct Elem;                               // 0 bf16, 1 f32, 2 f16: elements of 16 bytes, and the i-th
+template <>
+struct Elem<0> {
+  static constexpr int N = 8, SIZE = 2;
+  static constexpr uint32_t NINF = 0xff80;
+  static __device__ __forceinline__ float get(v4u v, int i) {
+    const uint32_t u = v[i / 2];
+    return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
+  }
+};
+template <>
+struct Elem<1> {
+  static constexpr int N = 4, SIZE = 4;
+  static constexpr uint32_t NINF = 0xff800000u;
+  static __device__ __forceinline__ float get(v4u v, int i) { return __uint_as_float(v[i]); }
+};
+template <>
+struct Elem<2> {
+  static constexpr int N = 8, SIZE = 2;
+  static constexpr uint32_t NINF = 0xfc00;
+  static __device__ __forceinline__ float get(v4u v, int i) {
+    const uint32_t u = v[i / 2];
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? u >> 16 : u));
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ float load_one(const uint8_t* row, long long i) {
+  const uint8_t* p = row + i * Elem<DT>::SIZE;
+  v4u v = {};
+  v[0] = Elem<DT>::SIZE == 4 ? *reinterpret_cast<const uint32_t*>(p)
+                             : *reinterpret_cast<const uint16_t*>(p);
+  return Elem<DT>::get(v, 0);
+}
+
+// unsigned keys in the order of the floats (the two zeros one), and back
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float(k ^ ((int)k < 0 ? 0x80000000u : 0xffffffffu));
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dppf(float v) {
+  return __int_as_float(dpp<CTRL>(__float_as_int(v), __float_as_int(v)));
+}
+__device__ __forceinline__ float lane_f(float v, int l) {
+  return __int_as_float(readlane(__float_as_int(v), l));
+}
+__device__ __forceinline__ float wave_max(float v) {   // wave-uniform; NaN only if all are
+  v = fmaxf(v, dppf<0xb1>(v));
+  v = fmaxf(v, dppf<0x4e>(v));
+  v = fmaxf(v, dppf<0x141>(v));
+  v = fmaxf(v, dppf<0x140>(v));
+  return fmaxf(fmaxf(lane_f(v, 0), lane_f(v, 16)), fmaxf(lane_f(v, 32), lane_f(v, 48)));
+}
+__device__ __forceinline__ float wave_add(float v) {   // wave-uniform, in a fixed order
+  v += dppf<0xb1>(v);
+  v += dppf<0x4e>(v);
+  v += dppf<0x141>(v);
+  v += dppf<0x140>(v);
+  return (lane_f(v, 0) + lane_f(v, 16)) + (lane_f(v, 32) + lane_f(v, 48));
+}
+
+__device__ __forceinline__ long long token_of(const void* tokens, int wide, int row) {
+  return wide ? ((const long long*)tokens)[row] : ((const int*)tokens)[row];
+}
+
+// The compiler forgets what it unpacked: unpacking again costs one instruction an element, keeping the
+// floats 64 registers.
+template <int CV>
+__device__ __forceinline__ void forget(v4u (&raw)[CV]) {
+#pragma unroll
+  for (int k = 0; k < CV; ++k) asm volatile("" : "+v"(raw[k]));
+}
+
+// The sums of a thread's CV vectors against c = RN(m log2 e). skip: leaves out one element equal to m.
+template <int DT, int CV, bool SKIP>
+__device__ __forceinline__ void sums(const v4u (&raw)[CV], float c, float m, bool skip, float& s,
+                                     float& t) {
+  s = t = 0.f;
+#pragma unroll
+  for (int k = 0; k < CV; ++k)
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::N; ++i) {
+      float x = Elem<DT>::get(raw[k], i);
+      if (SKIP && skip && x == m) {
+        x = -__builtin_inff();
+        skip = false;
+      }
+      const float y = fmaf(x, L2E, -c);
+      const float e = __builtin_amdgcn_exp2f(y);
+      s += e;
+      t = fmaf(fmaxf(y, -200.f), e, t);    // (-inf times its zero)
+    }
+}
+
+// One segment of one row: NT threads hold its CV * NT vectors of 16 bytes.
+template <int DT, int CV, bool TOP>
+__global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logits, long long ld,
+                                                int V, int nseg, const void* __restrict__ tokens,
+                                                int wide, int top, Part* __restrict__ parts,
+                                                uint64_t* __restrict__ lists) {
+  typedef Elem<DT> E;
+  __shared__ float rmax[NW], rfrom[NW], rs[2][NW], rt[2][NW];
+  __shared__ int rbefore[NW], rcount[NW], rhas[NW];
+  __shared__ uint64_t list[TOP ? NW : 1][TOP ? CAP : 1], rkey[NW];
+  const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE);
+  const int row = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
+  const uint8_t* p = logits + (size_t)row * ld * E::SIZE;
+  // vectors from the aligned address at or below the row's start on; index = v N + i - shift
+  const int shift = (int)((uintptr_t)p % 16) / E::SIZE;
+  const v4u* pv = reinterpret_cast<const v4u*>(p - shift * E::SIZE);
+  const int nvec = (shift + V + E::N - 1) / E::N, v0 = seg * CV * NT;
+  v4u raw[CV];
+#pragma unroll
+  for (int k = 0; k < CV; ++k) {
+    const int v = v0 + k * NT + tid;
+    if (v < nvec) {
+      raw[k] = __builtin_nontemporal_load(pv + v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[k][j] = E::SIZE == 4 ? E::NINF : E::NINF * 0x10001u;
+    }
+  }
+  auto entry = [&](float x, int k, int i) {            // by value, then the lowest index
+    return (uint64_t)key_of(x) << 32 | ~(uint32_t)((v0 + k * NT + tid) * E::N + i - shift);
+  };
+  const long long tok = token_of(tokens, wide, row);
+  const bool asked = tok >= 0 && tok < V;
+  const float xt = asked ? load_one<DT>(p, tok) : __builtin_inff();
+#pragma unroll
+  for (int k = 0; k < CV; ++k) {           // elements of the neighbours in a row's end vectors
+    const int v = v0 + k * NT + tid;
+    if ((v == 0 && shift) || v == nvec - 1)
+#pragma unroll
+      for (int i = 0; i < E::N; ++i) {
+        const int j = v * E::N + i - shift;
+        if (j < 0 || j >= V) {
+          if (E::SIZE == 4) raw[k][i] = E::NINF;
+          else raw[k][i / 2] = i % 2 ? (raw[k][i / 2] & 0xffffu) | E::NINF << 16
+                                     : (raw[k][i / 2] & 0xffff0000u) | E::NINF;
+        }
+      }
+  }
+  float tm = -__builtin_inff();
+#pragma unroll
+  for (int k = 0; k < CV; ++k)
+#pragma unroll
+    for (int i = 0; i < E::N; ++i) tm = fmaxf(tm, E::get(raw[k], i));
+  forget(raw);
+  const float wm = wave_max(tm);
+  if (lane == 0) rmax[w] = wm;
+  if (TOP) {
+    // a value that `top` of the wave's 64 threads have an element at or above: the upper 16 bits of the
+    // top-th largest of their maxima, bit by bit
+    const uint32_t k16 = key_of(tm) >> 16;
+    uint32_t at = 0;
+#pragma unroll
+    for (int b = 15; b >= 0; --b) {
+      const uint32_t c = at | 1u << b;
+      if (__popcll(__ballot(k16 >= c)) >= top) at = c;
+    }
+    if (lane == 0) rfrom[w] = at > 0x7fu ? of_key(at << 16) : -FLT_MAX;   // (finite ones only)
+  }
+  __syncthreads();
+  float m = rmax[0];
+#pragma unroll
+  for (int k = 1; k < NW; ++k) m = fmaxf(m, rmax[k]);
+  const float c = m == -__builtin_inff() ? 0.f : m * L2E;
+  float s, t;
+  sums<DT, CV, false>(raw, c, m, false, s, t);
+  forget(raw);
+  int before = 0;
+  if (m >= xt) {
+    const long long tv = (tok + shift) / E::N;
+#pragma unroll
+    for (int k = 0; k < CV; ++k) {
+      const int vw = v0 + k * NT + w * WAVE;           // the wave's first vector
+      if (vw + WAVE <= tv) {
+#pragma unroll
+        for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) >= xt));
+        if (vw == 0 && !(xt > -__builtin_inff())) before -= shift;      // not a neighbour's place
+      } else if (vw > tv) {
+#pragma unroll
+        for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) > xt));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E::N; ++i) {
+          const long long j = (long long)(vw + lane) * E::N + i - shift;
+          const float x = E::get(raw[k], i);
+          before += __popcll(__ballot(x > xt || (x == xt && j >= 0 && j < tok)));
+        }
+      }
+    }
+  }
+  forget(raw);
+  if (TOP) {
+    float from = rfrom[0];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) from = fmaxf(from, rfrom[k]);
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < CV; ++k)
+#pragma unroll
+      for (int i = 0; i < E::N; ++i) {
+        const float x = E::get(raw[k], i);
+        const uint64_t in = __ballot(x >= from);
+        if (in) {
+          const int at = count + mbcnt(in);
+          if (x >= from && at < CAP) list[w][at] = entry(x, k, i);
+          count += __popcll(in);
+        }
+      }
+    if (lane == 0) rcount[w] = count;
+  }
+  forget(raw);
+  s = wave_add(s);
+  t = wave_add(t);
+  if (lane == 0) {
+    rs[0][w] = s;
+    rt[0][w] = t;
+    rbefore[w] = before;
+    rhas[w] = 0;
+  }
+  __syncthreads();
+  s = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]);
+  t = (rt[0][0] + rt[0][1]) + (rt[0][2] + rt[0][3]);
+  const float r = fmaf(m, L2E, -c);        // log2 of the maximum's own term: c is rounded
+  const float unit = __builtin_amdgcn_exp2f(-r);
+  float rest = m > -__builtin_inff() ? s * unit - 1.f : s - 1.f;
+  if (m > -__builtin_inff() && s < 1.5f) {             // nearly certain: the sums without the maximum
+    forget(raw);
+    const uint64_t has = __ballot(tm == m);
+    if (lane == 0 && has) rhas[w] = 1;
+    __syncthreads();
+    const int first = rhas[0] ? 0 : rhas[1] ? 1 : rhas[2] ? 2 : 3;
+    sums<DT, CV, true>(raw, c, m, w == first && lane == __ffsll((unsigned long long)has) - 1, s, t);
+    s = wave_add(s);
+    t = wave_add(t);
+    if (lane == 0) {
+      rs[1][w] = s;
+      rt[1][w] = t;
+    }
+    __syncthreads();
+    s = (rs[1][0] + rs[1][1]) + (rs[1][2] + rs[1][3]);
+    t = (rt[1][0] + rt[1][1]) + (rt[1][2] + rt[1][3]);
+    rest = s * unit;
+  }
+  if (tid == 0) {
+    Part o;
+    o.m = m;
+    o.rest = rest;
+    o.t = m > -__builtin_inff() ? (t - r * s) * unit : 0.f;
+    o.before = rbefore[0] + rbefore[1] + rbefore[2] + rbefore[3];
+    parts[blockIdx.x] = o;
+  }
+  if (TOP) {
+    uint64_t* out = lists + (size_t)blockIdx.x * top;
+    int total = 0, most = 0;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      total += rcount[k];
+      most = max(most, rcount[k]);
+    }
+    if (most <= CAP) {                     // each candidate's place is how many come before it
+      for (int j = lane; j < rcount[w]; j += WAVE) {
+        const uint64_t key = list[w][j];
+        int place = 0;
+#pragma unroll
+        for (int k = 0; k < NW; ++k)
+          for (int l = 0; l < rcount[k]; ++l) place += list[k][l] > key;
+        if (place < top) out[place] = key;
+      }
+      if (tid >= total && tid < top) out[tid] = 0;
+    } else {                               // long runs of equal logits: one after the other
+      uint64_t last = ~0ull;
+      for (int n = 0; n < top; ++n) {
+        uint64_t best = 0;
+        forget(raw);
+        if (last)
+#pragma unroll
+          for (int k = 0; k < CV; ++k)
+#pragma unroll
+            for (int i = 0; i < E::N; ++i) {
+              const float x = E::get(raw[k], i);
+              const uint64_t key = x >= -FLT_MAX ? entry(x, k, i) : 0;
+              best = key < last && key > best ? key : best;
+            }
+        best = wave_reduce64(best, OpMax64());
+        if (lane == 0) rkey[w] = best;
+        __syncthreads();
+        OpMax64 op;
+        last = op(op(rkey[0], rkey[1]), op(rkey[2], rkey[3]));
+        if (tid == 0) out[n] = last;
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// Joins a row's segments: one wave a row. parts [R][nseg], lists [R][nseg][top] in falling order, 0 behind
+// the last.
+template <int DT>
+__global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logits, long long ld,
+                                               int V, int nseg, const void* __restrict__ tokens,
+                                               int wide, int top, const Part* __restrict__ parts,
+                                               const uint64_t* __restrict__ lists,
+                                               float* __restrict__ logprob, int* __restrict__ rank,
+                                               float* __restrict__ entropy,
+                                               float* __restrict__ top_logprobs,
+                                               int* __restrict__ top_ids) {
+  extern __shared__ uint64_t heads[];      // [nseg][top]
+  const int lane = lane_id(), row = (int)blockIdx.x;
+  const float ninf = -__builtin_inff(), nan = __builtin_nanf("");
+  const uint8_t* p = logits + (size_t)row * ld * Elem<DT>::SIZE;
+  Part q = {ninf, -1.f, 0.f, 0};
+  if (lane < nseg) q = parts[(size_t)row * nseg + lane];
+  for (int i = lane; i < nseg * top; i += WAVE) heads[i] = lists[(size_t)row * nseg * top + i];
+  const long long tok = token_of(tokens, wide, row);
+  const float xt = tok >= 0 && tok < V ? load_one<DT>(p, tok) : 0.f;
+  const float m = wave_max(q.m);
+  const bool none = m == ninf;
+  // the segment of the maximum keeps its rest, the others add all they have
+  const uint64_t has = __ballot(q.m == m);
+  const bool ref = lane == __ffsll((unsigned long long)has) - 1;
+  const float d = (q.m - m) * L2E, a = __builtin_amdgcn_exp2f(d);
+  float rest = q.rest, t = q.t;
+  if (!ref) {
+    rest = q.m > ninf ? a * (1.f + q.rest) : q.rest + 1.f;              // (a NaN stays)
+    t = q.m > ninf ? a * fmaf(d, 1.f + q.rest, q.t) : 0.f;
+  }
+  rest = wave_add(rest);
+  t = wave_add(t);
+  const int before = wave_sum(q.before);
+  const bool bad = rest != rest;
+  const float lz = none ? 0.f : log1pf(rest);
+  auto score = [&](float x) { return bad ? nan : none ? ninf : (x - m) - lz; };
+  if (lane == 0) {
+    const bool in = tok >= 0 && tok < V;
+    logprob[row] = tok < 0 ? 0.f : in ? score(xt) : nan;
+    rank[row] = in && !bad ? 1 + before : 0;
+    entropy[row] = bad ? nan : none ? 0.f : lz - (float)LN2 * t / (1.f + rest);
+  }
+  if (top == 0) return;
+  wave_lds_sync();
+  uint64_t head = lane < nseg ? heads[lane * top] : 0, mine = 0;
+  int next = 1, found = 0;
+  for (; found < top; ++found) {
+    const uint64_t best = wave_reduce64(head, OpMax64());
+    if (best == 0) break;
+    if (lane == found) mine = best;
+    if (head == best) head = next < top ? heads[lane * top + next++] : 0;
+  }
+  float* ol = top_logprobs + (size_t)row * top;
+  int* oi = top_ids + (size_t)row * top;
+  if (bad) {
+    if (lane < top) {
+      ol[lane] = nan;
+      oi[lane] = -1;
+    }
+    return;
+  }
+  if (lane < found) {
+    ol[lane] = score(of_key((uint32_t)(mine >> 32)));
+    oi[lane] = (int)~(uint32_t)mine;
+  }
+  if (found < top) {                       // fewer finite ones: the first at -inf, all among 64
+    const bool at = lane < V && load_one<DT>(p, lane) == ninf;
+    const int place = found + mbcnt(__ballot(at));
+    if (at && place < top) {
+      ol[place] = ninf;
+      oi[place] = lane;
+    }
+  }
+}
+
+// Vectors a thread holds, and segments of a row: the longest that leave no CU without work.
+struct Plan {
+  int cv, nseg;
+};
+static Plan plan(int dtype, int R, int V) {
+  const int n = dtype == 1 ? 4 : 8;
+  const int chunks = (V + 2 * n - 2) / n / NT + 1;     // of NT vectors, wherever the row starts
+  Plan p = {8, 0};
+  for (;; p.cv /= 2) {
+    p.nseg = (chunks + p.cv - 1) / p.cv;
+    const int half = (chunks + p.cv / 2 - 1) / (p.cv / 2 > 0 ? p.cv / 2 : 1);
+    if (p.cv == 1 || half > MAX_SEGS || (long long)R * p.nseg >= 512) return p;
+  }
+}
+
+}  // namespace lp
+}  // namespace rlu
+
+extern "C" int rlu_token_logprobs_workspace(int dtype, int R, int V, int top, long long* bytes) {
+  using namespace rlu::lp;
+  if (!bytes || dtype < 0 || dtype > 2 || R < 0 || V < 1 || V > MAX_V || top < 0 ||
+      top > MAX_TOP || top > V)
+    return -1;
+  const long long segs = (long long)R * plan(dtype, R, V).nseg;
+  if (segs > INT32_MAX) return -1;
+  *bytes = segs * (sizeof(Part) + 8 * top);
+  return 0;
+}
+
+extern "C" int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V,
+                                  const void* tokens, int wide, int top, float* logprob, int* rank,
+                                  float* entropy, float* top_logprobs, int* top_ids, void* ws,
+                                  hipStream_t stream) {
+  using namespace rlu::lp;
+  long long bytes;
+  if (rlu_token_logprobs_workspace(dtype, R, V, top, &bytes)) return -1;
+  if (ld < 0 || (wide != 0 && wide != 1)) return -1;
+  if (R == 0) return 0;
+  if (!logits || !tokens || !logprob || !rank || !entropy || !ws) return -1;
+  if (top && (!top_logprobs || !top_ids)) return -1;
+  if ((uintptr_t)logits % (dtype == 1 ? 4 : 2)) return -4;
+  const Plan pl = plan(dtype, R, V);
+  const auto* x = (const uint8_t*)logits;
+  auto* lists = (uint64_t*)ws;                         // (8-byte entries first: both aligned)
+  auto* parts = (Part*)(lists + (size_t)R * pl.nseg * top);
+  const dim3 grid((unsigned)(R * pl.nseg));
+#define RLU_SEG(DT, CV, TOP)                                                                       hipLaunchKernelGGL((segment_k<DT, CV, TOP>), grid, dim3(NT), 0, stream, x, ld, V, pl.nseg,                          tokens, wide, top, parts, lists)
+#define RLU_CV(DT, TOP)                 do {                                    if (pl.cv == 8) RLU_SEG(DT, 8, TOP);          else if (pl.cv == 4) RLU_SEG(DT, 4, TOP);     else if (pl.cv == 2) RLU_SEG(DT, 2, TOP);     else RLU_SEG(DT, 1, TOP);                   } while (0)
+#define RLU_DT(DT)                                                                                do {                                                                                              if (top) RLU_CV(DT, true);                                                                      else RLU_CV(DT, false);                                                                         hipLaunchKernelGGL((join_k<DT>), dim3((unsigned)R), dim3(rlu::WAVE), pl.nseg * top * 8,                            stream, x, ld, V, pl.nseg, tokens, wide, top, parts, lists, logprob, rank,                        entropy, top_logprobs, top_ids);                                           } while (0)
+  if (dtype == 0) RLU_DT(0);
+  else if (dtype == 1) RLU_DT(1);
+  else RLU_DT(2);
+#undef RLU_DT
+#undef RLU_CV
+#undef RLU_SEG
+  return (int)hipGetLastError();
+}

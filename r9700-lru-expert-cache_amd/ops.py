@@ -27,7 +27,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, device_ptr, lib, stream_ptr
+from ._lib import check, device_ptr, lib, on_device, stream_ptr
 
 _P = ctypes.c_void_p
 FP8 = torch.float8_e4m3fn
@@ -372,7 +372,7 @@ def pack_fp8_dense(w: torch.Tensor, ws: torch.Tensor) -> PackedFp8:
                          "beside the weight")
     rows = torch.zeros((nb * GROUP, k), dtype=torch.uint8, device=w.device)
     rows[:n] = w.view(torch.uint8)
-    with torch.cuda.device(w.device):
+    with on_device(w.device):
         wq = shuffle_fp8_weight(rows.view(FP8))
     return PackedFp8(wq=wq, ws=ws.contiguous(), n=n, k=k)
 
@@ -396,7 +396,7 @@ def gemm_fp8_dense(qx: torch.Tensor, xs: torch.Tensor, w: PackedFp8,
     if not xs.device == w.wq.device == w.ws.device == out.device == qx.device:
         raise ValueError("gemm_fp8_dense: operands on different devices")
     ldy = out.stride(0) if M > 1 else w.n
-    with torch.cuda.device(qx.device):
+    with on_device(qx.device):
         rc = lib().rlu_gemm_fp8blk_dense(_p(qx), _p(xs), _p(w.wq), _p(w.ws), _p(out), ldy, M, w.n,
                                          K, _P(stream_ptr()))
     check(rc, "rlu_gemm_fp8blk_dense")
