@@ -17,7 +17,7 @@ typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 constexpr int NT = 256, NW = NT / WAVE;    // threads and waves of a segment's workgroup
 constexpr int MAX_TOP = 32, MAX_V = 500000;
 constexpr int MAX_SEGS = WAVE;             // a row's segments, one to a lane of the joining wave
-constexpr int CAP = 256;                   // candidates a wave lists
+constexpr int BATCH = 16, CAP = 256;       // threads a wave lists from at a time, candidates it lists
 constexpr float L2E = 1.44269504f;
 constexpr double LN2 = 0.693147180559945309;
 
@@ -54,6 +54,48 @@ struct Elem<2> {
     const uint32_t u = v[i / 2];
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? u >> 16 : u));
   }
+};
+
+// A thread's maximum over its vectors.
+template <int DT, int CV>
+struct Max {
+  static __device__ __forceinline__ float of(const v4u (&raw)[CV]) {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < CV; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(raw[k][i]));
+    return m;
+  }
+};
+// Of 16-bit floats without unpacking them: as signed integers they are in order from 0 up, and where none
+// is up there the least unsigned one is the largest. (A NaN may or may not come out.)
+typedef short v2s __attribute__((ext_vector_type(2)));
+typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+template <int DT, int CV>
+__device__ __forceinline__ float packed_max(const v4u (&raw)[CV]) {
+  v2s hi = __builtin_bit_cast(v2s, (uint32_t)raw[0][0]);
+  v2us lo = __builtin_bit_cast(v2us, (uint32_t)raw[0][0]);
+#pragma unroll
+  for (int k = 0; k < CV; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi = __builtin_elementwise_max(hi, __builtin_bit_cast(v2s, (uint32_t)raw[k][i]));
+      lo = __builtin_elementwise_min(lo, __builtin_bit_cast(v2us, (uint32_t)raw[k][i]));
+    }
+  const short h = hi[0] > hi[1] ? hi[0] : hi[1];
+  const unsigned short l = lo[0] < lo[1] ? lo[0] : lo[1];
+  v4u v = {};
+  v[0] = h >= 0 ? (uint16_t)h : l;
+  return Elem<DT>::get(v, 0);
+}
+template <int CV>
+struct Max<0, CV> {
+  static __device__ __forceinline__ float of(const v4u (&raw)[CV]) { return packed_max<0>(raw); }
+};
+template <int CV>
+struct Max<2, CV> {
+  static __device__ __forceinline__ float of(const v4u (&raw)[CV]) { return packed_max<2>(raw); }
 };
 
 template <int DT>
@@ -108,16 +150,21 @@ __device__ __forceinline__ void forget(v4u (&raw)[CV]) {
   for (int k = 0; k < CV; ++k) asm volatile("" : "+v"(raw[k]));
 }
 
-// The sums of a thread's CV vectors against c = RN(m log2 e). skip: leaves out one element equal to m.
-template <int DT, int CV, bool SKIP>
-__device__ __forceinline__ void sums(const v4u (&raw)[CV], float c, float m, bool skip, float& s,
-                                     float& t) {
+// The sums of a thread's vectors, n of them, against c = RN(m log2 e).
+//   CLAMP: takes -inf (its product with its zero is a NaN without); SKIP: and leaves out one element
+//   equal to m where skip. COUNT: adds the wave's elements above thr(k) to before.
+template <int DT, int CV, bool CLAMP, bool SKIP, bool COUNT, class Thr>
+__device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, float m, bool skip,
+                                     Thr thr, float& s, float& t, int& before) {
   s = t = 0.f;
 #pragma unroll
-  for (int k = 0; k < CV; ++k)
+  for (int k = 0; k < CV; ++k) {
+    if (k >= n) continue;                              // (uniform)
+    const float above = COUNT ? thr(k) : 0.f;
 #pragma unroll
     for (int i = 0; i < Elem<DT>::N; ++i) {
       float x = Elem<DT>::get(raw[k], i);
+      if (COUNT) before += __popcll(__ballot(x > above));
       if (SKIP && skip && x == m) {
         x = -__builtin_inff();
         skip = false;
@@ -125,8 +172,9 @@ __device__ __forceinline__ void sums(const v4u (&raw)[CV], float c, float m, boo
       const float y = fmaf(x, L2E, -c);
       const float e = __builtin_amdgcn_exp2f(y);
       s += e;
-      t = fmaf(fmaxf(y, -200.f), e, t);    // (-inf times its zero)
+      t = fmaf(CLAMP ? fmaxf(y, -200.f) : y, e, t);
     }
+  }
 }
 
 // One segment of one row: NT threads hold its CV * NT vectors of 16 bytes.
@@ -136,9 +184,11 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
                                                 int wide, int top, Part* __restrict__ parts,
                                                 uint64_t* __restrict__ lists) {
   typedef Elem<DT> E;
-  __shared__ float rmax[NW], rfrom[NW], rs[2][NW], rt[2][NW];
+  __shared__ float rtm[NT], rs[2][NW], rt[2][NW], rfrom;
   __shared__ int rbefore[NW], rcount[NW], rhas[NW];
   __shared__ uint64_t list[TOP ? NW : 1][TOP ? CAP : 1], rkey[NW];
+  __shared__ v4u near[TOP ? NW : 1][TOP ? BATCH * CV : 1];
+  __shared__ int near_tid[TOP ? NW : 1][TOP ? BATCH : 1];
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE);
   const int row = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
   const uint8_t* p = logits + (size_t)row * ld * E::SIZE;
@@ -157,8 +207,8 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       for (int j = 0; j < 4; ++j) raw[k][j] = E::SIZE == 4 ? E::NINF : E::NINF * 0x10001u;
     }
   }
-  auto entry = [&](float x, int k, int i) {            // by value, then the lowest index
-    return (uint64_t)key_of(x) << 32 | ~(uint32_t)((v0 + k * NT + tid) * E::N + i - shift);
+  auto entry = [&](float x, int j) {                   // by value, then the lowest index
+    return (uint64_t)key_of(x) << 32 | ~(uint32_t)j;
   };
   const long long tok = token_of(tokens, wide, row);
   const bool asked = tok >= 0 && tok < V;
@@ -177,78 +227,75 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
         }
       }
   }
-  float tm = -__builtin_inff();
+  const float tm = Max<DT, CV>::of(raw);
+  rtm[tid] = tm;
+  __syncthreads();
+  float om[NW], m;                         // the lane's threads of all waves
 #pragma unroll
-  for (int k = 0; k < CV; ++k)
-#pragma unroll
-    for (int i = 0; i < E::N; ++i) tm = fmaxf(tm, E::get(raw[k], i));
-  forget(raw);
-  const float wm = wave_max(tm);
-  if (lane == 0) rmax[w] = wm;
-  if (TOP) {
-    // a value that `top` of the wave's 64 threads have an element at or above: the upper 16 bits of the
-    // top-th largest of their maxima, bit by bit
-    const uint32_t k16 = key_of(tm) >> 16;
+  for (int k = 0; k < NW; ++k) om[k] = rtm[k * WAVE + lane];
+  m = wave_max(fmaxf(fmaxf(om[0], om[1]), fmaxf(om[2], om[3])));
+  if (TOP && w == 0) {
+    // a value that `top` threads have an element at or above: the upper 16 bits of the top-th largest of
+    // their maxima, bit by bit
     uint32_t at = 0;
 #pragma unroll
     for (int b = 15; b >= 0; --b) {
       const uint32_t c = at | 1u << b;
-      if (__popcll(__ballot(k16 >= c)) >= top) at = c;
-    }
-    if (lane == 0) rfrom[w] = at > 0x7fu ? of_key(at << 16) : -FLT_MAX;   // (finite ones only)
-  }
-  __syncthreads();
-  float m = rmax[0];
+      int n = 0;
 #pragma unroll
-  for (int k = 1; k < NW; ++k) m = fmaxf(m, rmax[k]);
+      for (int k = 0; k < NW; ++k) n += __popcll(__ballot(key_of(om[k]) >= c << 16));
+      if (n >= top) at = c;
+    }
+    if (lane == 0) rfrom = at > 0x7fu ? of_key(at << 16) : -FLT_MAX;     // (finite ones only)
+  }
   const float c = m == -__builtin_inff() ? 0.f : m * L2E;
+  // vectors that the wave has, the token's, and the value just below its logit
+  const int left = nvec - v0 - w * WAVE, n = left <= 0 ? 0 : min(CV, (left + NT - 1) / NT);
+  const int tv = asked ? (int)((tok + shift) / E::N) : 0;
+  const uint32_t ub = __float_as_uint(xt + 0.f);
+  const float below = __uint_as_float(xt == 0.f ? 0x80000001u : xt > 0.f ? ub - 1 : ub + 1);
+  const bool count = m >= xt, low = !(xt > -__builtin_inff());
+  auto thr = [&](int k) __attribute__((always_inline)) {
+    const int vw = v0 + k * NT + w * WAVE;             // the wave's first vector
+    return vw + WAVE <= tv ? below : vw > tv ? xt : __builtin_inff();
+  };
+  auto none = [](int) { return 0.f; };
   float s, t;
-  sums<DT, CV, false>(raw, c, m, false, s, t);
-  forget(raw);
   int before = 0;
-  if (m >= xt) {
-    const long long tv = (tok + shift) / E::N;
-#pragma unroll
-    for (int k = 0; k < CV; ++k) {
-      const int vw = v0 + k * NT + w * WAVE;           // the wave's first vector
-      if (vw + WAVE <= tv) {
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) >= xt));
-        if (vw == 0 && !(xt > -__builtin_inff())) before -= shift;      // not a neighbour's place
-      } else if (vw > tv) {
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) > xt));
-      } else {
-#pragma unroll
-        for (int i = 0; i < E::N; ++i) {
-          const long long j = (long long)(vw + lane) * E::N + i - shift;
-          const float x = E::get(raw[k], i);
-          before += __popcll(__ballot(x > xt || (x == xt && j >= 0 && j < tok)));
-        }
-      }
-    }
-  }
-  forget(raw);
-  if (TOP) {
-    float from = rfrom[0];
-#pragma unroll
-    for (int k = 1; k < NW; ++k) from = fmaxf(from, rfrom[k]);
-    int count = 0;
+  bool again = n && __ballot(E::get(raw[0], 0) == -__builtin_inff());
+  if (!again) {
+    if (count && !low) sums<DT, CV, false, false, true>(raw, n, c, m, false, thr, s, t, before);
+    else sums<DT, CV, false, false, false>(raw, n, c, m, false, none, s, t, before);
+    again = __ballot(t != t);
+  } else if (count && !low) {
 #pragma unroll
     for (int k = 0; k < CV; ++k)
 #pragma unroll
-      for (int i = 0; i < E::N; ++i) {
-        const float x = E::get(raw[k], i);
-        const uint64_t in = __ballot(x >= from);
-        if (in) {
-          const int at = count + mbcnt(in);
-          if (x >= from && at < CAP) list[w][at] = entry(x, k, i);
-          count += __popcll(in);
+      for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) > thr(k)));
+  }
+  if (again) {
+    forget(raw);
+    sums<DT, CV, true, false, false>(raw, n, c, m, false, none, s, t, before);
+  }
+  if (count) {                             // the vectors beside the token's, and a token at -inf
+    forget(raw);
+#pragma unroll
+    for (int k = 0; k < CV; ++k) {
+      const int vw = v0 + k * NT + w * WAVE;
+      if (vw > tv || (!low && vw + WAVE <= tv)) {
+        if (low)
+#pragma unroll
+          for (int i = 0; i < E::N; ++i) before += __popcll(__ballot(E::get(raw[k], i) > xt));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E::N; ++i) {
+          const int j = (vw + lane) * E::N + i - shift;
+          const float x = E::get(raw[k], i);
+          before += __popcll(__ballot(x > xt || (x == xt && j >= 0 && j < (int)tok)));
         }
       }
-    if (lane == 0) rcount[w] = count;
+    }
   }
-  forget(raw);
   s = wave_add(s);
   t = wave_add(t);
   if (lane == 0) {
@@ -258,6 +305,37 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
     rhas[w] = 0;
   }
   __syncthreads();
+  if (TOP) {
+    // the elements from there on, of the threads that have any, BATCH threads at a time
+    const float from = rfrom;
+    forget(raw);
+    uint64_t todo = __ballot(tm >= from);
+    int count = 0;
+    while (todo) {
+      const int at = mbcnt(todo);
+      const bool mine = (todo >> lane & 1) && at < BATCH;
+      if (mine) {
+#pragma unroll
+        for (int k = 0; k < CV; ++k) near[w][at * CV + k] = raw[k];
+        near_tid[w][at] = tid;
+      }
+      wave_lds_sync();
+      const int n = min(__popcll(todo), BATCH) * CV * E::N;
+      for (int j0 = 0; j0 < n; j0 += WAVE) {
+        const int j = j0 + lane, a = j / (CV * E::N), k = j / E::N % CV, i = j % E::N;
+        const float x = j < n ? load_one<DT>((const uint8_t*)near[w], j) : -__builtin_inff();
+        const uint64_t in = __ballot(x >= from);
+        const int to = count + mbcnt(in);
+        if (x >= from && to < CAP)
+          list[w][to] = entry(x, (v0 + k * NT + near_tid[w][a]) * E::N + i - shift);
+        count += __popcll(in);
+      }
+      wave_lds_sync();
+      todo &= ~__ballot(mine);
+    }
+    if (lane == 0) rcount[w] = count;
+    __syncthreads();
+  }
   s = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]);
   t = (rt[0][0] + rt[0][1]) + (rt[0][2] + rt[0][3]);
   const float r = fmaf(m, L2E, -c);        // log2 of the maximum's own term: c is rounded
@@ -269,7 +347,9 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
     if (lane == 0 && has) rhas[w] = 1;
     __syncthreads();
     const int first = rhas[0] ? 0 : rhas[1] ? 1 : rhas[2] ? 2 : 3;
-    sums<DT, CV, true>(raw, c, m, w == first && lane == __ffsll((unsigned long long)has) - 1, s, t);
+    sums<DT, CV, true, true, false>(raw, n, c, m,
+                                    w == first && lane == __ffsll((unsigned long long)has) - 1, none,
+                                    s, t, before);
     s = wave_add(s);
     t = wave_add(t);
     if (lane == 0) {
@@ -311,14 +391,12 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       uint64_t last = ~0ull;
       for (int n = 0; n < top; ++n) {
         uint64_t best = 0;
-        forget(raw);
         if (last)
-#pragma unroll
-          for (int k = 0; k < CV; ++k)
-#pragma unroll
+          for (int v = v0 + tid; v < min(v0 + CV * NT, nvec); v += NT)
             for (int i = 0; i < E::N; ++i) {
-              const float x = E::get(raw[k], i);
-              const uint64_t key = x >= -FLT_MAX ? entry(x, k, i) : 0;
+              const int j = v * E::N + i - shift;
+              const float x = j >= 0 && j < V ? load_one<DT>(p, j) : -__builtin_inff();
+              const uint64_t key = x >= -FLT_MAX ? entry(x, j) : 0;
               best = key < last && key > best ? key : best;
             }
         best = wave_reduce64(best, OpMax64());
@@ -335,7 +413,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
 
 // Joins a row's segments: one wave a row. parts [R][nseg], lists [R][nseg][top] in falling order, 0 behind
 // the last.
-template <int DT>
+template <int DT, int K>
 __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logits, long long ld,
                                                int V, int nseg, const void* __restrict__ tokens,
                                                int wide, int top, const Part* __restrict__ parts,
@@ -344,7 +422,7 @@ __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logit
                                                float* __restrict__ entropy,
                                                float* __restrict__ top_logprobs,
                                                int* __restrict__ top_ids) {
-  extern __shared__ uint64_t heads[];      // [nseg][top]
+  extern __shared__ uint64_t heads[];      // [nseg][top], then WAVE chosen
   const int lane = lane_id(), row = (int)blockIdx.x;
   const float ninf = -__builtin_inff(), nan = __builtin_nanf("");
   const uint8_t* p = logits + (size_t)row * ld * Elem<DT>::SIZE;
@@ -378,13 +456,50 @@ __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logit
   }
   if (top == 0) return;
   wave_lds_sync();
-  uint64_t head = lane < nseg ? heads[lane * top] : 0, mine = 0;
-  int next = 1, found = 0;
-  for (; found < top; ++found) {
-    const uint64_t best = wave_reduce64(head, OpMax64());
-    if (best == 0) break;
-    if (lane == found) mine = best;
-    if (head == best) head = next < top ? heads[lane * top + next++] : 0;
+  // the top-th largest value of all the lists, bit by bit, then the place of each from there on
+  const int all = nseg * top;
+  uint64_t mine = 0;
+  int found = 0;
+  uint32_t at = 0;
+  uint64_t key[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) key[k] = k * WAVE + lane < all ? heads[k * WAVE + lane] : 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t c = at | 1u << b;
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) n += __popcll(__ballot((uint32_t)(key[k] >> 32) >= c));
+    if (n >= top) at = c;
+  }
+  uint64_t* chosen = heads + all;
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool in = key[k] && (uint32_t)(key[k] >> 32) >= at;
+    const uint64_t w = __ballot(in);
+    const int to = n + mbcnt(w);
+    if (in && to < WAVE) chosen[to] = key[k];
+    n += __popcll(w);
+  }
+  wave_lds_sync();
+  if (n <= WAVE) {
+    found = min(n, top);
+    const uint64_t own = lane < n ? chosen[lane] : 0;
+    int place = 0;
+    for (int k = 0; k < n; ++k) place += chosen[k] > own;
+    wave_lds_sync();
+    if (lane < n) chosen[place] = own;
+    wave_lds_sync();
+    if (lane < found) mine = chosen[lane];
+  } else {                                 // many equal ones: one after the other
+    uint64_t head = lane < nseg ? heads[lane * top] : 0;
+    int next = 1;
+    for (; found < top; ++found) {
+      const uint64_t best = wave_reduce64(head, OpMax64());
+      if (best == 0) break;
+      if (lane == found) mine = best;
+      if (head == best) head = next < top ? heads[lane * top + next++] : 0;
+    }
   }
   float* ol = top_logprobs + (size_t)row * top;
   int* oi = top_ids + (size_t)row * top;
@@ -416,7 +531,7 @@ struct Plan {
 static Plan plan(int dtype, int R, int V) {
   const int n = dtype == 1 ? 4 : 8;
   const int chunks = (V + 2 * n - 2) / n / NT + 1;     // of NT vectors, wherever the row starts
-  Plan p = {8, 0};
+  Plan p = {chunks >= 8 ? 8 : chunks > 2 ? 4 : chunks, 0};
   for (;; p.cv /= 2) {
     p.nseg = (chunks + p.cv - 1) / p.cv;
     const int half = (chunks + p.cv / 2 - 1) / (p.cv / 2 > 0 ? p.cv / 2 : 1);
@@ -456,13 +571,21 @@ extern "C" int rlu_token_logprobs(const void* logits, int dtype, long long ld, i
   auto* parts = (Part*)(lists + (size_t)R * pl.nseg * top);
   const dim3 grid((unsigned)(R * pl.nseg));
 #define RLU_SEG(DT, CV, TOP)                                                                       hipLaunchKernelGGL((segment_k<DT, CV, TOP>), grid, dim3(NT), 0, stream, x, ld, V, pl.nseg,                          tokens, wide, top, parts, lists)
+#define RLU_JOIN(DT, K)                                                                          \
+  hipLaunchKernelGGL((join_k<DT, K>), dim3((unsigned)R), dim3(rlu::WAVE),                        \
+                     top ? (pl.nseg * top + rlu::WAVE) * 8 : 0, stream, x, ld, V, pl.nseg, tokens, \
+                     wide, top, parts, lists, logprob, rank, entropy, top_logprobs, top_ids)
 #define RLU_CV(DT, TOP)                 do {                                    if (pl.cv == 8) RLU_SEG(DT, 8, TOP);          else if (pl.cv == 4) RLU_SEG(DT, 4, TOP);     else if (pl.cv == 2) RLU_SEG(DT, 2, TOP);     else RLU_SEG(DT, 1, TOP);                   } while (0)
-#define RLU_DT(DT)                                                                                do {                                                                                              if (top) RLU_CV(DT, true);                                                                      else RLU_CV(DT, false);                                                                         hipLaunchKernelGGL((join_k<DT>), dim3((unsigned)R), dim3(rlu::WAVE), pl.nseg * top * 8,                            stream, x, ld, V, pl.nseg, tokens, wide, top, parts, lists, logprob, rank,                        entropy, top_logprobs, top_ids);                                           } while (0)
+#define RLU_DT(DT)                                                                                do {                                                                                              if (top) RLU_CV(DT, true);                                                                      else RLU_CV(DT, false);                                                                         if (pl.nseg * top <= 4 * rlu::WAVE) RLU_JOIN(DT, 4);                                        \
+    else if (pl.nseg * top <= 12 * rlu::WAVE) RLU_JOIN(DT, 12);                                 \
+    else RLU_JOIN(DT, 32);                                                                      \
+  } while (0)
   if (dtype == 0) RLU_DT(0);
   else if (dtype == 1) RLU_DT(1);
   else RLU_DT(2);
 #undef RLU_DT
 #undef RLU_CV
+#undef RLU_JOIN
 #undef RLU_SEG
   return (int)hipGetLastError();
 }
