@@ -75,18 +75,23 @@ typedef unsigned short v2us __attribute__((ext_vector_type(2)));
 template <int DT, int CV>
 __device__ __forceinline__ float packed_max(const v4u (&raw)[CV]) {
   v2s hi = __builtin_bit_cast(v2s, (uint32_t)raw[0][0]);
-  v2us lo = __builtin_bit_cast(v2us, (uint32_t)raw[0][0]);
 #pragma unroll
   for (int k = 0; k < CV; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i)
       hi = __builtin_elementwise_max(hi, __builtin_bit_cast(v2s, (uint32_t)raw[k][i]));
-      lo = __builtin_elementwise_min(lo, __builtin_bit_cast(v2us, (uint32_t)raw[k][i]));
-    }
   const short h = hi[0] > hi[1] ? hi[0] : hi[1];
-  const unsigned short l = lo[0] < lo[1] ? lo[0] : lo[1];
   v4u v = {};
-  v[0] = h >= 0 ? (uint16_t)h : l;
+  v[0] = (uint16_t)h;
+  if (__ballot(h < 0)) {
+    v2us lo = __builtin_bit_cast(v2us, (uint32_t)raw[0][0]);
+#pragma unroll
+    for (int k = 0; k < CV; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        lo = __builtin_elementwise_min(lo, __builtin_bit_cast(v2us, (uint32_t)raw[k][i]));
+    if (h < 0) v[0] = lo[0] < lo[1] ? lo[0] : lo[1];
+  }
   return Elem<DT>::get(v, 0);
 }
 template <int CV>
@@ -151,11 +156,10 @@ __device__ __forceinline__ void forget(v4u (&raw)[CV]) {
 }
 
 // The sums of a thread's vectors, n of them, against c = RN(m log2 e).
-//   CLAMP: takes -inf (its product with its zero is a NaN without); SKIP: and leaves out one element
-//   equal to m where skip. COUNT: adds the wave's elements above thr(k) to before.
-template <int DT, int CV, bool CLAMP, bool SKIP, bool COUNT, class Thr>
-__device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, float m, bool skip,
-                                     Thr thr, float& s, float& t, int& before) {
+//   CLAMP: takes -inf (its product with its zero is a NaN without). COUNT: adds the wave's elements above thr(k) to before.
+template <int DT, int CV, bool CLAMP, bool COUNT, class Thr>
+__device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, Thr thr, float& s,
+                                     float& t, int& before) {
   s = t = 0.f;
 #pragma unroll
   for (int k = 0; k < CV; ++k) {
@@ -163,12 +167,8 @@ __device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, float
     const float above = COUNT ? thr(k) : 0.f;
 #pragma unroll
     for (int i = 0; i < Elem<DT>::N; ++i) {
-      float x = Elem<DT>::get(raw[k], i);
+      const float x = Elem<DT>::get(raw[k], i);
       if (COUNT) before += __popcll(__ballot(x > above));
-      if (SKIP && skip && x == m) {
-        x = -__builtin_inff();
-        skip = false;
-      }
       const float y = fmaf(x, L2E, -c);
       const float e = __builtin_amdgcn_exp2f(y);
       s += e;
@@ -184,8 +184,9 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
                                                 int wide, int top, Part* __restrict__ parts,
                                                 uint64_t* __restrict__ lists) {
   typedef Elem<DT> E;
-  __shared__ float rtm[NT], rs[2][NW], rt[2][NW], rfrom;
-  __shared__ int rbefore[NW], rcount[NW], rhas[NW];
+  __shared__ float rtm[NT], rs[NW], rt[NW], rfrom;
+  __shared__ int rbefore[NW], rcount[NW];
+  __shared__ v4u one[CV];
   __shared__ uint64_t list[TOP ? NW : 1][TOP ? CAP : 1], rkey[NW];
   __shared__ v4u near[TOP ? NW : 1][TOP ? BATCH * CV : 1];
   __shared__ int near_tid[TOP ? NW : 1][TOP ? BATCH : 1];
@@ -264,8 +265,8 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   int before = 0;
   bool again = n && __ballot(E::get(raw[0], 0) == -__builtin_inff());
   if (!again) {
-    if (count && !low) sums<DT, CV, false, false, true>(raw, n, c, m, false, thr, s, t, before);
-    else sums<DT, CV, false, false, false>(raw, n, c, m, false, none, s, t, before);
+    if (count && !low) sums<DT, CV, false, true>(raw, n, c, thr, s, t, before);
+    else sums<DT, CV, false, false>(raw, n, c, none, s, t, before);
     again = __ballot(t != t);
   } else if (count && !low) {
 #pragma unroll
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   }
   if (again) {
     forget(raw);
-    sums<DT, CV, true, false, false>(raw, n, c, m, false, none, s, t, before);
+    sums<DT, CV, true, false>(raw, n, c, none, s, t, before);
   }
   if (count) {                             // the vectors beside the token's, and a token at -inf
     forget(raw);
@@ -296,13 +297,33 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       }
     }
   }
+  // The maximum's own 1 is left out: small terms would be lost beside it. The first thread that has it hands
+  // its elements to the wave, which sums them again without the first that is equal to it.
+  const uint64_t h0 = __ballot(om[0] == m), h1 = __ballot(om[1] == m), h2 = __ballot(om[2] == m);
+  const int first = h0 ? 0 : h1 ? 1 : h2 ? 2 : 3;
+  if (w == first && m > -__builtin_inff()) {
+    const int f = __ffsll((unsigned long long)__ballot(tm == m)) - 1;
+    if (lane == f) {
+#pragma unroll
+      for (int k = 0; k < CV; ++k) one[k] = raw[k];
+      s = t = 0.f;
+    }
+    wave_lds_sync();
+    const bool in = lane < CV * E::N;
+    const float x = in ? load_one<DT>((const uint8_t*)one, lane) : 0.f;
+    const uint64_t eq = __ballot(in && x == m);
+    if (in && lane != __ffsll((unsigned long long)eq) - 1) {
+      const float y = fmaf(x, L2E, -c), e = __builtin_amdgcn_exp2f(y);
+      s += e;
+      t = fmaf(fmaxf(y, -200.f), e, t);
+    }
+  }
   s = wave_add(s);
   t = wave_add(t);
   if (lane == 0) {
-    rs[0][w] = s;
-    rt[0][w] = t;
+    rs[w] = s;
+    rt[w] = t;
     rbefore[w] = before;
-    rhas[w] = 0;
   }
   __syncthreads();
   if (TOP) {
@@ -320,52 +341,36 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
         near_tid[w][at] = tid;
       }
       wave_lds_sync();
-      const int n = min(__popcll(todo), BATCH) * CV * E::N;
-      for (int j0 = 0; j0 < n; j0 += WAVE) {
-        const int j = j0 + lane, a = j / (CV * E::N), k = j / E::N % CV, i = j % E::N;
-        const float x = j < n ? load_one<DT>((const uint8_t*)near[w], j) : -__builtin_inff();
+      // a pass takes SRC threads' PER elements each
+      constexpr int PER = CV * E::N, SRC = WAVE / PER;
+      static_assert(SRC * PER == WAVE, "a wave's pass");
+      const int n = min(__popcll(todo), BATCH), e = lane % PER;
+      const int at0 = (v0 + e / E::N * NT) * E::N + e % E::N - shift;
+      for (int a = lane / PER; a - lane / PER < n; a += SRC) {
+        const float x =
+            a < n ? load_one<DT>((const uint8_t*)near[w], a * PER + e) : -__builtin_inff();
         const uint64_t in = __ballot(x >= from);
         const int to = count + mbcnt(in);
-        if (x >= from && to < CAP)
-          list[w][to] = entry(x, (v0 + k * NT + near_tid[w][a]) * E::N + i - shift);
+        if (x >= from && to < CAP) list[w][to] = entry(x, at0 + near_tid[w][a] * E::N);
         count += __popcll(in);
       }
       wave_lds_sync();
       todo &= ~__ballot(mine);
     }
+    if (lane < 8 && count + lane < CAP) list[w][count + lane] = 0;      // (places are counted by 8)
     if (lane == 0) rcount[w] = count;
     __syncthreads();
   }
-  s = (rs[0][0] + rs[0][1]) + (rs[0][2] + rs[0][3]);
-  t = (rt[0][0] + rt[0][1]) + (rt[0][2] + rt[0][3]);
-  const float r = fmaf(m, L2E, -c);        // log2 of the maximum's own term: c is rounded
-  const float unit = __builtin_amdgcn_exp2f(-r);
-  float rest = m > -__builtin_inff() ? s * unit - 1.f : s - 1.f;
-  if (m > -__builtin_inff() && s < 1.5f) {             // nearly certain: the sums without the maximum
-    forget(raw);
-    const uint64_t has = __ballot(tm == m);
-    if (lane == 0 && has) rhas[w] = 1;
-    __syncthreads();
-    const int first = rhas[0] ? 0 : rhas[1] ? 1 : rhas[2] ? 2 : 3;
-    sums<DT, CV, true, true, false>(raw, n, c, m,
-                                    w == first && lane == __ffsll((unsigned long long)has) - 1, none,
-                                    s, t, before);
-    s = wave_add(s);
-    t = wave_add(t);
-    if (lane == 0) {
-      rs[1][w] = s;
-      rt[1][w] = t;
-    }
-    __syncthreads();
-    s = (rs[1][0] + rs[1][1]) + (rs[1][2] + rs[1][3]);
-    t = (rt[1][0] + rt[1][1]) + (rt[1][2] + rt[1][3]);
-    rest = s * unit;
-  }
+  s = (rs[0] + rs[1]) + (rs[2] + rs[3]);
+  t = (rt[0] + rt[1]) + (rt[2] + rt[3]);
   if (tid == 0) {
+    const float r = fmaf(m, L2E, -c);      // log2 of the maximum's own term: c is rounded
+    const float unit = __builtin_amdgcn_exp2f(-r);
+    const bool some = m > -__builtin_inff();
     Part o;
     o.m = m;
-    o.rest = rest;
-    o.t = m > -__builtin_inff() ? (t - r * s) * unit : 0.f;
+    o.rest = m == __builtin_inff() ? __builtin_nanf("") : some ? s * unit : s - 1.f;
+    o.t = some ? (t - r * s) * unit : 0.f;
     o.before = rbefore[0] + rbefore[1] + rbefore[2] + rbefore[3];
     parts[blockIdx.x] = o;
   }
@@ -383,7 +388,9 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
         int place = 0;
 #pragma unroll
         for (int k = 0; k < NW; ++k)
-          for (int l = 0; l < rcount[k]; ++l) place += list[k][l] > key;
+          for (int l = 0; l < rcount[k]; l += 8)
+#pragma unroll
+            for (int o = 0; o < 8; ++o) place += list[k][l + o] > key;
         if (place < top) out[place] = key;
       }
       if (tid >= total && tid < top) out[tid] = 0;
@@ -456,22 +463,25 @@ __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logit
   }
   if (top == 0) return;
   wave_lds_sync();
-  // the top-th largest value of all the lists, bit by bit, then the place of each from there on
+  // a value that at least top are at or above: of the lists' entries at one depth the one that so many
+  // lists reach it (its upper 16 bits, bit by bit); then the place of each from there on
   const int all = nseg * top;
   uint64_t mine = 0;
   int found = 0;
+  const int deep = min(top, (2 * top + nseg - 1) / nseg), reach = (top + deep - 1) / deep;
+  const uint32_t probe = lane < nseg ? (uint32_t)(heads[lane * top + deep - 1] >> 32) : 0;
   uint32_t at = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t c = at | 1u << b;
+    if (__popcll(__ballot(probe >= c)) >= reach) at = c;
+  }
   uint64_t key[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) key[k] = k * WAVE + lane < all ? heads[k * WAVE + lane] : 0;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t c = at | 1u << b;
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) n += __popcll(__ballot((uint32_t)(key[k] >> 32) >= c));
-    if (n >= top) at = c;
-  }
   uint64_t* chosen = heads + all;
+  chosen[lane] = 0;
+  wave_lds_sync();
   int n = 0;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -486,7 +496,9 @@ __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logit
     found = min(n, top);
     const uint64_t own = lane < n ? chosen[lane] : 0;
     int place = 0;
-    for (int k = 0; k < n; ++k) place += chosen[k] > own;
+    for (int k = 0; k < n; k += 8)         // (zeros behind the last)
+#pragma unroll
+      for (int l = 0; l < 8; ++l) place += chosen[k + l] > own;
     wave_lds_sync();
     if (lane < n) chosen[place] = own;
     wave_lds_sync();
