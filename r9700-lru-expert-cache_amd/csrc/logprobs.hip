@@ -155,10 +155,26 @@ __device__ __forceinline__ void forget(v4u (&raw)[CV]) {
   for (int k = 0; k < CV; ++k) asm volatile("" : "+v"(raw[k]));
 }
 
-// The sums of a thread's vectors, n of them, against c = RN(m log2 e).
-//   CLAMP: takes -inf (its product with its zero is a NaN without). COUNT: adds the wave's elements above thr(k) to before.
-template <int DT, int CV, bool CLAMP, bool COUNT, class Thr>
-__device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, Thr thr, float& s,
+// log2(e^(x - m)) and its sums take c = RN(m log2 e), one multiply-add an element: with the same c in all
+// of them its rounding is undone at the end. Where that rounding is not small (|m| past 4096, 2^-11; a row at
+// the type's lowest value overflows there) base = m is taken off first.
+struct Ref {
+  float base, c;
+};
+__device__ __forceinline__ Ref ref_of(float m) {
+  const bool far = !(fabsf(m) <= 4096.f), inf = fabsf(m) == __builtin_inff();
+  return far && !inf ? Ref{m, 0.f} : Ref{0.f, m == -__builtin_inff() ? 0.f : m * L2E};
+}
+__device__ __forceinline__ void term(float x, Ref f, float& s, float& t) {
+  const float y = fmaf(x - f.base, L2E, -f.c), e = __builtin_amdgcn_exp2f(y);
+  s += e;
+  t = fmaf(fmaxf(y, -200.f), e, t);        // (-inf times its zero)
+}
+
+// The sums of a thread's vectors, n of them. ANY: takes -inf and far maxima. COUNT: adds the wave's elements
+// above thr(k) to before.
+template <int DT, int CV, bool ANY, bool COUNT, class Thr>
+__device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, Ref f, Thr thr, float& s,
                                      float& t, int& before) {
   s = t = 0.f;
 #pragma unroll
@@ -169,10 +185,13 @@ __device__ __forceinline__ void sums(const v4u (&raw)[CV], int n, float c, Thr t
     for (int i = 0; i < Elem<DT>::N; ++i) {
       const float x = Elem<DT>::get(raw[k], i);
       if (COUNT) before += __popcll(__ballot(x > above));
-      const float y = fmaf(x, L2E, -c);
-      const float e = __builtin_amdgcn_exp2f(y);
-      s += e;
-      t = fmaf(CLAMP ? fmaxf(y, -200.f) : y, e, t);
+      if (ANY) {
+        term(x, f, s, t);
+      } else {
+        const float y = fmaf(x, L2E, -f.c), e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        t = fmaf(y, e, t);
+      }
     }
   }
 }
@@ -249,7 +268,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
     }
     if (lane == 0) rfrom = at > 0x7fu ? of_key(at << 16) : -FLT_MAX;     // (finite ones only)
   }
-  const float c = m == -__builtin_inff() ? 0.f : m * L2E;
+  const Ref ref = ref_of(m);
   // vectors that the wave has, the token's, and the value just below its logit
   const int left = nvec - v0 - w * WAVE, n = left <= 0 ? 0 : min(CV, (left + NT - 1) / NT);
   const int tv = asked ? (int)((tok + shift) / E::N) : 0;
@@ -263,10 +282,10 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   auto none = [](int) { return 0.f; };
   float s, t;
   int before = 0;
-  bool again = n && __ballot(E::get(raw[0], 0) == -__builtin_inff());
+  bool again = (n && __ballot(E::get(raw[0], 0) == -__builtin_inff())) || ref.base != 0.f;
   if (!again) {
-    if (count && !low) sums<DT, CV, false, true>(raw, n, c, thr, s, t, before);
-    else sums<DT, CV, false, false>(raw, n, c, none, s, t, before);
+    if (count && !low) sums<DT, CV, false, true>(raw, n, ref, thr, s, t, before);
+    else sums<DT, CV, false, false>(raw, n, ref, none, s, t, before);
     again = __ballot(t != t);
   } else if (count && !low) {
 #pragma unroll
@@ -276,7 +295,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   }
   if (again) {
     forget(raw);
-    sums<DT, CV, true, false>(raw, n, c, none, s, t, before);
+    sums<DT, CV, true, false>(raw, n, ref, none, s, t, before);
   }
   if (count) {                             // the vectors beside the token's, and a token at -inf
     forget(raw);
@@ -312,11 +331,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
     const bool in = lane < CV * E::N;
     const float x = in ? load_one<DT>((const uint8_t*)one, lane) : 0.f;
     const uint64_t eq = __ballot(in && x == m);
-    if (in && lane != __ffsll((unsigned long long)eq) - 1) {
-      const float y = fmaf(x, L2E, -c), e = __builtin_amdgcn_exp2f(y);
-      s += e;
-      t = fmaf(fmaxf(y, -200.f), e, t);
-    }
+    if (in && lane != __ffsll((unsigned long long)eq) - 1) term(x, ref, s, t);
   }
   s = wave_add(s);
   t = wave_add(t);
@@ -364,7 +379,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   s = (rs[0] + rs[1]) + (rs[2] + rs[3]);
   t = (rt[0] + rt[1]) + (rt[2] + rt[3]);
   if (tid == 0) {
-    const float r = fmaf(m, L2E, -c);      // log2 of the maximum's own term: c is rounded
+    const float r = fmaf(m - ref.base, L2E, -ref.c);   // the maximum's own log2: what c's rounding left
     const float unit = __builtin_amdgcn_exp2f(-r);
     const bool some = m > -__builtin_inff();
     Part o;
@@ -447,7 +462,7 @@ __global__ __launch_bounds__(WAVE) void join_k(const uint8_t* __restrict__ logit
   float rest = q.rest, t = q.t;
   if (!ref) {
     rest = q.m > ninf ? a * (1.f + q.rest) : q.rest + 1.f;              // (a NaN stays)
-    t = q.m > ninf ? a * fmaf(d, 1.f + q.rest, q.t) : 0.f;
+    t = a > 0.f ? a * fmaf(d, 1.f + q.rest, q.t) : 0.f;
   }
   rest = wave_add(rest);
   t = wave_add(t);

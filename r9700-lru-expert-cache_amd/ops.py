@@ -13,6 +13,8 @@ Mirrors the reference's Python entry points for these stages:
   shuffle_fp8_weight              shuffle_weight_gfx1201 (kernels/fp8_target_lmhead.py:47,64),
                                   here the gfx950 MFMA fragment order every GEMM reads
   pack_fp8_block                  kernels/fp8_target_lmhead.py:44-66
+  pack_fp8_dense, gemm_fp8_dense  the block-scaled product for any number of rows and columns (no
+                                  counterpart: the reference's head kernel takes decode rows only)
   moe_gemm_tiled                  the grouped GEMM for prefill-sized inputs (no counterpart:
                                   the reference ran one closed kernel at every M)
 Errors from the C-ABI raise RuntimeError; there is no fallback implementation (Fp8TargetHead
@@ -28,6 +30,7 @@ from dataclasses import dataclass
 import torch
 
 from ._lib import check, device_ptr, lib, on_device, stream_ptr
+from .logprobs import TokenLogprobs, token_logprobs
 
 _P = ctypes.c_void_p
 FP8 = torch.float8_e4m3fn
@@ -281,6 +284,11 @@ def gemm_fp8_block(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch
 FP8_LMHEAD_MAX_M = int(os.environ.get("VLLM_TARGET_FP8_LMHEAD_MAX_M", "64"))
 
 
+# rows of logits that Fp8TargetHead.logprobs holds at a time: 311 MB at vocab 151936, where the product
+# already runs at its full rate
+LOGPROBS_ROWS = 1024
+
+
 class Fp8TargetHead:
     """Drop-in replacement for the lm_head's quant_method at decode M
     (kernels/fp8_target_lmhead.py:77-93). The weight is packed once (pack_fp8_block). apply()
@@ -299,6 +307,32 @@ class Fp8TargetHead:
         y = gemm_fp8_block(flat, self.wq, self.ws)
         self.n_fp8 += 1
         return y.reshape(*x.shape[:-1], y.shape[-1])
+
+    def logprobs(self, x: torch.Tensor, tokens: torch.Tensor, top_n: int = 0):
+        """logprobs.TokenLogprobs of this head's logits for x [..., K] bf16 and tokens [...] (any number
+        of rows, a prompt's too): quantized rows, gemm_fp8_dense and logprobs.token_logprobs,
+        LOGPROBS_ROWS rows of logits at a time. Up to 64 rows the logits are apply's bit for bit."""
+        if x.dtype != torch.bfloat16 or x.shape[-1] != self.wq.shape[1]:
+            raise ValueError(f"logprobs takes bf16 rows of {self.wq.shape[1]}")
+        if tokens.shape != x.shape[:-1]:
+            raise ValueError(f"logprobs: tokens {tuple(tokens.shape)} for rows {tuple(x.shape[:-1])}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("logprobs has no gradient: detach the rows")
+        w = PackedFp8(wq=self.wq, ws=self.ws, n=self.wq.shape[0], k=self.wq.shape[1])
+        flat, ids = x.reshape(-1, w.k), tokens.reshape(-1)
+        if flat.stride(1) != 1:
+            flat = flat.contiguous()
+        if not flat.shape[0]:
+            parts = [token_logprobs(flat.new_empty((0, w.n)), ids, top_n)]
+        else:
+            parts = []
+        with on_device(x.device):
+            for r0 in range(0, flat.shape[0], LOGPROBS_ROWS):
+                r1 = min(flat.shape[0], r0 + LOGPROBS_ROWS)
+                y = gemm_fp8_dense(*fp8_quant_group(flat[r0:r1], GROUP), w)
+                parts.append(token_logprobs(y, ids[r0:r1], top_n))
+        out = parts[0] if len(parts) == 1 else TokenLogprobs(*map(torch.cat, zip(*parts)))
+        return TokenLogprobs(*[t.reshape(*tokens.shape, *t.shape[1:]) for t in out])
 
     def __getattr__(self, name):
         if name == "orig":                          # not set yet (copy / unpickle)
