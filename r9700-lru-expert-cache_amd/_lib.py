@@ -86,8 +86,9 @@ def lib() -> ctypes.CDLL:
 
 def stream_ptr(stream=None) -> int:
     import torch
-    s = torch.cuda.current_stream() if stream is None else stream
-    return s.cuda_stream
+    if stream is None:       # without building a Stream object for it: 0.3 us, not 2.9
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return stream.cuda_stream
 
 
 _HERE = contextlib.nullcontext()
