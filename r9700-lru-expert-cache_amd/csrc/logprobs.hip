@@ -562,7 +562,7 @@ static Plan plan(int dtype, int R, int V) {
   for (;; p.cv /= 2) {
     p.nseg = (chunks + p.cv - 1) / p.cv;
     const int half = (chunks + p.cv / 2 - 1) / (p.cv / 2 > 0 ? p.cv / 2 : 1);
-    if (p.cv == 1 || half > MAX_SEGS || (long long)R * p.nseg >= 512) return p;
+    if (p.cv == 1 || half > MAX_SEGS || (long long)R * p.nseg >= 256) return p;
   }
 }
 
