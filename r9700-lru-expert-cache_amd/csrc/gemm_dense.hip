@@ -314,20 +314,23 @@ extern "C" int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void
   auto* o = (uint16_t*)y;
   // Which kernel: the least of these estimates in us, each of a round of the CUs (fixed part, a 128-deep
   // step's) as measured. Tiles, with every CU busy: Big 8 + 1.6, Mid 6.5 + 1.22, Small 4 + 0.55 alone
-  // on its CU and 6 + 0.95 for two. The head's kernel, 64 rows x 64 columns and a K split over its waves:
-  // 3.7 + 1.35 for a wave's steps.
+  // on its CU and 6 + 0.95 for two, and 2.5 more where rows do not start at 16 bytes. The head's kernel,
+  // 64 rows x 64 columns and K split over its waves: 3.7 + 1.35 for a wave's steps.
   //   rows x n x K           head / Big / Mid / Small (us)
   //   256 x 2560 x 2560      10.5 / 28.5 / 24.9 / 15.2    1024 x 2560     24 / 29 / 25.6 / 16
   //   4096 x 2560 x 2560     - / 34 / 31 / 39             2048 x 10240    - / 69 / 64 / 70
   //   128 x 151936 x 2560    192 / 119 / 114 / 104        160 x 151936    270 / 126 / 117 / 141
   //   256 x 151936 x 2560    373 / 138 / 173 / 158        512 x 32000     118 / 36 / 50 / 43
+  //   617 x 1543 x 768       8.4 / - / - / 10.8
   // Up to 64 rows the head's kernel reads the weights once, as it does for gemm_fp8_block.
   const int steps = K / 128, sk = head::sk_of(K);
   if (M <= 64 && sk) return head::rows(q, xs, p, ws, o, ldy, M, n, K, stream);
-  const double ns = (double)dense::per_cu<dense::Small>(M, n);
-  const double big = dense::per_cu<dense::Big>(M, n) * (8 + 1.6 * steps);
-  const double mid = dense::per_cu<dense::Mid>(M, n) * (6.5 + 1.22 * steps);
-  const double small = (long long)ns / 2 * (6 + 0.95 * steps) + (long long)ns % 2 * (4 + 0.55 * steps);
+  const long long ns = dense::per_cu<dense::Small>(M, n);
+  const double odd = ldy % 8 || (uintptr_t)y % 16 ? 2.5 : 0;
+  const double big = dense::per_cu<dense::Big>(M, n) * (8 + odd + 1.6 * steps);
+  const double mid = dense::per_cu<dense::Mid>(M, n) * (6.5 + odd + 1.22 * steps);
+  const double small =
+      ns / 2 * (6 + odd + 0.95 * steps) + ns % 2 * (4 + odd + 0.55 * steps);
   const double tile = small < mid ? (small < big ? small : big) : mid < big ? mid : big;
   if (sk && M <= 65535 * 64) {
     const long long items = (n + 127) / 128 * 2, wgs = (items * sk + 3) / 4 * ((M + 63) / 64);
