@@ -1,6 +1,34 @@
-// The dense fp8 block-scaled GEMM for many rows: y[M, n] bf16 = A[M, K] W[n, K]^T, A e4m3 row-major
-// with a float32 scale per row and 128 columns, W e4m3 in fragment order with one per 128 x 128
-// block.
+// The dense fp8 block-scaled GEMM for any number of rows: y[M, n] bf16 = A[M, K] W[n, K]^T, A e4m3
+// row-major with a float32 scale per row and 128 columns, W e4m3 in fragment order with one per 128 x 128
+// block:  y = sum over 128-deep steps k of xs[m, k] ws[n / 128, k] (A_k W_k^T)[m, n].
+//
+// Bound, with many rows: the matrix cores at the clock that the chip's power leaves them (1.9 - 2.2 GHz
+// under this load), with a multiply-add of every product by its scale beside them and both operands
+// through LDS. A bare loop of 32 x 32 x 64 MFMAs and their scaling runs at 3.3 PFLOP/s on two waves a
+// SIMD, this kernel at 2.1 (8192 x 10240 x 2560 in 203 us; 2048 x 151936 x 2560 in 790, 2.0), the
+// library's fp8 product of 8192^3, which scales nothing, at 2.65. With few rows: the weights' read, and
+// below about 256 tiles the length of one (1.0 us a step of the largest alone).
+//
+//   * A tile is 256 x 256, 192 x 256 or 128 x 128; a wave has 32 x 32 tiles, up to 4 x 2 of them (64 columns
+//     of 128 rows), all in registers. W is the MFMA's first operand: a lane then holds one row of y, and its
+//     scale is one register. 32 x 32 x 64 and not 16 x 16 x 128: half the operand reads and instructions,
+//     3.3 against 2.8 PFLOP/s in the bare loop. Without scales the instruction is 8 bytes shorter.
+//   * A step's rows and weights come straight to LDS, two steps of them. Rows are stored by chunks of 16
+//     bytes, chunk q of row r at q ^ (r / 2 & 7): no bank conflicts (r & 7 instead: 13% of the cycles).
+//     The weights are already in fragment order. Three steps of LDS with a smaller tile: 1.4 PFLOP/s where
+//     two with this one had 1.7; one more step of weights alone (192 x 256) changed nothing.
+//   * The scaling of a 32 x 32 tile is issued behind the products of the next one, so that the vector unit
+//     works under the matrix cores; operand reads go out two at a time between products, ahead of need, and
+//     a step's loads one or two a tile: in one go after the barrier they kept every wave from its products
+//     (225 -> 209 us at 8192 x 10240). The second half of a row tile's depth is held once and not twice, and
+//     what a lane can recompute it does: with 8 registers more the loop spills, and a spill's reload waits
+//     for all loads to LDS (1.3 PFLOP/s).
+//   * The weights' scales are scalar loads, a step ahead and just before the barrier: their wait is one for
+//     every LDS read in flight. The rows' go to LDS, 8 steps at a time.
+//   * Measured against one another and slower: the two waves of a SIMD taking turns at products and LDS reads
+//     (1.56 PFLOP/s), products and scaling in the compiler's own order (1.7).
+//   * Output through LDS to 16-byte pieces, stored without a place in the L2 (2048 x
+//     151936: 895 against 915 us).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -33,8 +61,8 @@ __device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t b, int voff, int 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_ptr)dst, 4, voff, soff, 0, 0);
 }
 
-// Barrier behind which every wave's loads to LDS so far have arrived (the fence of a barrier alone
-// does not wait for them).
+// Barrier behind which every wave's loads to LDS so far but its last LEFT have arrived (the fence of a
+// barrier alone does not wait for them).
 template <int LEFT = 0>
 __device__ __forceinline__ void staged_barrier() {
   static_assert(LEFT < 64, "vmcnt has 6 bits");
@@ -63,9 +91,9 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
                                                            uint16_t* __restrict__ y,
                                                            long long ldy, int M, int n, int K) {
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* lx = lds;                                  // [2][BM rows][8 chunks of 16 B, swizzled]
-  uint8_t* lw = lds + C::ST * C::X;                       // [2][BN / 16 strips][2][64 lanes][16 B]
-  uint8_t* ls = lw + C::ST * C::W;                        // [2][BM / 8][8 rows][SC, swizzled] floats
+  uint8_t* lx = lds;                       // [ST][BM rows][8 chunks of 16 B, swizzled]
+  uint8_t* lw = lds + C::ST * C::X;        // [ST][BN / 16 strips][2][64 lanes][16 B]
+  uint8_t* ls = lw + C::ST * C::W;         // [2][BM / 8][8 rows][SC floats, swizzled]
   const int lane = lane_id();
   const int w = uniform((int)threadIdx.x / WAVE);
   const int nkg = K / 128;
@@ -140,12 +168,13 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
   };
   auto read_x = [&](int b, int t, int h) __attribute__((always_inline)) {
     const uint8_t* p = lx + b * C::X + t * 4096;
-    (h ? x1 : x0[t % C::SLOTS]) = pack8(*reinterpret_cast<const v4u*>(p + (ox ^ (64 * h))),
-                                 *reinterpret_cast<const v4u*>(p + (ox ^ (64 * h + 16))));
+    (h ? x1 : x0[t % C::SLOTS]) =
+        pack8(*reinterpret_cast<const v4u*>(p + (ox ^ (64 * h))),
+              *reinterpret_cast<const v4u*>(p + (ox ^ (64 * h + 16))));
   };
   auto read_s = [&](int kb, int t) __attribute__((always_inline)) {
     sx = *reinterpret_cast<const float*>(ps + t * 1024 + (kb / SC & 1) * C::S +
-                                                ((kb ^ (r + 2 * (r / 8))) & 7) * 4);
+                                         ((kb ^ (r + 2 * (r / 8))) & 7) * 4);
   };
   constexpr int T = C::WM * C::WN;
   // (a part staged behind step s's barrier has arrived at that of step s + ST - 1, before the reads for s + ST)

@@ -41,7 +41,9 @@ SHAPES = [(1, 1, 128), (1, 128, 256), (3, 5, 384), (17, 129, 1152), (63, 127, 12
           (65, 1, 128), (65, 7, 256), (127, 129, 384), (128, 128, 128), (129, 1543, 1152),
           (200, 4099, 384), (255, 256, 2048), (257, 257, 2560), (300, 9999, 128), (617, 1543, 768),
           (1025, 2600, 1152), (2100, 6145, 384), (4096, 2560, 256), (4100, 2561, 1152),
-          (700, 33000, 256), (1500, 40000, 1152), (193, 60000, 2048), (160, 151936, 256)]
+          (700, 33000, 256), (1500, 40000, 1152), (193, 60000, 2048), (160, 151936, 256),
+          # 31 and 97 steps, which the head's kernel does not take
+          (1024, 2561, 2560), (7, 300, 3968), (40, 129, 12416)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
