@@ -342,6 +342,7 @@ int rlu_moe_gemm_fp8blk_tiled_noalloc(const void* qx, const float* xs, const voi
  *   -inf logits have probability 0. A row of nothing else: log probabilities -inf, entropy 0.
  *   A row with a NaN or +inf: NaN, rank 0, ids -1.
  *   A token below 0 asks for none: logprob 0, rank 0. One >= V: logprob NaN, rank 0.
+ * A row's ends are read in whole 16 bytes, at addresses that are multiples of 16.
  * 1 <= V <= 500000, 0 <= top <= min(32, V). top_logprobs / top_ids [R, top] (NULL where top is 0). ws: what
  * the first call says, 8-byte aligned, used until the second call's kernels end. R = 0 launches nothing.
  * Returns -1 (bad sizes or a NULL pointer), -4 (misaligned logits). */

@@ -386,6 +386,16 @@ class PackedFp8:
     n: int               # output features
     k: int
 
+    def __post_init__(self):
+        n_pad = -(-self.n // GROUP) * GROUP
+        if self.n < 1 or self.k < 1 or self.k % GROUP or \
+                self.wq.shape != (n_pad, self.k) or self.wq.dtype != FP8 or \
+                self.ws.shape != (n_pad // GROUP, self.k // GROUP) or \
+                self.ws.dtype != torch.float32 or \
+                not (self.wq.is_contiguous() and self.ws.is_contiguous()):
+            raise ValueError(f"PackedFp8: contiguous e4m3 [{n_pad}, {self.k}] and float32 block "
+                             f"scales, not {tuple(self.wq.shape)} and {tuple(self.ws.shape)}")
+
     @property
     def n_pad(self) -> int:
         return self.wq.shape[0]

@@ -330,3 +330,30 @@ def test_head_logprobs_in_chunks_and_of_no_rows(mods, monkeypatch):
     again = head.logprobs(wide[:, ::2], t, 3)
     for a, b in zip(parts, again):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_head_logprobs_in_a_replayed_graph(mods, rows):
+    _, ops = mods
+    g = torch.Generator(DEV).manual_seed(rows)
+    head = ops.Fp8TargetHead(object(), torch.randn(1280, 512, generator=g, device=DEV).bfloat16())
+    xs = [torch.randn(rows, 512, generator=g, device=DEV).bfloat16() for _ in range(3)]
+    ts = [torch.randint(1280, (rows,), generator=g, device=DEV) for _ in range(3)]
+    gpu_case(f"head logprobs graph rows={rows}")
+    x, t, st = xs[0].clone(), ts[0].clone(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(st):
+        head.logprobs(x, t, 5)
+    st.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        out = head.logprobs(x, t, 5)
+    for i in (0, 1, 2, 1):
+        with torch.cuda.stream(st):
+            x.copy_(xs[i])
+            t.copy_(ts[i])
+            graph.replay()
+        want = head.logprobs(xs[i], ts[i], 5)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)

@@ -93,6 +93,19 @@ def test_pack_fp8_dense_refuses_types_and_devices(mods, fake):
             mods[0].pack_fp8_dense(w, ws)
 
 
+@pytest.mark.parametrize("bad", [
+    dict(wq=lambda e: e(100, 256, dtype=F8)), dict(wq=lambda e: e(128, 512, dtype=F8)),
+    dict(wq=lambda e: e(128, 256, dtype=BF)), dict(wq=lambda e: e(256, 128, dtype=F8).T),
+    dict(ws=lambda e: e(2, 2)), dict(ws=lambda e: e(1, 2, dtype=BF)), dict(ws=lambda e: e(1, 4)[:, ::2]),
+    dict(n=lambda e: 129), dict(n=lambda e: 0), dict(k=lambda e: 200)])
+def test_a_packed_weight_fits_its_sizes(mods, fake, bad):
+    args = dict(wq=fake(128, 256, dtype=F8), ws=fake(1, 2), n=100, k=256)
+    mods[0].PackedFp8(**args)
+    args.update({k: v(fake) for k, v in bad.items()})
+    with pytest.raises(ValueError):
+        mods[0].PackedFp8(**args)
+
+
 def test_head_logprobs_refuses(mods, fake):
     ops = mods[0]
     head = ops.Fp8TargetHead.__new__(ops.Fp8TargetHead)
