@@ -15,7 +15,6 @@ import torch
 
 from ._lib import check, lib, on_device, stream_ptr
 
-_P = ctypes.c_void_p
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_TOP = 32
 MAX_VOCAB = 500000
@@ -73,8 +72,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_n: int = 0) -
     ws = torch.empty(_workspace(code, rows, vocab, top_n), dtype=torch.uint8, device=dev)
     with on_device(dev):
         rc = lib().rlu_token_logprobs(
-            _P(logits.data_ptr()), code, logits.stride(0), rows, vocab, _P(tokens.data_ptr()),
-            int(tokens.dtype == torch.int64), top_n, *[_P(t.data_ptr()) for t in out],
-            _P(ws.data_ptr()), _P(stream_ptr()))
+            logits.data_ptr(), code, logits.stride(0), rows, vocab, tokens.data_ptr(),
+            int(tokens.dtype == torch.int64), top_n, *[t.data_ptr() for t in out], ws.data_ptr(),
+            stream_ptr())
     check(rc, "rlu_token_logprobs")
     return out

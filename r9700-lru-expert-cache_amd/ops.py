@@ -441,8 +441,9 @@ def gemm_fp8_dense(qx: torch.Tensor, xs: torch.Tensor, w: PackedFp8,
         raise ValueError("gemm_fp8_dense: operands on different devices")
     ldy = out.stride(0) if M > 1 else w.n
     with on_device(qx.device):
-        rc = lib().rlu_gemm_fp8blk_dense(_p(qx), _p(xs), _p(w.wq), _p(w.ws), _p(out), ldy, M, w.n,
-                                         K, _P(stream_ptr()))
+        rc = lib().rlu_gemm_fp8blk_dense(qx.data_ptr(), xs.data_ptr(), w.wq.data_ptr(),
+                                         w.ws.data_ptr(), out.data_ptr(), ldy, M, w.n, K,
+                                         stream_ptr())
     check(rc, "rlu_gemm_fp8blk_dense")
     return out
 
