@@ -378,7 +378,7 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       // a pass takes SRC threads' PER elements each
       constexpr int PER = CV * E::N, SRC = WAVE / PER;
       static_assert(SRC * PER == WAVE, "a wave's pass");
-      const int n = min(__popcll(todo), BATCH), e = lane % PER;
+      const int left = (int)__popcll(todo), n = left < BATCH ? left : BATCH, e = lane % PER;
       const int at0 = (v0 + e / E::N * NT) * E::N + e % E::N - shift;
       for (int a = lane / PER; a - lane / PER < n; a += SRC) {
         const float x =
@@ -417,8 +417,10 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       most = max(most, rcount[k]);
     }
     if (most <= CAP) {                     // each candidate's place is how many come before it
-      for (int j = lane; j < rcount[w]; j += WAVE) {
-        const uint64_t key = list[w][j];
+      const int c1 = rcount[0], c2 = c1 + rcount[1], c3 = c2 + rcount[2];
+      for (int j = tid; j < total; j += NT) {          // (mostly the first wave's alone)
+        const int of = (j >= c1) + (j >= c2) + (j >= c3);
+        const uint64_t key = list[of][j - (of == 0 ? 0 : of == 1 ? c1 : of == 2 ? c2 : c3)];
         int place = 0;
 #pragma unroll
         for (int k = 0; k < NW; ++k)
