@@ -5,8 +5,8 @@
 //
 // Bound: the read, 1.24 GB at 4096 x 151936 bf16 or 2048 x 151936 f32. float32 takes 187 + 5 us of it (6.6
 // TB/s; a bare read 7.0); in 16 bits there are twice the elements, and the vector unit is the limit where the
-// token is not among the highest (201 - 217 us against 257 - 261: the comparisons for its rank) and with
-// alternatives (20 of them: 265 - 313). An element is an unpacking, a multiply-add, an exponential (as
+// token is not among the highest (196 - 199 us against 220 - 267: the comparisons for its rank) and with
+// alternatives (20 of them: 252 - 282). An element is an unpacking, a multiply-add, an exponential (as
 // long as four others), an add and a multiply-add, 5 instructions of 9.5 in all.
 //
 //   * A row is cut into segments of 32 KB, a workgroup each, that stay in registers between the maximum and
