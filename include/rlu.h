@@ -191,7 +191,8 @@ int rlu_gemm_fp8blk_m64(const void* qx, const float* xs, const void* w, const fl
  * fp8_target_lmhead.py:31): y [M, n] bf16 (rows ldy elements apart) = qx [M, K] e4m3 (xs [M, K/128])
  * x w [n_pad, K]^T (ws [n_pad/128, K/128]), n_pad = n up to the next multiple of 128, w in fragment
  * order, for any M and n: one weight read per tile of rows. Elements outside [M, n] are not
- * written. M = 0 launches nothing. Returns -1 (bad sizes, ldy < n or a NULL pointer), -2 (K % 128). */
+ * written. M = 0 launches nothing. Returns -1 (bad sizes, ldy < n or a NULL pointer), -2 (K % 128),
+ * -4 (qx or w not at a multiple of 16 bytes, the others not at their elements'). */
 int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void* w, const float* ws, void* y,
                           long long ldy, int M, int n, int K, hipStream_t stream);
 
@@ -345,7 +346,8 @@ int rlu_moe_gemm_fp8blk_tiled_noalloc(const void* qx, const float* xs, const voi
  * A row's ends are read in whole 16 bytes, at addresses that are multiples of 16.
  * 1 <= V <= 500000, 0 <= top <= min(32, V). top_logprobs / top_ids [R, top] (NULL where top is 0). ws: what
  * the first call says, 8-byte aligned, used until the second call's kernels end. R = 0 launches nothing.
- * Returns -1 (bad sizes or a NULL pointer), -4 (misaligned logits). */
+ * Returns -1 (bad sizes, more than 2^24 - 1 workgroups for R rows, or a NULL pointer), -4 (misaligned logits
+ * or ws). */
 int rlu_token_logprobs_workspace(int dtype, int R, int V, int top, long long* bytes);
 int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V,
                        const void* tokens, int wide, int top, float* logprob, int* rank,

@@ -338,6 +338,8 @@ extern "C" int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void
   if (K % 128 || K > (1 << 22)) return -2;
   if (M == 0) return 0;
   if (!qx || !xs || !w || !ws || !y) return -1;
+  if (((uintptr_t)qx | (uintptr_t)w) % 16 || ((uintptr_t)xs | (uintptr_t)ws) % 4 || (uintptr_t)y % 2)
+    return -4;
   const auto* q = (const uint8_t*)qx;
   const auto* p = (const uint8_t*)w;
   auto* o = (uint16_t*)y;

@@ -596,7 +596,7 @@ extern "C" int rlu_token_logprobs_workspace(int dtype, int R, int V, int top, lo
       top > MAX_TOP || top > V)
     return -1;
   const long long segs = (long long)R * plan(dtype, R, V).nseg;
-  if (segs > INT32_MAX) return -1;
+  if (segs > UINT32_MAX / NT) return -1;               // (a launch counts its threads in 32 bits)
   *bytes = segs * (sizeof(Part) + 8 * top);
   return 0;
 }
@@ -612,7 +612,7 @@ extern "C" int rlu_token_logprobs(const void* logits, int dtype, long long ld, i
   if (R == 0) return 0;
   if (!logits || !tokens || !logprob || !rank || !entropy || !ws) return -1;
   if (top && (!top_logprobs || !top_ids)) return -1;
-  if ((uintptr_t)logits % (dtype == 1 ? 4 : 2)) return -4;
+  if ((uintptr_t)logits % (dtype == 1 ? 4 : 2) || (uintptr_t)ws % 8) return -4;
   const Plan pl = plan(dtype, R, V);
   const auto* x = (const uint8_t*)logits;
   auto* lists = (uint64_t*)ws;                         // (8-byte entries first: both aligned)

@@ -312,16 +312,16 @@ class Fp8TargetHead:
         """logprobs.TokenLogprobs of this head's logits for x [..., K] bf16 and tokens [...] (any number
         of rows, a prompt's too): quantized rows, gemm_fp8_dense and logprobs.token_logprobs,
         LOGPROBS_ROWS rows of logits at a time. Up to 64 rows the logits are apply's bit for bit."""
-        if x.dtype != torch.bfloat16 or x.shape[-1] != self.wq.shape[1]:
-            raise ValueError(f"logprobs takes bf16 rows of {self.wq.shape[1]}")
+        if x.dtype != torch.bfloat16 or x.shape[-1] != self.wq.shape[1] or \
+                x.device != self.wq.device:
+            raise ValueError(f"logprobs takes bf16 rows of {self.wq.shape[1]} beside the weight")
         if tokens.shape != x.shape[:-1]:
             raise ValueError(f"logprobs: tokens {tuple(tokens.shape)} for rows {tuple(x.shape[:-1])}")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError("logprobs has no gradient: detach the rows")
         w = PackedFp8(wq=self.wq, ws=self.ws, n=self.wq.shape[0], k=self.wq.shape[1])
-        flat, ids = x.reshape(-1, w.k), tokens.reshape(-1)
-        if flat.stride(1) != 1:
-            flat = flat.contiguous()
+        # (a single row may count as contiguous whatever its stride: not once it is flat)
+        flat, ids = x.reshape(-1).contiguous().view(-1, w.k), tokens.reshape(-1).contiguous()
         if not flat.shape[0]:
             parts = [token_logprobs(flat.new_empty((0, w.n)), ids, top_n)]
         else:

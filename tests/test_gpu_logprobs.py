@@ -357,3 +357,25 @@ def test_head_logprobs_in_a_replayed_graph(mods, rows):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [1, 4])
+def test_head_logprobs_of_strided_rows_and_tokens(mods, rows):
+    """Rows and tokens apart, at any stride, and one row expanded: as their copies."""
+    _, ops = mods
+    g = torch.Generator(DEV).manual_seed(rows)
+    head = ops.Fp8TargetHead(object(), torch.randn(256, 128, generator=g, device=DEV).bfloat16())
+    x = torch.randn(rows, 128, generator=g, device=DEV).bfloat16()
+    t = torch.randint(256, (rows,), generator=g, device=DEV)
+    gpu_case(f"head logprobs strided rows={rows}")
+    odd = torch.zeros(rows, 133, device=DEV).bfloat16()
+    odd[:, :128] = x
+    apart = torch.zeros(rows, 256, device=DEV).bfloat16()
+    apart[:, ::2] = x
+    ids = torch.zeros(rows, 3, dtype=torch.int64, device=DEV)
+    ids[:, 1] = t
+    for a, b, want in ((odd[:, :128], ids[:, 1], (x, t)), (apart[:, ::2], t, (x, t)),
+                       (x[:1].expand(rows, 128), t, (x[:1].repeat(rows, 1), t)),
+                       (x, t[:1].expand(rows), (x, t[:1].repeat(rows)))):
+        for p, q in zip(head.logprobs(a, b, 3), head.logprobs(*want, 3)):
+            assert torch.equal(p, q)

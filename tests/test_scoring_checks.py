@@ -112,7 +112,8 @@ def test_head_logprobs_refuses(mods, fake):
     head.wq, head.ws = fake(128, 256, dtype=F8), fake(1, 2)
     x, t = fake(2, 3, 256, dtype=BF), fake(2, 3, dtype=torch.int64)
     for a in ((fake(2, 3, 256), t), (fake(2, 3, 128, dtype=BF), t), (x, fake(6, dtype=torch.int64)),
-              (x, fake(2, dtype=torch.int64)), (fake(2, 3, 256, dtype=BF).requires_grad_(), t)):
+              (x, fake(2, dtype=torch.int64)), (fake(2, 3, 256, dtype=BF).requires_grad_(), t),
+              (fake(2, 3, 256, dtype=BF, device="cpu"), fake(2, 3, dtype=torch.int64, device="cpu"))):
         with pytest.raises(ValueError):
             head.logprobs(*a)
 
@@ -129,6 +130,8 @@ def test_gemm_return_codes(lib):
     assert call(p, p, p, p, p, 2 ** 31 - 1, 4, 2 ** 31 - 1, 256, n) == -1
     for i in range(5):
         assert call(*[n if j == i else p for j in range(5)], 100, 4, 100, 256, n) == -1
+    for i, off in enumerate((8, 2, 8, 2, 1)):                        # qx, xs, w, ws, y
+        assert call(*[P(4096 + off) if j == i else p for j in range(5)], 100, 4, 100, 256, n) == -4
 
 
 def test_logprobs_return_codes(lib):
@@ -139,9 +142,10 @@ def test_logprobs_return_codes(lib):
     assert ws(0, 4, 151936, 20, b) == 0 and size.value > 0
     assert ws(0, 0, 151936, 20, b) == 0 and size.value == 0
     for a in ((3, 4, 100, 0), (-1, 4, 100, 0), (0, -1, 100, 0), (0, 4, 0, 0), (0, 4, 500001, 0),
-              (0, 4, 100, -1), (0, 4, 100, 33), (0, 4, 5, 6), (0, 2 ** 31 - 1, 151936, 0)):
+              (0, 4, 100, -1), (0, 4, 100, 33), (0, 4, 5, 6), (0, 2 ** 31 - 1, 151936, 0),
+              (0, 2 ** 24, 100, 0)):                                  # past 2^32 threads
         assert ws(*a, b) == -1
-    assert ws(0, 4, 100, 0, n) == -1
+    assert ws(0, 4, 100, 0, n) == -1 and ws(0, 2 ** 24 - 1, 100, 0, b) == 0
 
     def call(x=p, dtype=0, ld=100, rows=4, vocab=100, tok=p, wide=1, top=2, out=(p,) * 5, work=p):
         return lib.rlu_token_logprobs(x, dtype, ld, rows, vocab, tok, wide, top, *out, work, n)
@@ -151,6 +155,7 @@ def test_logprobs_return_codes(lib):
     for i in range(5):
         assert call(out=[n if j == i else p for j in range(5)]) == -1
     assert call(x=P(4097)) == -4 and call(x=P(4098), dtype=1) == -4
+    assert call(work=P(4100)) == -4
 
 
 @pytest.mark.parametrize("dtype,elems", [(0, 8), (1, 4), (2, 8)])
