@@ -36,7 +36,7 @@ typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 constexpr int NT = 256, NW = NT / WAVE;    // threads and waves of a segment's workgroup
 constexpr int MAX_TOP = 32, MAX_V = 500000;
 constexpr int MAX_SEGS = WAVE;             // a row's segments, one to a lane of the joining wave
-constexpr int BATCH = 16, CAP = 256;       // threads a wave lists from at a time, candidates it lists
+constexpr int CAP = 256;                   // candidates a wave lists
 constexpr float L2E = 1.44269504f;
 constexpr double LN2 = 0.693147180559945309;
 
@@ -226,8 +226,9 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   __shared__ int rbefore[NW], rcount[NW];
   __shared__ v4u one[CV];
   __shared__ uint64_t list[TOP ? NW : 1][TOP ? CAP : 1], rkey[NW];
-  __shared__ v4u near[TOP ? NW : 1][TOP ? BATCH * CV : 1];
-  __shared__ int near_tid[TOP ? NW : 1][TOP ? BATCH : 1];
+  constexpr int BATCH = WAVE / CV;         // threads a wave lists from at a time
+  __shared__ v4u near[TOP ? NW : 1][TOP ? WAVE : 1];
+  __shared__ int near_v[TOP ? NW : 1][TOP ? BATCH : 1], hit[TOP ? NW : 1][TOP ? WAVE : 1];
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE);
   const int row = (int)(blockIdx.x / (unsigned)nseg), seg = (int)(blockIdx.x % (unsigned)nseg);
   const uint8_t* p = logits + (size_t)row * ld * E::SIZE;
@@ -361,7 +362,8 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   }
   __syncthreads();
   if (TOP) {
-    // the elements from there on, of the threads that have any, BATCH threads at a time
+    // the elements from there on: of the threads that have any, BATCH at a time, their vectors that do
+    // (a lane a vector), and of those the elements (a lane each)
     const float from = rfrom;
     forget(raw);
     uint64_t todo = __ballot(tm >= from);
@@ -372,21 +374,25 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
       if (mine) {
 #pragma unroll
         for (int k = 0; k < CV; ++k) near[w][at * CV + k] = raw[k];
-        near_tid[w][at] = tid;
+        near_v[w][at] = v0 + tid;
       }
       wave_lds_sync();
-      // a pass takes SRC threads' PER elements each
-      constexpr int PER = CV * E::N, SRC = WAVE / PER;
-      static_assert(SRC * PER == WAVE, "a wave's pass");
-      const int left = (int)__popcll(todo), n = left < BATCH ? left : BATCH, e = lane % PER;
-      const int at0 = (v0 + e / E::N * NT) * E::N + e % E::N - shift;
-      for (int a = lane / PER; a - lane / PER < n; a += SRC) {
-        const float x =
-            a < n ? load_one<DT>((const uint8_t*)near[w], a * PER + e) : -__builtin_inff();
-        const uint64_t in = __ballot(x >= from);
-        const int to = count + mbcnt(in);
-        if (x >= from && to < CAP) list[w][to] = entry(x, at0 + near_tid[w][a] * E::N);
-        count += __popcll(in);
+      const int left = (int)__popcll(todo), n = left < BATCH ? left : BATCH;
+      const v4u one_v[1] = {near[w][lane]};
+      const bool has = lane < n * CV && Max<DT, 1>::of(one_v) >= from;
+      const uint64_t hits = __ballot(has);
+      const int nh = (int)__popcll(hits);
+      if (has) hit[w][mbcnt(hits)] = lane;
+      wave_lds_sync();
+      for (int i = lane / E::N; i - lane / E::N < nh; i += WAVE / E::N) {
+        const int of = hit[w][i < nh ? i : 0], e = lane % E::N;
+        const float x = load_one<DT>((const uint8_t*)(near[w] + of), e);
+        const bool in = i < nh && x >= from;
+        const uint64_t all = __ballot(in);
+        const int to = count + mbcnt(all);
+        if (in && to < CAP)
+          list[w][to] = entry(x, (near_v[w][of / CV] + of % CV * NT) * E::N + e - shift);
+        count += (int)__popcll(all);
       }
       wave_lds_sync();
       todo &= ~__ballot(mine);
