@@ -273,18 +273,17 @@ __global__ __launch_bounds__(NT) void segment_k(const uint8_t* __restrict__ logi
   float om[NW], m;                         // the lane's threads of all waves
 #pragma unroll
   for (int k = 0; k < NW; ++k) om[k] = rtm[k * WAVE + lane];
-  m = wave_max(fmaxf(fmaxf(om[0], om[1]), fmaxf(om[2], om[3])));
+  const float gm = fmaxf(fmaxf(om[0], om[1]), fmaxf(om[2], om[3]));
+  m = wave_max(gm);
   if (TOP && w == 0) {
-    // a value that `top` threads have an element at or above: the upper 16 bits of the top-th largest of
-    // their maxima, bit by bit
+    // a value that `top` of 64 groups of threads have an element at or above: the upper 16 bits of the
+    // top-th largest of their maxima, bit by bit
+    const uint32_t key = key_of(gm);
     uint32_t at = 0;
 #pragma unroll
     for (int b = 15; b >= 0; --b) {
       const uint32_t c = at | 1u << b;
-      int n = 0;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) n += __popcll(__ballot(key_of(om[k]) >= c << 16));
-      if (n >= top) at = c;
+      if ((int)__popcll(__ballot(key >= c << 16)) >= top) at = c;
     }
     if (lane == 0) rfrom = at > 0x7fu ? of_key(at << 16) : -FLT_MAX;     // (finite ones only)
   }
