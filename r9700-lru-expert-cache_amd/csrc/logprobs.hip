@@ -4,10 +4,11 @@
 //   rank = 1 + #{x > x_t} + #{j < t: x_j = x_t}, alternatives by value, the lowest index first.
 //
 // Bound: the read, 1.24 GB at 4096 x 151936 bf16 or 2048 x 151936 f32. float32 takes 187 + 5 us of it (6.6
-// TB/s; a bare read 7.0); in 16 bits there are twice the elements, and the vector unit is the limit where the
-// token is not among the highest (196 - 199 us against 220 - 267: the comparisons for its rank) and with
-// alternatives (20 of them: 252 - 282). An element is an unpacking, a multiply-add, an exponential (as
-// long as four others), an add and a multiply-add, 5 instructions of 9.5 in all.
+// TB/s; a bare read 7.0). In 16 bits there are twice the elements and the vector unit has no cycle left, either:
+// 195 - 210 us in a row of calls, up to 260 in the first milliseconds after other work; with 20 alternatives it
+// is the limit, 240 - 265. An element is an unpacking, a multiply-add, an exponential (as long as four others),
+// an add and a multiply-add, half an operation of the maximum and for the rank a comparison, 9.5 in all. Where
+// the token is among the highest the comparisons are left out: 3%.
 //
 //   * A row is cut into segments of 32 KB, a workgroup each, that stay in registers between the maximum and
 //     the sums: no running rescaling, and eight workgroups' loads in flight a CU. Shorter ones where there
@@ -18,9 +19,12 @@
 //   * The maximum's own term is left out of Z: in a nearly certain row 1 + 1e-9 is 1, and entropy and the
 //     likeliest token's log probability would be 0. Its thread's elements are summed again by its wave, an
 //     element a lane (by a second pass of all, where Z came near 1: 230 us where this takes 201).
-//   * The alternatives of a segment are its elements at or above the n-th largest of its 256 threads' maxima,
-//     a little over n of them; the n-th largest of a wave's 64 lets three times as many through. Lists of
-//     fixed length hold them; longer runs of equal logits are walked one by one.
+//   * The alternatives of a segment are its elements at or above the n-th largest of the maxima of 64 groups
+//     of four threads, a little over n of them (of all 256 threads: 21 instead of 24 where n is 20, and four
+//     times the comparisons, 268 us for 265; of each wave's own 64: three times as many). They are looked for
+//     among the vectors of the threads that have any, a lane a vector, and there a lane an element (a lane an
+//     element throughout: 278 for 265). Lists of fixed length hold them; longer runs of equal logits are walked
+//     one by one.
 #include <float.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -623,15 +627,27 @@ extern "C" int rlu_token_logprobs(const void* logits, int dtype, long long ld, i
   auto* lists = (uint64_t*)ws;                         // (8-byte entries first: both aligned)
   auto* parts = (Part*)(lists + (size_t)R * pl.nseg * top);
   const dim3 grid((unsigned)(R * pl.nseg));
-#define RLU_SEG(DT, CV, TOP)                                                                       hipLaunchKernelGGL((segment_k<DT, CV, TOP>), grid, dim3(NT), 0, stream, x, ld, V, pl.nseg,                          tokens, wide, top, parts, lists)
+#define RLU_SEG(DT, CV, TOP)                                                                       \
+  hipLaunchKernelGGL((segment_k<DT, CV, TOP>), grid, dim3(NT), 0, stream, x, ld, V, pl.nseg,       \
+                     tokens, wide, top, parts, lists)
 #define RLU_JOIN(DT, K)                                                                          \
   hipLaunchKernelGGL((join_k<DT, K>), dim3((unsigned)R), dim3(rlu::WAVE),                        \
                      top ? (pl.nseg * top + rlu::WAVE) * 8 : 0, stream, x, ld, V, pl.nseg, tokens, \
                      wide, top, parts, lists, logprob, rank, entropy, top_logprobs, top_ids)
-#define RLU_CV(DT, TOP)                 do {                                    if (pl.cv == 8) RLU_SEG(DT, 8, TOP);          else if (pl.cv == 4) RLU_SEG(DT, 4, TOP);     else if (pl.cv == 2) RLU_SEG(DT, 2, TOP);     else RLU_SEG(DT, 1, TOP);                   } while (0)
-#define RLU_DT(DT)                                                                                do {                                                                                              if (top) RLU_CV(DT, true);                                                                      else RLU_CV(DT, false);                                                                         if (pl.nseg * top <= 4 * rlu::WAVE) RLU_JOIN(DT, 4);                                        \
-    else if (pl.nseg * top <= 12 * rlu::WAVE) RLU_JOIN(DT, 12);                                 \
-    else RLU_JOIN(DT, 32);                                                                      \
+#define RLU_CV(DT, TOP)                                                                            \
+  do {                                                                                             \
+    if (pl.cv == 8) RLU_SEG(DT, 8, TOP);                                                           \
+    else if (pl.cv == 4) RLU_SEG(DT, 4, TOP);                                                      \
+    else if (pl.cv == 2) RLU_SEG(DT, 2, TOP);                                                      \
+    else RLU_SEG(DT, 1, TOP);                                                                      \
+  } while (0)
+#define RLU_DT(DT)                                                                                 \
+  do {                                                                                             \
+    if (top) RLU_CV(DT, true);                                                                     \
+    else RLU_CV(DT, false);                                                                        \
+    if (pl.nseg * top <= 4 * rlu::WAVE) RLU_JOIN(DT, 4);                                           \
+    else if (pl.nseg * top <= 12 * rlu::WAVE) RLU_JOIN(DT, 12);                                    \
+    else RLU_JOIN(DT, 32);                                                                         \
   } while (0)
   if (dtype == 0) RLU_DT(0);
   else if (dtype == 1) RLU_DT(1);

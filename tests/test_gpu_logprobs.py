@@ -122,6 +122,27 @@ def test_equal_logits_go_by_index(score, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V", [(7, 3001), (16, 16387), (40, 33001), (200, 33001)])
+def test_candidates_around_a_lists_length(score, dtype, R, V):
+    """So many elements at the highest value that a wave lists from none to all of its threads, and up to and past
+    the 256 that its list holds; a few higher ones in every other row."""
+    g = torch.Generator(DEV).manual_seed(R + V)
+    share = torch.tensor([0.001, 0.004, 0.01, 0.02, 0.04, 0.06, 0.0625, 0.07, 0.1, 0.2], device=DEV)
+    f = 2.0 * torch.rand(R, V, generator=g, device=DEV)
+    many = torch.rand(R, V, generator=g, device=DEV) < share.repeat(-(-R // 10))[:R, None]
+    f[many] = 4.0
+    f[::2].scatter_(1, torch.randint(V, (len(f[::2]), 4), generator=g, device=DEV), 6.0)
+    f[::3] -= 9.0
+    x = f.to(TYPES[dtype])
+    tok = torch.randint(V, (R,), generator=g, device=DEV)
+    gpu_case(f"logprobs candidates {dtype} R={R} V={V}")
+    for top in (1, 3, 20, 32):
+        got = score(x, tok, top)
+        torch.cuda.synchronize()
+        check(got, x, tok, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V,offset", [(50, 0), (3000, 1), (70001, 3)])
 def test_masked_rows(score, dtype, V, offset):
     """-inf everywhere, but for one, for fewer than the alternatives, for most; the type's lowest value in
