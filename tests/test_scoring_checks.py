@@ -65,9 +65,9 @@ def test_token_logprobs_refuses(mods, fake, bad):
     dict(qx=lambda e: e(1024, dtype=F8)),
     dict(xs=lambda e: e(4, 1)), dict(xs=lambda e: e(3, 2)),
     dict(xs=lambda e: e(2, 4).T), dict(xs=lambda e: e(4, 2, dtype=BF)),
-    dict(xs=lambda e: e(4, 2, device="cpu")),
+    dict(xs=lambda e: e(4, 2, device="cpu")), dict(xs=lambda e: e(4, 2).requires_grad_()),
     dict(out=lambda e: e(4, 101, dtype=BF)), dict(out=lambda e: e(4, 100)),
-    dict(out=lambda e: e(100, 4, dtype=BF).T),
+    dict(out=lambda e: e(100, 4, dtype=BF).T), dict(out=lambda e: e(4, 100, dtype=BF).requires_grad_()),
     dict(out=lambda e: e(1, 100, dtype=BF).expand(4, 100)),          # rows on top of each other
     dict(out=lambda e: e(4, 100, dtype=BF, device="cpu"))])
 def test_gemm_fp8_dense_refuses(mods, fake, bad):
