@@ -418,7 +418,7 @@ def pack_fp8_dense(w: torch.Tensor, ws: torch.Tensor) -> PackedFp8:
     rows[:n] = w.view(torch.uint8)
     with on_device(w.device):
         wq = shuffle_fp8_weight(rows.view(FP8))
-    return PackedFp8(wq=wq, ws=ws.contiguous(), n=n, k=k)
+    return PackedFp8(wq=wq, ws=ws.detach().contiguous(), n=n, k=k)
 
 
 def gemm_fp8_dense(qx: torch.Tensor, xs: torch.Tensor, w: PackedFp8,
