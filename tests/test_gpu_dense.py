@@ -136,6 +136,17 @@ def test_packed_weight_is_padded_with_zeros(ops):
     assert torch.equal(ops.shuffle_fp8_weight(rows.view(F8)).view(torch.uint8), p.wq.view(torch.uint8))
 
 
+def test_block_scales_of_a_parameter(ops):
+    """A layer's scales may ask for a gradient: the packed ones do not, and the product takes them."""
+    qx, xs, w, ws = whole(20, 256, 256, 5)
+    gpu_case("dense, a parameter's scales")
+    p = ops.pack_fp8_dense(w, torch.nn.Parameter(ws))
+    assert not p.ws.requires_grad
+    y = ops.gemm_fp8_dense(qx, xs, p)
+    torch.cuda.synchronize()
+    assert torch.equal(y, exact(qx, xs, w, ws).to(BF))
+
+
 @pytest.mark.parametrize("M,N,K", [(48, 300, 1152), (300, 1543, 768), (2100, 6145, 384)])
 def test_other_streams_and_graph_replays(ops, M, N, K):
     """Two captured graphs replayed at once on two streams with new rows each time, beside eager calls."""
