@@ -409,6 +409,12 @@ int rlu_selftest_silu(unsigned long long* bad, hipStream_t stream);
  * 0, -1 (bad sizes or NULL), -2 (K % 128, K < 512, or rows * K past 2 GB). */
 int rlu_selftest_prefill_rows(int rows, int K, unsigned long long* bad);
 
+/* On the host, without a GPU: the dense GEMM's loads, over the tiles of each of its shapes that M rows and n
+ * columns end in, that would touch memory past the last row, column block or step if only the vector offset
+ * counted in a buffer's range check, and those of the operands that would be dropped if the scalar one did,
+ * too. Returns 0, -1 (bad sizes or NULL), -2 (K % 128, or K past 2^22). */
+int rlu_selftest_dense_loads(int M, int n, int K, unsigned long long* bad);
+
 /* Likewise: the weight steps of K (128 deep) that a workgroup of that kernel loads for `items` items.
  * Returns 0, -1 (bad sizes or NULL), -2 (K % 128 or K < 512). */
 int rlu_selftest_prefill_steps(int items, int K, unsigned long long* steps);

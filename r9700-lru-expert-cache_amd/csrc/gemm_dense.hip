@@ -83,6 +83,45 @@ struct Cfg {
   static constexpr int LDS = ST * (X + W) + 2 * S;
 };
 
+// A wave's loads of step kb, one at a time: j counts XI of rows (8 each, 8 lanes a row), then WI of half strips
+// of weights; row_scales is one of XI parts, of the SC steps from kb on. ld(e, at, bytes, voffset, soffset): piece
+// e of the step, through a buffer of `bytes` from byte `at` of the tile's operand on. Only the vector offset is
+// sure to count in a buffer's range check, so what decides whether there is such a row lies in the base and the
+// vector offset, the scalar one moves within a row or a strip alone, and past the last step or strip the buffer
+// is empty: such a load touches no memory. (Masks, and one buffer for all rows of a wave and one for its strips: a
+// condition is made a branch, with which the loop spills, and a buffer each took 20 scalar instructions more a
+// step: 768 x 2560 x 2048 14.5 us, this 13.9.)
+// A row's chunk q lies at q ^ (row / 2 & 7), so that 16 rows' reads of one chunk meet all 64 banks (by row & 7,
+// row r and r + 8 shared theirs).
+template <class C>
+__host__ __device__ __forceinline__ int row_lane(int w, int lane, int K, int j) {
+  return (8 * j + lane / 8) * K + ((lane ^ (8 * (w * C::XI + j) + lane / 8) / 2) & 7) * 16;
+}
+template <class C, class LD>
+__host__ __device__ __forceinline__ void row_or_weights(int w, int lane, const int (&vx)[C::XI],
+                                                        int rows, int cols, int K, int kb, int j,
+                                                        const LD& ld) {
+  const int live = (kb - K / 128) >> 31;
+  if (j < C::XI) {
+    const int r0 = 8 * w * C::XI;
+    ld(w * C::XI + j, r0 * K, max(0, rows - r0) * K & live, vx[j], kb * 128);
+  } else {
+    const int e = w * C::WI + j - C::XI, c0 = w * C::WI / 2 * 16;
+    static_assert(128 % (C::WI * 8) == 0 && C::WI % 2 == 0, "a wave's strips are there together");
+    ld(e, c0 * K, (c0 < cols ? C::WI * 8 * K : 0) & live, lane * 16 + (j - C::XI) / 2 * 16 * K,
+       kb * 2048 + (e & 1) * 1024);
+  }
+}
+template <class C, class LD>
+__host__ __device__ __forceinline__ void row_scales(int w, int lane, int rows, int K, int kb, int i,
+                                                    const LD& ld) {
+  const int nkg = K / 128, e = w * C::XI + i, j = (lane ^ (lane / 8 + 2 * e)) & 7;
+  const int r0 = 8 * w * C::XI;
+  // (SC steps on from kb: past a row's last they are the next one's, and not used)
+  ld(e, (r0 * nkg + kb) * 4, max(0, (rows - r0) * nkg - kb) * 4 & (kb - nkg) >> 31,
+     ((8 * i + lane / 8) * nkg + j) * 4, 0);
+}
+
 template <class C>
 __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __restrict__ qx,
                                                            const float* __restrict__ xs,
@@ -110,32 +149,31 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
   const uint8_t* gx = qx + (size_t)m0 * K;
   const uint8_t* gw = wq + (size_t)n0 * K;
   const float* gs = xs + (size_t)m0 * nkg;
-  // past the last step the buffers have no bytes: such a load touches no memory
-  auto buf = [&](const void* p, int bytes, bool live) __attribute__((always_inline)) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, live ? bytes : 0, BUF_WORD3);
+  auto buf = [&](const void* p, int at, int bytes) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)p + (unsigned)at), 0, bytes,
+                                             BUF_WORD3);
   };
-  // a wave's loads take 8 rows, 8 lanes a row; a row's chunk q lies at q ^ (row / 2 & 7), so that 16
-  // rows' reads of one chunk meet all 64 banks (by row & 7, row r and r + 8 shared theirs)
-  const int vx = lane / 8 * K + ((lane ^ (lane / 16 + (w * C::XI & 1) * 4)) & 7) * 16;
-  const int vw = lane * 16;
-  // A step's loads, one at a time: XI of rows, WI of half strips, and a part of the row scales that the
-  // steps from the next multiple of SC on read (the last part again once all are on their way).
+  int vx[C::XI];
+#pragma unroll
+  for (int j = 0; j < C::XI; ++j) vx[j] = row_lane<C>(w, lane, K, j);
+  // A step's loads: XI + WI, and a part of the row scales that the steps from the next multiple of SC on read
+  // (the last part again once all are on their way).
   constexpr int PIECES = C::XI + C::WI + 1;
   auto scales = [&](int b, int kb, int i) __attribute__((always_inline)) {
-    const int e = w * C::XI + i;
-    const int j = (lane ^ (lane / 8 + 2 * e)) & 7;
-    to_lds4(buf(gs, rows * nkg * 4, kb < nkg), (lane / 8 * nkg + j) * 4, (e * 8 * nkg + kb) * 4,
-            ls + b * C::S + e * 256);
+    row_scales<C>(w, lane, rows, K, kb, i,
+                  [&](int e, int at, int bytes, int voff, int soff) __attribute__((always_inline)) {
+      to_lds4(buf(gs, at, bytes), voff, soff, ls + b * C::S + e * 256);
+    });
   };
   auto piece = [&](int b, int kb, int j) __attribute__((always_inline)) {
-    if (j < C::XI) {
-      const int e = w * C::XI + j;
-      to_lds16(buf(gx, rows * K, kb < nkg), vx ^ (j % 2 * 64), e * 8 * K + kb * 128,
-               lx + b * C::X + e * 1024);
-    } else if (j < C::XI + C::WI) {
-      const int e = w * C::WI + j - C::XI;             // half a strip's step
-      to_lds16(buf(gw, cols * K, kb < nkg), vw,
-               (e / 2) * nkg * 2048 + kb * 2048 + (e & 1) * 1024, lw + b * C::W + e * 1024);
+    if (j < C::XI + C::WI) {
+      const bool x = j < C::XI;
+      row_or_weights<C>(w, lane, vx, rows, cols, K, kb, j,
+                        [&](int e, int at, int bytes, int voff, int soff)
+                            __attribute__((always_inline)) {
+        to_lds16(buf(x ? gx : gw, at, bytes), voff, soff,
+                 (x ? lx + b * C::X : lw + b * C::W) + e * 1024);
+      });
     } else {
       const int s = kb - C::ST, c = (s >> 3) + 1;
       static_assert(SC == 8, "s >> 3");
@@ -316,6 +354,51 @@ static int launch(hipStream_t st, const uint8_t* qx, const float* xs, const uint
   return (int)hipGetLastError();
 }
 
+// The loads of a tile of `rows` x `cols` (weights' rows, by whole 16) of K by which dense_k would touch memory
+// that it has no use for (all past the last step, row or strip; of the scales those behind the last row's), with
+// only the vector offset in a buffer's range check, and those of its operands that a check of the vector and the
+// scalar offset would drop.
+template <class C>
+static unsigned long long loads_wrong(int rows, int cols, int K) {
+  unsigned long long bad = 0;
+  const int nkg = K / 128;
+  for (int w = 0; w < C::NW; ++w)
+    for (int lane = 0; lane < WAVE; ++lane) {
+      // own: the byte to load, -1 for none
+      auto count = [&](long long own, int at, int bytes, int voff, int soff, int n) {
+        const long long to = (long long)at + voff + soff;
+        if (own < 0 ? voff < bytes : to != own || (long long)voff + soff + n > bytes) ++bad;
+      };
+      int vx[C::XI];
+      for (int j = 0; j < C::XI; ++j) vx[j] = row_lane<C>(w, lane, K, j);
+      for (int kb = 0; kb < nkg + C::ST + SC; ++kb) {
+        const bool live = kb < nkg;
+        for (int j = 0; j < C::XI + C::WI; ++j)
+          row_or_weights<C>(w, lane, vx, rows, cols, K, kb, j,
+                            [&](int e, int at, int bytes, int voff, int soff) {
+            if (j < C::XI) {                           // row r's chunk q lies at q ^ (r / 2 & 7)
+              const int r = 8 * e + lane / 8, q = (lane ^ r / 2) & 7;
+              count(live && r < rows ? (long long)r * K + kb * 128 + q * 16 : -1, at, bytes, voff,
+                    soff, 16);
+            } else {                                   // half h of strip s
+              const int s = e / 2, h = e % 2;
+              count(live && 16 * s < cols ? (long long)(s * nkg + kb) * 2048 + h * 1024 + lane * 16
+                                          : -1,
+                    at, bytes, voff, soff, 16);
+            }
+          });
+        for (int i = 0; i < C::XI && kb % SC == 0; ++i)
+          row_scales<C>(w, lane, rows, K, kb, i, [&](int e, int at, int bytes, int voff, int soff) {
+            // step kb + j of row r at j ^ (r + 2 (r / 8)) & 7
+            const int r = 8 * e + lane / 8, j = (lane ^ (r + r / 8 * 2)) & 7;
+            const long long to = ((long long)r * nkg + kb + j) * 4;
+            count(live && to < (long long)rows * nkg * 4 ? to : -1, at, bytes, voff, soff, 4);
+          });
+      }
+    }
+  return bad;
+}
+
 typedef Cfg<4, 2, 2, 4, 2> Big;        // 256 x 256, one workgroup a CU
 typedef Cfg<3, 2, 2, 4, 2> Mid;        // 192 x 256, one
 typedef Cfg<2, 2, 2, 2, 2> Small;      // 128 x 128, two
@@ -372,4 +455,20 @@ extern "C" int rlu_gemm_fp8blk_dense(const void* qx, const float* xs, const void
     return dense::launch<dense::Small>(stream, q, xs, p, ws, o, ldy, M, n, K);
   if (tile == mid) return dense::launch<dense::Mid>(stream, q, xs, p, ws, o, ldy, M, n, K);
   return dense::launch<dense::Big>(stream, q, xs, p, ws, o, ldy, M, n, K);
+}
+
+// Host only: counts into *bad, over the tiles of each shape that M x n ends in, the loads that would touch
+// memory they should not with only the vector offset in the buffers' range check, and the operands' that
+// would be dropped with both offsets in it. Returns -1 (bad sizes or NULL), -2 (K % 128 or too large).
+extern "C" int rlu_selftest_dense_loads(int M, int n, int K, unsigned long long* bad) {
+  using namespace rlu::dense;
+  if (M < 1 || n < 1 || K < 1 || n > INT32_MAX - 256 || !bad) return -1;
+  if (K % 128 || K > (1 << 22)) return -2;
+  auto last = [&](auto c) {
+    typedef decltype(c) C;
+    const int rows = (M - 1) % C::BM + 1, cols = ((n + 127) / 128 * 128 - 1) % C::BN + 1;
+    return loads_wrong<C>(rows, cols, K);
+  };
+  *bad = last(Big()) + last(Mid()) + last(Small());
+  return 0;
 }
