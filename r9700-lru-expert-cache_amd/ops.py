@@ -439,7 +439,7 @@ def gemm_fp8_dense(qx: torch.Tensor, xs: torch.Tensor, w: PackedFp8,
         raise ValueError(f"gemm_fp8_dense: out must be bf16 [{M}, {w.n}] with rows apart")
     if not xs.device == w.wq.device == w.ws.device == out.device == qx.device:
         raise ValueError("gemm_fp8_dense: operands on different devices")
-    if torch.is_grad_enabled() and (xs.requires_grad or w.ws.requires_grad or out.requires_grad):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (qx, xs, w.wq, w.ws, out)):
         raise ValueError("gemm_fp8_dense has no gradient: detach its operands")
     ldy = out.stride(0) if M > 1 else w.n
     with on_device(qx.device):

@@ -78,6 +78,17 @@ def test_gemm_fp8_dense_refuses(mods, fake, bad):
         mods[0].gemm_fp8_dense(**args)
 
 
+@pytest.mark.parametrize("which", ["qx", "wq"])
+def test_gemm_fp8_dense_refuses_fp8_operands_that_ask_for_a_gradient(mods, fake, which):
+    """A tensor that asks for one still does when it is cast to e4m3."""
+    t = dict(qx=fake(4, 256, dtype=F8), wq=fake(128, 256, dtype=F8))
+    t[which] = torch.empty(t[which].shape, device="cuda").requires_grad_().to(F8)
+    assert t[which].requires_grad
+    w = mods[0].PackedFp8(wq=t["wq"], ws=fake(1, 2), n=100, k=256)
+    with pytest.raises(ValueError, match="gradient"):
+        mods[0].gemm_fp8_dense(t["qx"], fake(4, 2), w)
+
+
 @pytest.mark.parametrize("w,ws", [((100, 256), (1, 1)), ((129, 256), (1, 2)), ((100, 200), (1, 2)),
                                   ((0, 256), (0, 2)), ((100, 0), (1, 0)), ((100,), (1, 2))])
 def test_pack_fp8_dense_refuses(mods, fake, w, ws):
