@@ -87,8 +87,13 @@ def lib() -> ctypes.CDLL:
 
 def stream_ptr(stream=None) -> int:
     import torch
-    if stream is None:       # without building a Stream object for it: 0.3 us, not 2.9
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if stream is None:
+        # without building a Stream object for it: 0.3 us, not 2.9. (Not of torch's public interface: a
+        # torch that lacks it builds the object.)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            return raw(torch.cuda.current_device())
+        stream = torch.cuda.current_stream()
     return stream.cuda_stream
 
 
