@@ -61,26 +61,24 @@ __device__ __forceinline__ void to_lds4(__amdgpu_buffer_rsrc_t b, int voff, int 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (lds_ptr)dst, 4, voff, soff, 0, 0);
 }
 
-// Barrier behind which every wave's loads to LDS so far but its last LEFT have arrived (the fence of a
-// barrier alone does not wait for them).
-template <int LEFT = 0>
+// Barrier behind which every wave's loads to LDS so far have arrived (the fence of a barrier alone does not
+// wait for them).
 __device__ __forceinline__ void staged_barrier() {
-  static_assert(LEFT < 64, "vmcnt has 6 bits");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (LEFT & 15) | (LEFT >> 4) << 14);        // vmcnt(LEFT)
+  __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0)
   lds_barrier();
 }
 
 // A wave has WM x WN tiles of 32 rows x 32 columns, a workgroup GM x GN waves.
-template <int WM_, int WN_, int GM_, int GN_, int ST_>
+template <int WM_, int WN_, int GM_, int GN_>
 struct Cfg {
-  static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_, ST = ST_;
+  static constexpr int WM = WM_, WN = WN_, GM = GM_, GN = GN_;
   static constexpr int BM = 32 * WM * GM, BN = 32 * WN * GN, NW = GM * GN;
   static constexpr int X = BM * 128, W = BN * 128;              // bytes of a step
   static constexpr int S = BM * SC * 4;                         // bytes of SC steps' row scales
   static constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW;      // loads of a wave
   static_assert(XI * 8 * NW == BM && WI * 8 * NW == BN, "the waves share the loads evenly");
   static constexpr int SLOTS = WM % 2 ? WM : 2;                 // row tiles' operands held
-  static constexpr int LDS = ST * (X + W) + 2 * S;
+  static constexpr int LDS = 2 * (X + W) + 2 * S;
 };
 
 // A wave's loads of step kb, one at a time: j counts XI of rows (8 each, 8 lanes a row), then WI of half strips
@@ -130,9 +128,9 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
                                                            uint16_t* __restrict__ y,
                                                            long long ldy, int M, int n, int K) {
   extern __shared__ __align__(16) uint8_t lds[];
-  uint8_t* lx = lds;                       // [ST][BM rows][8 chunks of 16 B, swizzled]
-  uint8_t* lw = lds + C::ST * C::X;        // [ST][BN / 16 strips][2][64 lanes][16 B]
-  uint8_t* ls = lw + C::ST * C::W;         // [2][BM / 8][8 rows][SC floats, swizzled]
+  uint8_t* lx = lds;                       // [2][BM rows][8 chunks of 16 B, swizzled]
+  uint8_t* lw = lds + 2 * C::X;            // [2][BN / 16 strips][2][64 lanes][16 B]
+  uint8_t* ls = lw + 2 * C::W;             // [2][BM / 8][8 rows][SC floats, swizzled]
   const int lane = lane_id();
   const int w = uniform((int)threadIdx.x / WAVE);
   const int nkg = K / 128;
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
                  (x ? lx + b * C::X : lw + b * C::W) + e * 1024);
       });
     } else {
-      const int s = kb - C::ST, c = (s >> 3) + 1;
+      const int s = kb - 2, c = (s >> 3) + 1;
       static_assert(SC == 8, "s >> 3");
       scales(c & 1, c * SC, min(s & 7, C::XI - 1));
     }
@@ -215,20 +213,20 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
                                          ((kb ^ (r + 2 * (r / 8))) & 7) * 4);
   };
   constexpr int T = C::WM * C::WN;
-  // (a part staged behind step s's barrier has arrived at that of step s + ST - 1, before the reads for s + ST)
-  static_assert(C::XI <= SC - C::ST + 1, "all parts are there when the next SC steps begin");
-  // Behind a step's barrier its buffer is free for step kb + ST, whose loads go out a few in each of the
+  // (a part staged behind step s's barrier has arrived at that of step s + 1, before the reads for s + 2)
+  static_assert(C::XI <= SC - 1, "all parts are there when the next SC steps begin");
+  // Behind a step's barrier its buffer is free for step kb + 2, whose loads go out a few in each of the
   // WINDOW tiles from there on: in one go they kept every wave from its products.
   constexpr int WINDOW = T - 3 > C::WN ? T - 3 : C::WN, PER = (PIECES + WINDOW - 1) / WINDOW;
-  // the step whose operands are in buffer b; bp, bn: the buffers of the steps before and after it
-  auto step = [&](int bp, int b, int bn, int kb) __attribute__((always_inline)) {
+  // the step whose operands are in buffer b; the steps before and after it have buffer bn
+  auto step = [&](int b, int bn, int kb) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < T; ++i) {
       const int t = i / C::WN, u = i % C::WN;          // a tile, and in p the one before it
       const int p = (i + T - 1) % T;
       const bool last = t + 1 == C::WM;
       if (last && u == 0) {
-        staged_barrier<(C::ST - 2) * PIECES>();
+        staged_barrier();
         __builtin_amdgcn_sched_barrier(0);
       }
       // the next row tile's operands are read between the products, a few at a time
@@ -255,7 +253,7 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
       const int q = (i + C::WN) % T;                   // tiles since the barrier
 #pragma unroll
       for (int j = q * PER; j < (q + 1) * PER && j < PIECES; ++j)
-        piece(last ? b : bp, last ? kb + C::ST : kb - 1 + C::ST, j);
+        piece(last ? b : bn, last ? kb + 2 : kb + 1, j);
       __builtin_amdgcn_sched_barrier(0x3f4);
       acc[p / C::WN][p % C::WN] = __builtin_elementwise_fma(
           d[(i + 1) & 1], (v16f)(f[p / C::WN % C::SLOTS]), acc[p / C::WN][p % C::WN]);
@@ -267,10 +265,10 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
 #pragma unroll
   for (int i = 0; i < C::XI; ++i) scales(0, 0, i);
 #pragma unroll
-  for (int i = 0; i < C::ST; ++i)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < PIECES - 1; ++j)
-      if (i + 1 < C::ST || j < C::WN * PER) piece(i, i, j);
+      if (i == 0 || j < C::WN * PER) piece(i, i, j);
   staged_barrier();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -282,10 +280,9 @@ __global__ __launch_bounds__(C::NW * WAVE, 2) void dense_k(const uint8_t* __rest
 #pragma unroll
   for (int k = 0; k < 16; ++k) d[1][k] = 0.f;
   f[(C::WM - 1) % C::SLOTS] = 0.f;
-  for (int kb = 0, bp = C::ST - 1, b = 0; kb < nkg; ++kb) {
-    const int bn = b + 1 == C::ST ? 0 : b + 1;
-    step(bp, b, bn, kb);
-    bp = b;
+  for (int kb = 0, b = 0; kb < nkg; ++kb) {
+    const int bn = b ^ 1;
+    step(b, bn, kb);
     b = bn;
   }
   acc[C::WM - 1][C::WN - 1] = __builtin_elementwise_fma(
@@ -371,7 +368,7 @@ static unsigned long long loads_wrong(int rows, int cols, int K) {
       };
       int vx[C::XI];
       for (int j = 0; j < C::XI; ++j) vx[j] = row_lane<C>(w, lane, K, j);
-      for (int kb = 0; kb < nkg + C::ST + SC; ++kb) {
+      for (int kb = 0; kb < nkg + 2 + SC; ++kb) {
         const bool live = kb < nkg;
         for (int j = 0; j < C::XI + C::WI; ++j)
           row_or_weights<C>(w, lane, vx, rows, cols, K, kb, j,
@@ -399,9 +396,9 @@ static unsigned long long loads_wrong(int rows, int cols, int K) {
   return bad;
 }
 
-typedef Cfg<4, 2, 2, 4, 2> Big;        // 256 x 256, one workgroup a CU
-typedef Cfg<3, 2, 2, 4, 2> Mid;        // 192 x 256, one
-typedef Cfg<2, 2, 2, 2, 2> Small;      // 128 x 128, two
+typedef Cfg<4, 2, 2, 4> Big;           // 256 x 256, one workgroup a CU
+typedef Cfg<3, 2, 2, 4> Mid;           // 192 x 256, one
+typedef Cfg<2, 2, 2, 2> Small;       // 128 x 128, two
 
 // tiles of a shape that the fullest CU gets
 template <class C>
