@@ -400,3 +400,31 @@ def test_head_logprobs_of_strided_rows_and_tokens(mods, rows):
                        (x, t[:1].expand(rows), (x, t[:1].repeat(rows)))):
         for p, q in zip(head.logprobs(a, b, 3), head.logprobs(*want, 3)):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("shape,N,K,rows", [((600,), 1024, 256, 256), ((3, 700), 1280, 512, 1024),
+                                            ((129,), 2048, 384, 64), ((65,), 1152, 2560, 1),
+                                            ((5, 3), 1152, 256, 15)])
+def test_head_logprobs_are_those_of_its_chunks(mods, monkeypatch, shape, N, K, rows):
+    """Every field, bit for bit, of the two calls on each `rows` rows, joined in order."""
+    lp, ops = mods
+    g = torch.Generator(DEV).manual_seed(N + K + rows)
+    head = ops.Fp8TargetHead(object(), (torch.randn(N, K, generator=g, device=DEV) * 0.1).bfloat16())
+    x = torch.randn(*shape, K, generator=g, device=DEV).bfloat16()
+    t = torch.randint(N, shape, generator=g, device=DEV)
+    monkeypatch.setattr(ops, "LOGPROBS_ROWS", rows)
+    gpu_case(f"head logprobs chunks {shape} N={N} K={K} rows={rows}")
+    got = head.logprobs(x, t, 6)
+    flat, ids = x.reshape(-1, K), t.reshape(-1)
+    w = ops.PackedFp8(wq=head.wq, ws=head.ws, n=N, k=K)
+    at = 0
+    for r in range(0, flat.shape[0], rows):
+        logits = ops.gemm_fp8_dense(*ops.fp8_quant_group(flat[r:r + rows]), w)
+        want = lp.token_logprobs(logits, ids[r:r + rows], 6)
+        torch.cuda.synchronize()
+        check(want, logits, ids[r:r + rows], 6)
+        for name, a, b in zip(lp.TokenLogprobs._fields, got, want):
+            part = a.reshape(flat.shape[0], *a.shape[len(shape):])[at:at + b.shape[0]]
+            assert torch.equal(part, b), (name, r)
+        at += want.logprob.shape[0]
+    assert at == flat.shape[0] and all(a.shape[:len(shape)] == shape for a in got)
