@@ -5,7 +5,7 @@
 // Bound, with many rows: the matrix cores at the clock that the chip's power leaves them (1.75 - 1.8 GHz
 // under this load), with a multiply-add of every product by its scale beside them and both operands
 // through LDS. A bare loop of 32 x 32 x 64 MFMAs and their scaling runs at 3.3 PFLOP/s on two waves a
-// SIMD, this kernel at 2.1 (8192 x 10240 x 2560 in 196 - 207 us; 2048 x 151936 x 2560 in 757 - 817, 2.0), the
+// SIMD, this kernel at 2.1 (8192 x 10240 x 2560 in 194 - 207 us; 2048 x 151936 x 2560 in 757 - 838, 2.0), the
 // library's fp8 product of 8192^3, which scales nothing, at 2.65. With few rows: the weights' read, and
 // below about 256 tiles the length of one (1.0 us a step of the largest alone).
 //

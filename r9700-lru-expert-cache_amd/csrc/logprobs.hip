@@ -11,9 +11,9 @@
 // the token is among the highest the comparisons are left out: 3%.
 //
 //   * A row is cut into segments of 32 KB, a workgroup each, that stay in registers between the maximum and
-//     the sums: no running rescaling, and eight workgroups' loads in flight a CU. Shorter ones where there
-//     would be under 256 (32 / 16 / 8 KB: 20 rows with 20 alternatives 14.1 / 13.9 / 15.0 us, one row without
-//     7.7 / 6.4 / 6.1). A wave a row then joins them, 4 - 8 us, nearly all of it the chain of its steps.
+//     the sums: no running rescaling, and eight workgroups' loads in flight a CU (52 VGPRs; with alternatives 67,
+//     and seven). Shorter ones where there would be under 256 (32 / 16 / 8 KB: 20 rows with 20 alternatives
+//     14.1 / 13.9 / 15.0 us, one row without 7.7 / 6.4 / 6.1). A wave a row then joins them, 4 - 8 us, nearly all of it the chain of its steps.
 //   * 16-bit logits are unpacked again for each pass and their maximum is taken packed: held unpacked they
 //     took 256 VGPRs, and 4096 rows with 20 alternatives 1589 us, then 423.
 //   * The maximum's own term is left out of Z: in a nearly certain row 1 + 1e-9 is 1, and entropy and the
@@ -23,8 +23,11 @@
 //     of four threads, a little over n of them (of all 256 threads: 21 instead of 24 where n is 20, and four
 //     times the comparisons, 268 us for 265; of each wave's own 64: three times as many). They are looked for
 //     among the vectors of the threads that have any, a lane a vector, and there a lane an element (a lane an
-//     element throughout: 278 for 265). Lists of fixed length hold them; longer runs of equal logits are walked
-//     one by one.
+//     element throughout: 278 for 265). Lists of fixed length hold them.
+//   * Where a wave has more candidates than its list holds, the segment is read again once for each alternative.
+//     That happens to runs of equal logits, to segments masked with a finite value of which fewer than n groups
+//     keep anything else, and to float32 rows whose spread is lost in 16 bits (100 +- 0.1). 256 x 151936, 20 / 5 / 1
+//     alternatives: 800 - 865 / 255 / 90 - 103 us, masked with -inf instead 35 - 40 us.
 #include <float.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -284,8 +284,8 @@ def gemm_fp8_block(x: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor) -> torch
 FP8_LMHEAD_MAX_M = int(os.environ.get("VLLM_TARGET_FP8_LMHEAD_MAX_M", "64"))
 
 
-# rows of logits that Fp8TargetHead.logprobs holds at a time: 311 MB at vocab 151936, where the product
-# already runs at its full rate
+# rows of logits that Fp8TargetHead.logprobs holds at a time: 311 MB at vocab 151936. 4096 rows x 2560, 5
+# alternatives, 512 / 1024 / 2048 / 4096 at a time: 2071 / 1966 / 1864 / 1811 us
 LOGPROBS_ROWS = 1024
 
 
