@@ -354,6 +354,42 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
                        float* entropy, float* top_logprobs, int* top_ids, void* ws,
                        hipStream_t stream);
 
+/* ---- losses over logits ----------------------------------------------------------------------------
+ * No counterpart in the reference. Of each of R rows of logits [R, V] (dtype, ld and V as for
+ * rlu_token_logprobs) a loss and, where grad is not NULL, the gradient of the losses' sum: [R, V] of the
+ * logits' type, rows ldg elements apart (>= V), at any element's address, nothing written beside them; it may be
+ * the logits themselves (same address and ld), but must not overlap them otherwise. p = softmax(x / temperature),
+ * weight [R] f32 or NULL (1). A row of weight 0 is not read: loss, log probability and gradient are 0.
+ *   policy_loss: lp = ln p of the row's token (int64 if wide 1, int32 if 0), rho = e^(lp - old), adv its advantage,
+ *     loss = weight (-min(rho adv, clamp(rho, 1 - clip_low, 1 + clip_high) adv) + kl (e^(ref - lp) - (ref - lp) - 1)),
+ *     without the last term where kl is 0 or ref_logprobs NULL. Also lp itself, [R]. A token below 0 is none (a
+ *     padded row): as weight 0. One >= V: NaN.
+ *   distill_top: top_ids [R, top] int32 (below 0: none; >= V: NaN row), top_logprobs [R, top].
+ *     rest 1: q = e^top_logprobs and one outcome more, all tokens not listed, of probability 1 - sum q (0 where
+ *     that is negative): loss = weight sum q ln(q / p) over the listed and that one. Where no unlisted token has a
+ *     probability the last has no term.
+ *     rest 0: q = softmax(top_logprobs / temperature) over the listed, which may be logits.
+ *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf: NaN throughout.
+ * 0 <= clip_low <= 1, clip_high >= 0, 0 <= kl < inf, temperature > 0 and 1 / temperature finite, 1 <= top <= 32. ws:
+ * what the first call says (top 1 for the policy loss), 8-byte aligned, used until the call's kernels end.
+ * R = 0 launches nothing. Returns -1 (bad sizes or arguments, more than 2^23 - 1 workgroups, or a NULL pointer),
+ * -4 (misaligned logits, grad or ws). */
+int rlu_loss_workspace(int dtype, int R, int V, int top, long long* bytes);
+int rlu_policy_loss(const void* logits, int dtype, long long ld, int R, int V, const void* tokens,
+                    int wide, const float* old_logprobs, const float* advantages,
+                    const float* ref_logprobs, const float* weight, float clip_low,
+                    float clip_high, float kl, float temperature, float* loss, float* logprob,
+                    void* grad, long long ldg, void* ws, hipStream_t stream);
+int rlu_distill_top(const void* logits, int dtype, long long ld, int R, int V, const int* top_ids,
+                    const float* top_logprobs, int top, int rest, const float* weight,
+                    float temperature, float* loss, void* grad, long long ldg, void* ws,
+                    hipStream_t stream);
+
+/* x [R, V] (dtype and rows as the gradient's above) times by[r * step] in place, row by row; rows whose factor
+ * is 1 are not touched. Returns -1, -4 as those. */
+int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* by,
+                   long long step, hipStream_t stream);
+
 /* Replaces the closed r4d_gemm_w4a16_nt_m64 behind draft_w4_lmhead_gemm / gemm_w4a16
  * (kernels/draft_w4_lmhead.py:351-403), in this build's gfx950 W4 format:
  *   y [M, N] bf16 = x [M, K] bf16 . (scale * (q - zero))^T, 1 <= M <= 16,

@@ -18,6 +18,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_long
 _LL = ctypes.c_longlong
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); one line per export of include/rlu.h
 SIGNATURES: dict[str, tuple] = {
@@ -40,6 +41,10 @@ SIGNATURES: dict[str, tuple] = {
     "rlu_gemm_fp8blk_dense": (_I, [_P] * 5 + [_LL] + [_I] * 3 + [_P]),
     "rlu_token_logprobs_workspace": (_I, [_I] * 4 + [_P]),
     "rlu_token_logprobs": (_I, [_P, _I, _LL, _I, _I, _P, _I, _I] + [_P] * 7),
+    "rlu_loss_workspace": (_I, [_I] * 4 + [_P]),
+    "rlu_policy_loss": (_I, [_P, _I, _LL, _I, _I, _P, _I] + [_P] * 4 + [_F] * 4 + [_P] * 3 + [_LL, _P, _P]),
+    "rlu_distill_top": (_I, [_P, _I, _LL, _I, _I, _P, _P, _I, _I, _P, _F, _P, _P, _LL, _P, _P]),
+    "rlu_scale_rows": (_I, [_P, _I, _LL, _I, _I, _P, _LL, _P]),
     "rlu_gemm_w4_m16": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _P]),
     "rlu_gemm_w4_m64": (_I, [_P, _I, _I, _P, _P, _P, _I, _P]),
     "rlu_pack_w4": (_I, [_P, _I, _LL, _I, _I, _I, _P, _P, _P]),
