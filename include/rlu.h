@@ -390,6 +390,23 @@ int rlu_distill_top(const void* logits, int dtype, long long ld, int R, int V, c
 int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* by,
                    long long step, hipStream_t stream);
 
+/* ---- low-rank adapters ---------------------------------------------------------------------------------
+ * No counterpart in the reference: n adapters beside one projection, a [n][R][K], b [n][N][R], scale [n] f32.
+ * dtype 0 bf16, 2 f16. 1 <= n <= 1024, 1 <= R <= 128, 1 <= K, N <= 2^24. R columns, K and N may be odd, every 16-bit
+ * operand lies at any element's address, its rows ld elements apart.
+ * rlu_lora_plan: a batch's rows by adapter, once for all its projections. ids [rows] int64 (wide 1) or int32: below
+ *   0 none, n or more: the row becomes NaN. size: rows of a tile, 16 or 64. cap = rows / size + min(rows, n + 2).
+ *   order [rows], tiles [cap][4] (16-byte aligned), first [n + 3]: for the calls below, which trust them.
+ * rlu_lora_add: hidden [rows][R] f32 = scale x a^T (0 in rows without an adapter), out [rows][N] = y + hidden b^T
+ *   (y in those), with two launches. out may be y (same address and ld), but overlaps nothing else.
+ * rows = 0 launches nothing. Returns -1 (bad sizes, more than 2^32 threads, or a NULL pointer), -4 (misaligned). */
+int rlu_lora_plan(const void* ids, int wide, int rows, int n, int size, int cap, int* order,
+                  int* tiles, int* first, hipStream_t stream);
+int rlu_lora_add(const void* x, long long ldx, const void* a, const void* b, const float* scale,
+                 int dtype, const int* order, const int* tiles, const int* first, int rows, int n,
+                 int size, int cap, int K, int N, int R, float* hidden, const void* y,
+                 long long ldy, void* out, long long ldo, hipStream_t stream);
+
 /* Replaces the closed r4d_gemm_w4a16_nt_m64 behind draft_w4_lmhead_gemm / gemm_w4a16
  * (kernels/draft_w4_lmhead.py:351-403), in this build's gfx950 W4 format:
  *   y [M, N] bf16 = x [M, K] bf16 . (scale * (q - zero))^T, 1 <= M <= 16,

@@ -1,0 +1,164 @@
+"""Low-rank adapters of many requests beside a shared, frozen projection, on librlu.so: for each row the
+adapter that its request asks for, out = y + s (x A^T) B^T, and the backward pass that trains them.
+
+No counterpart in the reference. The projection itself is whatever gave y: ops.gemm_fp8_dense, the heads, or
+any product of the caller's; rows, adapters and outputs are bf16 or f16.
+
+  plan_rows      a batch's rows by adapter: once, for all the projections that the batch passes
+  add_lora       for serving (in place or into another tensor), and for autograd in eager code
+  add_lora_grad  the backward pass by hand, also in a captured graph
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import check, lib, on_device, stream_ptr
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 2}
+MAX_RANK = 128
+MAX_ADAPTERS = 1024
+MAX_FEATURES = 1 << 24
+
+
+@dataclass(frozen=True)
+class LoraStack:
+    """n adapters of one projection: hold this on the layer. Adapters of a lower rank are padded with zeros."""
+    a: torch.Tensor        # [n, rank, K] bf16 or f16
+    b: torch.Tensor        # [n, N, rank], the same type
+    scale: torch.Tensor    # f32 [n], usually alpha / rank
+
+    def __post_init__(self):
+        a, b, s = self.a, self.b, self.scale
+        if a.ndim != 3 or b.ndim != 3 or a.dtype not in _DTYPE_CODE or b.dtype != a.dtype or \
+                s.dtype != torch.float32 or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[1] or \
+                s.shape != a.shape[:1] or not (a.is_contiguous() and b.is_contiguous() and
+                                               s.is_contiguous()):
+            raise ValueError("LoraStack: contiguous bf16 or f16 a [n, rank, K] and b [n, N, rank] with "
+                             f"float32 scale [n], not {tuple(a.shape)}, {tuple(b.shape)}, {tuple(s.shape)}")
+        if not a.is_cuda or b.device != a.device or s.device != a.device:
+            raise ValueError("LoraStack: all on one GPU")
+        if not (1 <= self.n <= MAX_ADAPTERS and 1 <= self.rank <= MAX_RANK and
+                1 <= a.shape[2] <= MAX_FEATURES and 1 <= b.shape[1] <= MAX_FEATURES):
+            raise ValueError(f"LoraStack: {tuple(a.shape)}, {tuple(b.shape)}: 1..{MAX_ADAPTERS} adapters of rank "
+                             f"1..{MAX_RANK} over 1..{MAX_FEATURES} features")
+        if s.requires_grad:
+            raise ValueError("LoraStack: the scale has no gradient")
+
+    @property
+    def n(self) -> int:
+        return self.a.shape[0]
+
+    @property
+    def rank(self) -> int:
+        return self.a.shape[1]
+
+
+@dataclass(frozen=True)
+class LoraRows:
+    """A batch's rows by adapter, as the kernels read them (plan_rows makes it)."""
+    order: torch.Tensor    # int32 [rows]: the rows of adapter 0, of adapter 1, ...; without one; ids past the last
+    tiles: torch.Tensor    # int32 [cap, 4]
+    first: torch.Tensor    # int32 [n + 3]
+    rows: int
+    n: int                 # adapters that the ids count
+    size: int              # rows of a tile
+
+
+def plan_rows(ids: torch.Tensor, n: int) -> LoraRows:
+    """ids [rows] int32 or int64, the adapter of each of a batch's rows in a stack of n: below 0 none; a row whose id
+    is n or more becomes NaN. Reads ids on the GPU, without a synchronisation."""
+    if ids.ndim != 1 or ids.dtype not in (torch.int32, torch.int64) or not ids.is_cuda or \
+            not ids.is_contiguous():
+        raise ValueError("plan_rows takes contiguous int32 or int64 ids [rows] on the GPU")
+    if not 1 <= n <= MAX_ADAPTERS:
+        raise ValueError(f"plan_rows: {n} adapters, not 1..{MAX_ADAPTERS}")
+    rows, dev = ids.shape[0], ids.device
+    if rows > 1 << 24:
+        raise ValueError(f"plan_rows: {rows} rows, at most {1 << 24}")
+    # few rows: tiles of 16 (most adapters have fewer); many: an adapter's factors are read once for 64
+    size = 16 if rows < 1024 else 64
+    cap = rows // size + min(rows, n + 2)
+    order = torch.empty(rows, dtype=torch.int32, device=dev)
+    tiles = torch.empty((cap, 4), dtype=torch.int32, device=dev)
+    first = torch.empty(n + 3, dtype=torch.int32, device=dev)
+    with on_device(dev):
+        rc = lib().rlu_lora_plan(ids.data_ptr(), int(ids.dtype == torch.int64), rows, n, size, cap,
+                                 order.data_ptr(), tiles.data_ptr(), first.data_ptr(), stream_ptr())
+    check(rc, "rlu_lora_plan")
+    return LoraRows(order, tiles, first, rows, n, size)
+
+
+def _check_rows(name: str, what: str, t: torch.Tensor, rows: int, cols: int, w: LoraStack) -> None:
+    if t.shape != (rows, cols) or t.dtype != w.a.dtype or t.device != w.a.device or \
+            (cols > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: {what} must be {w.a.dtype} [{rows}, {cols}] beside the adapters, a row's elements "
+                         "next to each other")
+
+
+def _check_batch(name: str, w: LoraStack, rows: LoraRows) -> None:
+    if rows.n != w.n or rows.order.device != w.a.device:
+        raise ValueError(f"{name}: rows planned for {rows.n} adapters on {rows.order.device}, a stack of {w.n} "
+                         f"on {w.a.device}")
+
+
+def _check_hidden(name: str, hidden: torch.Tensor, rows: int, w: LoraStack) -> None:
+    if hidden.shape != (rows, w.rank) or hidden.dtype != torch.float32 or \
+            not hidden.is_contiguous() or hidden.device != w.a.device or hidden.requires_grad:
+        raise ValueError(f"{name}: hidden must be contiguous float32 [{rows}, {w.rank}] beside the adapters")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes that t's rows reach over."""
+    size, (rows, cols) = t.element_size(), t.shape
+    return t.data_ptr(), t.data_ptr() + ((rows - 1) * t.stride(0) + cols) * size if rows else t.data_ptr()
+
+
+def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
+    (a, b), (c, d) = _span(s), _span(t)
+    return a < d and c < b
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _forward(y, x, w, rows, hidden, out) -> None:
+    if rows.rows == 0:
+        return
+    with on_device(x.device):
+        rc = lib().rlu_lora_add(
+            x.data_ptr(), _ld(x), w.a.data_ptr(), w.b.data_ptr(), w.scale.data_ptr(),
+            _DTYPE_CODE[x.dtype], rows.order.data_ptr(), rows.tiles.data_ptr(), rows.first.data_ptr(),
+            rows.rows, w.n, rows.size, rows.tiles.shape[0], x.shape[1], y.shape[1], w.rank,
+            hidden.data_ptr(), y.data_ptr(), _ld(y), out.data_ptr(), _ld(out), stream_ptr())
+    check(rc, "rlu_lora_add")
+
+
+def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
+             out: torch.Tensor | None = None, hidden: torch.Tensor | None = None) -> torch.Tensor:
+    """y [rows, N] + scale (x [rows, K] a^T) b^T with each row's adapter, all of the stack's type; sums and
+    x a^T in float32, rounded once. Rows may be apart (x, y and out of any stride). A row without an adapter is y's.
+    out: where the result goes, y itself among others; a new tensor without it.
+    hidden: float32 [rows, rank] that receives scale x a^T, for add_lora_grad."""
+    _check_batch("add_lora", w, rows)
+    _check_rows("add_lora", "x", x, rows.rows, w.a.shape[2], w)
+    _check_rows("add_lora", "y", y, rows.rows, w.b.shape[1], w)
+    if hidden is not None:
+        _check_hidden("add_lora", hidden, rows.rows, w)
+    if out is not None:
+        _check_rows("add_lora", "out", out, rows.rows, w.b.shape[1], w)
+        if rows.rows > 1 and out.stride(0) < out.shape[1]:
+            raise ValueError("add_lora: out's rows overlap")
+        same = out.data_ptr() == y.data_ptr() and _ld(out) == _ld(y)
+        if (not same and _overlap(out, y)) or _overlap(out, x):
+            raise ValueError("add_lora: out overlaps y or x (it may be y, or apart from both)")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, w.a, w.b)):
+        raise ValueError("add_lora has no gradient: detach its operands")
+    if hidden is None:
+        hidden = torch.empty((rows.rows, w.rank), dtype=torch.float32, device=x.device)
+    if out is None:
+        out = torch.empty((rows.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+    _forward(y, x, w, rows, hidden, out)
+    return out
