@@ -399,6 +399,9 @@ int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* 
  *   order [rows], tiles [cap][4] (16-byte aligned), first [n + 3]: for the calls below, which trust them.
  * rlu_lora_add: hidden [rows][R] f32 = scale x a^T (0 in rows without an adapter), out [rows][N] = y + hidden b^T
  *   (y in those), with two launches. out may be y (same address and ld), but overlaps nothing else.
+ * rlu_lora_grad: from dy [rows][N] and hidden as rlu_lora_add left it, with u = scale dy b: dx [rows][K] = u a (0 in
+ *   rows without an adapter), da = u^T x, db = dy^T hidden of each adapter over its rows (0 for one without rows);
+ *   each may be NULL. ws: what rlu_lora_grad_workspace says, 16-byte aligned, used until the kernels end.
  * rows = 0 launches nothing. Returns -1 (bad sizes, more than 2^32 threads, or a NULL pointer), -4 (misaligned). */
 int rlu_lora_plan(const void* ids, int wide, int rows, int n, int size, int cap, int* order,
                   int* tiles, int* first, hipStream_t stream);
@@ -406,6 +409,13 @@ int rlu_lora_add(const void* x, long long ldx, const void* a, const void* b, con
                  int dtype, const int* order, const int* tiles, const int* first, int rows, int n,
                  int size, int cap, int K, int N, int R, float* hidden, const void* y,
                  long long ldy, void* out, long long ldo, hipStream_t stream);
+int rlu_lora_grad_workspace(int dtype, int rows, int n, int size, int cap, int K, int N, int R,
+                            long long* bytes);
+int rlu_lora_grad(const void* dy, long long lddy, const void* x, long long ldx, const void* a,
+                  const void* b, const float* scale, int dtype, const int* order, const int* tiles,
+                  const int* first, int rows, int n, int size, int cap, int K, int N, int R,
+                  const float* hidden, void* dx, long long lddx, void* da, void* db, void* ws,
+                  hipStream_t stream);
 
 /* Replaces the closed r4d_gemm_w4a16_nt_m64 behind draft_w4_lmhead_gemm / gemm_w4a16
  * (kernels/draft_w4_lmhead.py:351-403), in this build's gfx950 W4 format:

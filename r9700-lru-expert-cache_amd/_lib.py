@@ -47,6 +47,8 @@ SIGNATURES: dict[str, tuple] = {
     "rlu_scale_rows": (_I, [_P, _I, _LL, _I, _I, _P, _LL, _P]),
     "rlu_lora_plan": (_I, [_P] + [_I] * 5 + [_P] * 4),
     "rlu_lora_add": (_I, [_P, _LL, _P, _P, _P, _I, _P, _P, _P] + [_I] * 7 + [_P, _P, _LL, _P, _LL, _P]),
+    "rlu_lora_grad_workspace": (_I, [_I] * 8 + [_P]),
+    "rlu_lora_grad": (_I, [_P, _LL, _P, _LL, _P, _P, _P, _I, _P, _P, _P] + [_I] * 7 + [_P, _P, _LL] + [_P] * 4),
     "rlu_gemm_w4_m16": (_I, [_P, _I, _I, _P, _P, _P, _I, _I, _P]),
     "rlu_gemm_w4_m64": (_I, [_P, _I, _I, _P, _P, _P, _I, _P]),
     "rlu_pack_w4": (_I, [_P, _I, _LL, _I, _I, _I, _P, _P, _P]),

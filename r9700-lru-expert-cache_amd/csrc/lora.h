@@ -98,5 +98,41 @@ struct Split {
   }
 };
 
+// A row of h or u, R floats, as fragments of both its parts: of the lane's 8 ranks of each 32. Returns by what sums
+// with them are multiplied: float16's were brought into its range by a power of two.
+template <int DT, int KS>
+__device__ __forceinline__ float split_row(const float* row, int R, int g, v4u (&hi)[KS], v4u (&lo)[KS]) {
+  float h[KS][8], m = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int r = 32 * k + 8 * g + e;
+      h[k][e] = r < R ? row[r] : 0.f;
+      m = fmaxf(m, fabsf(h[k][e]));
+    }
+  float by = 1.f;
+  if (DT != 0) {
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    by = scale_to(m);
+  }
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const Split<DT> p(h[k][e] * by), q(h[k][e + 1] * by);
+      hi[k][e / 2] = p.hi | q.hi << 16;
+      lo[k][e / 2] = p.lo | q.lo << 16;
+    }
+  return 1.f / by;
+}
+
+static inline bool sizes_ok(int dtype, int rows, int n, int size, int cap, int K, int N, int R) {
+  return (dtype == 0 || dtype == 2) && rows >= 0 && n >= 1 && n <= MAX_ADAPTERS &&
+         (size == 16 || size == 64) && K >= 1 && N >= 1 && K <= 1 << 24 && N <= 1 << 24 && R >= 1 &&
+         R <= MAX_RANK && cap == (int)(rows / size + (rows < n + 2 ? rows : n + 2));
+}
+
 }  // namespace lora
 }  // namespace rlu

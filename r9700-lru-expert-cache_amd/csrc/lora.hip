@@ -181,33 +181,8 @@ __global__ __launch_bounds__(256) void expand_k(Fwd f, int strips) {
   v4u hi[MT][KS], lo[MT][KS];
   float back[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    float h[KS][8], m = 0.f;
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int r = 32 * k + 8 * g + e;
-        h[k][e] = r < f.R ? f.hidden[(size_t)row[i] * f.R + r] : 0.f;
-        m = fmaxf(m, fabsf(h[k][e]));
-      }
-    float by = 1.f;
-    back[i] = 1.f;
-    if (DT != 0) {
-      m = fmaxf(m, __shfl_xor(m, 16));
-      m = fmaxf(m, __shfl_xor(m, 32));
-      by = scale_to(m);
-      back[i] = 1.f / by;
-    }
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const Split<DT> p(h[k][e] * by), q(h[k][e + 1] * by);
-        hi[i][k][e / 2] = p.hi | q.hi << 16;
-        lo[i][k][e / 2] = p.lo | q.lo << 16;
-      }
-  }
+  for (int i = 0; i < MT; ++i)
+    back[i] = split_row<DT, KS>(f.hidden + (size_t)row[i] * f.R, f.R, g, hi[i], lo[i]);
   const uint16_t* b = f.b + (size_t)max(t.adapter, 0) * f.N * f.R;       // (BAD: h is NaN)
   for (int c0 = n0 + w * 32; c0 < min(n0 + STRIP, f.N); c0 += 128) {
     v4u bv[2][KS];
@@ -245,12 +220,6 @@ __global__ __launch_bounds__(256) void expand_k(Fwd f, int strips) {
       if (16 * i + col < t.count) store8(f.out + (size_t)row[i] * f.ldo + c, o, f.N - c);
     }
   }
-}
-
-static bool sizes_ok(int dtype, int rows, int n, int size, int cap, int K, int N, int R) {
-  return (dtype == 0 || dtype == 2) && rows >= 0 && n >= 1 && n <= MAX_ADAPTERS &&
-         (size == 16 || size == 64) && K >= 1 && N >= 1 && K <= 1 << 24 && N <= 1 << 24 && R >= 1 &&
-         R <= MAX_RANK && cap == (int)(rows / size + (rows < n + 2 ? rows : n + 2));
 }
 
 template <int DT, int MT>

@@ -10,6 +10,8 @@ any product of the caller's; rows, adapters and outputs are bf16 or f16.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -155,10 +157,85 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
         if (not same and _overlap(out, y)) or _overlap(out, x):
             raise ValueError("add_lora: out overlaps y or x (it may be y, or apart from both)")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, w.a, w.b)):
-        raise ValueError("add_lora has no gradient: detach its operands")
+        if out is not None or hidden is not None:
+            raise ValueError("add_lora: autograd keeps its own hidden and makes its own out; detach the operands "
+                             "for a gradient by hand")
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("add_lora: a captured graph takes add_lora_grad, without autograd")
+        return _AddLora.apply(y, x, w.a, w.b, w, rows)
     if hidden is None:
         hidden = torch.empty((rows.rows, w.rank), dtype=torch.float32, device=x.device)
     if out is None:
         out = torch.empty((rows.rows, y.shape[1]), dtype=y.dtype, device=y.device)
     _forward(y, x, w, rows, hidden, out)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_workspace(dtype: int, rows: int, n: int, size: int, cap: int, K: int, N: int,
+                    rank: int) -> int:
+    b = ctypes.c_longlong()
+    check(lib().rlu_lora_grad_workspace(dtype, rows, n, size, cap, K, N, rank, ctypes.byref(b)),
+          "rlu_lora_grad_workspace")
+    return b.value
+
+
+def _backward(dy, x, w, rows, hidden, need):
+    K, N, dev = w.a.shape[2], w.b.shape[1], x.device
+    make = torch.empty if rows.rows else torch.zeros
+    dx = torch.empty((rows.rows, K), dtype=x.dtype, device=dev) if need[0] else None
+    da = make(w.a.shape, dtype=x.dtype, device=dev) if need[1] else None
+    db = make(w.b.shape, dtype=x.dtype, device=dev) if need[2] else None
+    if rows.rows and any(need):
+        code, cap = _DTYPE_CODE[x.dtype], rows.tiles.shape[0]
+        # taken and given back on the current stream: calls on two streams, or two captured graphs, have their own
+        ws = torch.empty(_grad_workspace(code, rows.rows, w.n, rows.size, cap, K, N, w.rank),
+                         dtype=torch.uint8, device=dev)
+        with on_device(dev):
+            rc = lib().rlu_lora_grad(
+                dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), w.a.data_ptr(), w.b.data_ptr(),
+                w.scale.data_ptr(), code, rows.order.data_ptr(), rows.tiles.data_ptr(),
+                rows.first.data_ptr(), rows.rows, w.n, rows.size, cap, K, N, w.rank, hidden.data_ptr(),
+                *[0 if dx is None else dx.data_ptr(), K], *[0 if t is None else t.data_ptr()
+                                                            for t in (da, db)],
+                ws.data_ptr(), stream_ptr())
+        check(rc, "rlu_lora_grad")
+    return dx, da, db
+
+
+def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
+                  hidden: torch.Tensor, need: tuple[bool, bool, bool] = (True, True, True)):
+    """From the gradient dy [rows, N] of add_lora's output, its x, rows and the hidden that it filled: the gradients
+    (dx [rows, K], da [n, rank, K], db [n, N, rank]) of the stack's type, None where need says no. That of y is
+    dy itself. Sums in float32, in an order that only the sizes decide."""
+    _check_batch("add_lora_grad", w, rows)
+    _check_rows("add_lora_grad", "x", x, rows.rows, w.a.shape[2], w)
+    _check_rows("add_lora_grad", "dy", dy, rows.rows, w.b.shape[1], w)
+    _check_hidden("add_lora_grad", hidden, rows.rows, w)
+    if len(need) != 3:
+        raise ValueError("add_lora_grad: need says whether dx, da and db are wanted")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (dy, x, w.a, w.b)):
+        raise ValueError("add_lora_grad returns the gradients itself: detach its operands")
+    return _backward(dy, x, w, rows, hidden, need)
+
+
+class _AddLora(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, a, b, w, rows):
+        hidden = torch.empty((rows.rows, w.rank), dtype=torch.float32, device=x.device)
+        out = torch.empty((rows.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+        _forward(y, x, w, rows, hidden, out)
+        ctx.save_for_backward(x, a, b, hidden)
+        ctx.w, ctx.rows = w, rows
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("add_lora: a captured graph takes add_lora_grad, without autograd")
+        x, _, _, hidden = ctx.saved_tensors            # (refuses a or b written to since)
+        if dy.stride(1) != 1 and dy.shape[1] > 1:
+            dy = dy.contiguous()
+        need = ctx.needs_input_grad
+        return (dy if need[0] else None, *_backward(dy, x, ctx.w, ctx.rows, hidden, need[1:4]), None, None)

@@ -217,6 +217,8 @@ class _Rows(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, by, *_):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured graph takes a loss's gradient by hand, without autograd")
         grad, ctx.grad = ctx.grad, None
         if grad is None:
             raise RuntimeError("a loss's gradient is handed out once: compute the loss again for a "

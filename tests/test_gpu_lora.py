@@ -86,6 +86,35 @@ class Case:
         assert torch.equal(out[bare], self.y[bare])
 
 
+    def check_grad(self, dx, da, db, hidden=None):
+        """Against the float64 formulas; a gradient over an adapter's rows adds up those rows."""
+        d, x = self.dy.double(), self.x.double()
+        A, B = self.of(self.w.a), self.of(self.w.b)
+        s = self.of(self.w.scale)[:, None]
+        N, R = B.shape[1:]
+        h, he = self.hidden()
+        u = s * torch.bmm(d[:, None, :], B)[:, 0]
+        ue = s * torch.bmm(d.abs()[:, None, :], B.abs())[:, 0] * (2 * N + 8) * STEP
+        # a value in two parts: split; float16's tiles are scaled to their largest, 2^-34 of which is the last step
+        part = lambda t: self.split * t.abs() + t.abs().amax() * 2.0 ** -34          # noqa: E731
+        up, hp = part(u) + ue, part(h) + he
+        if dx is not None:
+            want = torch.bmm(u[:, None, :], A)[:, 0]
+            size = torch.bmm(u.abs()[:, None, :], A.abs())[:, 0]
+            self.near(dx, want, torch.bmm(up[:, None, :], A.abs())[:, 0] + 4 * (R + 1) * STEP * size, "dx")
+            assert (dx[self.ids < 0] == 0).all()
+        for got, v, by, by_err, what in ((da, x, u, up, "da"), (db, d, h, hp, "db")):
+            if got is None:
+                continue
+            for i in range(self.w.n):
+                at = self.ids == i
+                want, size = by[at].T @ v[at], by[at].abs().T @ v[at].abs()
+                limit = by_err[at].T @ v[at].abs() + 4 * (int(at.sum()) + 8) * STEP * size
+                if what == "db":
+                    want, limit = want.T, limit.T
+                self.near(got[i], want, limit, f"{what}[{i}]")
+
+
 SIZES = [  # rows, K, N, R, n
     (1, 2560, 2560, 16, 1), (1, 1, 1, 1, 1), (2, 7, 5, 3, 2), (5, 33, 31, 8, 3), (16, 128, 512, 16, 1),
     (17, 100, 513, 17, 40), (63, 768, 1543, 8, 12), (64, 256, 100, 24, 2), (100, 31, 33, 33, 5),
@@ -295,3 +324,206 @@ def test_graphs_replayed_with_new_rows(lora, rows):
             want = step(c.ids, c.x, c.y)
             torch.cuda.synchronize()
             assert torch.equal(outs[j][0], want[0]) and torch.equal(outs[j][1], want[1])
+
+
+# ---- the backward pass --------------------------------------------------------------------------
+def both(lora, c, need=(True, True, True)):
+    hidden = torch.full((c.x.shape[0], c.w.rank), NAN, device=DEV)
+    lora.add_lora(c.y, c.x, c.w, c.rows, hidden=hidden)
+    return lora.add_lora_grad(c.dy, c.x, c.w, c.rows, hidden, need)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,K,N,R,n", SIZES)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 5)])
+def test_gradients(lora, dtype, rows, K, N, R, n, pad, offset):
+    c = Case(lora, rows, K, N, R, n, dtype, pad=pad, offset=offset)
+    gpu_case(f"lora grad {dtype} rows={rows} K={K} N={N} R={R} n={n} pad={pad}")
+    got = both(lora, c)
+    torch.cuda.synchronize()
+    c.check_grad(*got)
+
+
+@pytest.mark.parametrize("rows,n,ids", [
+    (2000, 3, "one"), (2000, 70, "few"), (1500, 2, "none"), (90, 5, "runs"), (5000, 6, "runs"), (700, 1024, "few"),
+    (129, 2, "one")])
+def test_gradients_of_uneven_batches(lora, rows, n, ids):
+    """One adapter with every row, over many runs of tiles; most without any; no row with one; ids in runs."""
+    g = torch.Generator(DEV).manual_seed(rows)
+    of = {"one": torch.full((rows,), n - 1, device=DEV), "none": torch.full((rows,), -1, device=DEV),
+          "few": torch.randint(3, (rows,), generator=g, device=DEV) * (n // 3),
+          "runs": torch.randint(-1, n, (rows,), generator=g, device=DEV).sort().values}[ids].int()
+    for K, N, R in ((200, 264, 16), (72, 40, 40)):
+        c = Case(lora, rows, K, N, R, n, "bf16", ids=of)
+        gpu_case(f"lora grad rows={rows} n={n} {ids} K={K}")
+        got = both(lora, c)
+        torch.cuda.synchronize()
+        c.check_grad(*got)
+        empty = [i for i in range(n) if not (of == i).any()]
+        assert (got[1][empty] == 0).all() and (got[2][empty] == 0).all()
+
+
+@pytest.mark.parametrize("rows,K,N,R", [(96, 2560, 2560, 16), (40, 136, 50000, 16), (1030, 512, 20000, 64)])
+def test_gradients_of_long_products(lora, rows, K, N, R):
+    c = Case(lora, rows, K, N, R, 2, "bf16")
+    gpu_case(f"lora grad long rows={rows} K={K} N={N}")
+    got = both(lora, c)
+    torch.cuda.synchronize()
+    c.check_grad(*got)
+
+
+def test_gradients_asked_for_one_by_one(lora):
+    for rows in (70, 1100):
+        c = Case(lora, rows, 136, 200, 16, 3, "f16")
+        gpu_case(f"lora grad need rows={rows}")
+        want = both(lora, c)
+        for need in ((True, False, False), (False, True, False), (False, False, True), (False, True, True),
+                     (False, False, False)):
+            got = both(lora, c, need)
+            torch.cuda.synchronize()
+            for t, u, n in zip(got, want, need):
+                assert torch.equal(t, u) if n else t is None
+
+
+@pytest.mark.parametrize("rows", [45, 1300])
+def test_gradients_of_ids_past_the_last_and_nan(lora, rows):
+    """A bad row has no part in the adapters' gradients; a NaN in a row goes to that row and to its adapter alone;
+    rows without an adapter have 0, whatever adapter 0 holds."""
+    ids = (torch.arange(rows, device=DEV) % 5 - 1).int()             # -1 .. 3 of a stack of 3
+    c = Case(lora, rows, 72, 100, 8, 3, "bf16", ids=ids)
+    gpu_case("lora grad ids past the last")
+    dx, da, db = both(lora, c)
+    bad = ids == 3
+    torch.cuda.synchronize()
+    assert dx[bad].isnan().all()
+    dx[bad] = 0
+    c.check_grad(dx, da, db)
+    c.x[1, 3] = NAN                                                  # (adapter 0's row)
+    c.w.a[0, 2, 5] = INF
+    got = both(lora, c)
+    torch.cuda.synchronize()
+    assert (got[0][ids < 0] == 0).all() and got[1][0, :, 3].isnan().all()
+    keep = [r for r in range(rows) if ids[r] in (1, 2)]
+    assert torch.equal(got[0][keep], dx[keep])
+    assert torch.equal(got[1][1:], da[1:]) and torch.equal(got[2][1:], db[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_large_and_small_gradients(lora, dtype):
+    """u past float16's range and below its smallest; bf16's likewise."""
+    for big in ((2.0 ** 11, 2.0 ** -12) if dtype == "f16" else (2.0 ** 60, 2.0 ** -60)):
+        c = Case(lora, 100, 136, 96, 16, 2, dtype, bare=0.0)
+        c.w.b.mul_(big)
+        c.w.a.mul_(1 / big)
+        c.dy.mul_(16.0 if big > 1 else 0.25)
+        c.x.mul_(2.0 ** -8 if big > 1 else 4.0)
+        gpu_case(f"lora grad scale {big} {dtype}")
+        got = both(lora, c)
+        torch.cuda.synchronize()
+        assert all(torch.isfinite(t).all() for t in got)
+        c.check_grad(*got)
+
+
+def test_gradients_against_differences(lora):
+    """Of L = sum dy (y + h B^T) along random directions, with operands that are exact in bf16 before and after a step.
+    L is linear in x, in a and in b alone, so its central difference has no error but the outputs' roundings."""
+    g = torch.Generator(DEV).manual_seed(1)
+    c = Case(lora, 40, 64, 48, 8, 3, "bf16")
+    for t in (c.x, c.w.a, c.w.b, c.dy, c.y):
+        t.copy_((torch.randint(-8, 9, t.shape, generator=g, device=DEV)) / 8)
+    dx, da, db = both(lora, c)
+    gpu_case("lora against differences")
+
+    def loss():
+        # in float32, whose hidden part is exact enough: the output's rounding is what a difference would see
+        h = torch.empty(40, 8, device=DEV)
+        lora.add_lora(c.y, c.x, c.w, c.rows, hidden=h)
+        return (c.dy.double() * torch.bmm(c.of(c.w.b), h.double()[:, :, None])[:, :, 0]).sum()
+    for t, grad in ((c.x, dx), (c.w.a, da)):
+        for _ in range(3):
+            step = torch.randint(-1, 2, t.shape, generator=g, device=DEV).to(t.dtype)
+            keep = t.clone()
+            t.copy_(keep + step)
+            up = loss()
+            t.copy_(keep - step)
+            by = (up - loss()) / 2
+            t.copy_(keep)
+            got = (grad.double() * step.double()).sum()
+            size = (grad.double().abs() * step.double().abs()).sum()
+            assert (by - got).abs() <= (c.eps + 600 * STEP) * size + 600 * STEP * up.abs(), (by, got)
+    # and in b, whose product the output adds up: hidden stays, the difference is the gradient's own sum
+    h = torch.empty(40, 8, device=DEV)
+    lora.add_lora(c.y, c.x, c.w, c.rows, hidden=h)
+    step = torch.randint(-1, 2, c.w.b.shape, generator=g, device=DEV).double()
+    by = (c.dy.double() * torch.bmm(c.of(step), h.double()[:, :, None])[:, :, 0]).sum()
+    size = (db.double().abs() * step.abs()).sum()
+    assert (by - (db.double() * step).sum()).abs() <= (c.eps + 600 * STEP) * size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [30, 1100])
+def test_autograd(lora, dtype, rows):
+    c = Case(lora, rows, 72, 130, 16, 3, dtype, pad=2, offset=1)
+    want = both(lora, c)
+    y, x, a, b = (t.detach().requires_grad_() for t in (c.y, c.x, c.w.a, c.w.b))
+    w = lora.LoraStack(a, b, c.w.scale)
+    gpu_case(f"lora autograd {dtype} rows={rows}")
+    out = lora.add_lora(y, x, w, c.rows)
+    assert torch.equal(out, lora.add_lora(c.y, c.x, c.w, c.rows))
+    got = torch.autograd.grad(out, (y, x, a, b), c.dy, retain_graph=True)
+    for t, u in zip(got, (c.dy, *want)):
+        assert torch.equal(t, u)
+    again = torch.autograd.grad(out, (x, b), c.dy)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[2])
+    (lora.add_lora(c.y, c.x, w, c.rows).sum() * 2.0).backward()       # (an expanded gradient)
+    c.dy = torch.full_like(c.dy, 2.0)
+    for t, u in zip((a.grad, b.grad), both(lora, c)[1:]):
+        assert torch.equal(t, u)
+    out = lora.add_lora(y, x, w, c.rows)
+    with torch.no_grad():
+        a.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.backward(c.dy)
+
+
+def test_gradients_on_streams_and_in_graphs(lora):
+    for rows in (60, 1300):
+        c = Case(lora, rows, 264, 530, 16, 9, "bf16")
+        gpu_case(f"lora grad on three streams at once rows={rows}")
+        torch.cuda.synchronize()
+        got = []
+        for st in [torch.cuda.Stream() for _ in range(3)]:
+            with torch.cuda.stream(st):
+                got += [both(lora, c) for _ in range(3)]
+        torch.cuda.synchronize()
+        for t in got[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(got[0], t))
+        others = Case(lora, rows, 264, 530, 16, 9, "bf16", seed=7)
+        others.w = c.w
+        ids, x, dy = c.ids.clone(), c.x.clone(), c.dy.clone()
+        graph = torch.cuda.CUDAGraph()
+        leaf = lora.LoraStack(c.w.a.detach().requires_grad_(), c.w.b, c.w.scale)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            p = lora.plan_rows(ids, 9)
+            hidden = torch.empty(rows, 16, device=DEV)
+            lora.add_lora(c.y, x, c.w, p, hidden=hidden)
+            outs = lora.add_lora_grad(dy, x, c.w, p, hidden)
+            with pytest.raises(ValueError, match="add_lora_grad"):
+                lora.add_lora(c.y, x, leaf, p)
+        for case in (others, c, others, c):
+            for t, s in zip((ids, x, dy), (case.ids, case.x, case.dy)):
+                t.copy_(s)
+            graph.replay()
+            want = both(lora, case)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_no_rows_have_zero_gradients(lora):
+    w = lora.LoraStack(torch.ones(2, 8, 16, dtype=torch.bfloat16, device=DEV),
+                       torch.ones(2, 24, 8, dtype=torch.bfloat16, device=DEV), torch.ones(2, device=DEV))
+    rows = lora.plan_rows(torch.empty(0, dtype=torch.int64, device=DEV), 2)
+    e = lambda n: torch.empty(0, n, dtype=torch.bfloat16, device=DEV)                  # noqa: E731
+    dx, da, db = lora.add_lora_grad(e(24), e(16), w, rows, torch.empty(0, 8, device=DEV))
+    assert dx.shape == (0, 16) and (da == 0).all() and (db == 0).all()
