@@ -29,11 +29,16 @@ using lp::wave_add;
 using lp::wave_max;
 
 constexpr int MAX_TOP = 32, MAX_V = 500000;
-constexpr int CV = 4;                      // vectors of 16 bytes of a thread's chunk
-constexpr int NT = 512, NW = NT / WAVE;
-constexpr int CHUNK = CV * NT;
+constexpr int MOST_NW = 16;
+
+// Threads of a workgroup, and the vectors of 16 bytes that each of them takes at a time.
+template <int THREADS, int VECTORS>
+struct Shape {
+  static constexpr int NT = THREADS, NW = NT / WAVE, CV = VECTORS, CHUNK = CV * NT;
+};
 constexpr int MAX_SEGS = WAVE;
 enum { POLICY, DISTILL };
+typedef v4u v4ua __attribute__((aligned(2)));          // (16 bytes at any element's address)
 
 struct Args {
   const uint8_t* logits;
@@ -50,6 +55,10 @@ struct Args {
   uint8_t* grad;
   long long ldg;
 };
+
+typedef Shape<512, 4> Usual;               // a row's workgroup (Wide: of long float32 rows), and a segment's
+typedef Shape<1024, 4> Wide;
+typedef Shape<256, 2> Short;
 
 // The maximum of a row's unlisted logits and sum e^((x - m) / T) over them. Nothing: -inf, 0.
 struct Part {
@@ -84,7 +93,7 @@ __device__ __forceinline__ uint32_t bits_of(float x) {
 }
 
 // raw's element at of its CV vectors becomes b (a dynamic index would put raw into memory)
-template <int DT>
+template <int DT, int CV>
 __device__ __forceinline__ void put(v4u (&raw)[CV], int k, int e, uint32_t b) {
   const int word = k * 4 + (Elem<DT>::SIZE == 4 ? e : e / 2);
 #pragma unroll
@@ -100,8 +109,8 @@ __device__ __forceinline__ void put(v4u (&raw)[CV], int k, int e, uint32_t b) {
 struct Listed {
   int id[MAX_TOP];
   float grad[MAX_TOP];
-  uint32_t owns[NT];                       // bit j: the thread's vectors hold id[j]
-  float m[NW], s[NW];
+  float m[MOST_NW], s[MOST_NW];
+  uint32_t owns[MOST_NW * WAVE];           // bit j: the thread's vectors hold id[j]
 };
 
 // Of a thread's vectors from `from` on the first that holds a listed logit.
@@ -115,23 +124,23 @@ __device__ __forceinline__ int next_of(const Listed& l, uint32_t owns, int shift
   return next;
 }
 // Puts of(j) in the place of each listed logit j of the thread's chunk at `base`.
-template <int DT, class Of>
-__device__ __forceinline__ int replace(v4u (&raw)[CV], const Listed& l, uint32_t owns, int shift,
-                                       int base, Of of) {
+template <int DT, class S, class Of>
+__device__ __forceinline__ void replace(v4u (&raw)[S::CV], const Listed& l, uint32_t owns, int shift,
+                                        int base, Of of) {
   for (uint32_t b = owns; b; b &= b - 1) {
     const int j = __ffs((int)b) - 1, i = l.id[j] + shift, v = i / Elem<DT>::N;
-    if (v >= base && v < base + CHUNK) put<DT>(raw, (v - base) / NT, i % Elem<DT>::N, of(j));
+    if (v >= base && v < base + S::CHUNK) put<DT>(raw, (v - base) / S::NT, i % Elem<DT>::N, of(j));
   }
-  return next_of<DT>(l, owns, shift, base + CHUNK);
 }
 
-template <int DT>
-__device__ __forceinline__ void load(v4u (&raw)[CV], const Row& r, int base) {
+// LAST: nobody asks for these again
+template <int DT, class S, bool LAST>
+__device__ __forceinline__ void load(v4u (&raw)[S::CV], const Row& r, int base) {
 #pragma unroll
-  for (int k = 0; k < CV; ++k) {
-    const int v = base + k * NT + (int)threadIdx.x;
+  for (int k = 0; k < S::CV; ++k) {
+    const int v = base + k * S::NT + (int)threadIdx.x;
     if (v < r.nvec) {
-      raw[k] = r.pv[v];
+      raw[k] = LAST ? __builtin_nontemporal_load(r.pv + v) : r.pv[v];
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -140,12 +149,12 @@ __device__ __forceinline__ void load(v4u (&raw)[CV], const Row& r, int base) {
   }
 }
 // elements of the neighbours in a row's end vectors
-template <int DT>
-__device__ __forceinline__ void trim(v4u (&raw)[CV], const Row& r, int V, int base) {
+template <int DT, class S>
+__device__ __forceinline__ void trim(v4u (&raw)[S::CV], const Row& r, int V, int base) {
   typedef Elem<DT> E;
 #pragma unroll
-  for (int k = 0; k < CV; ++k) {
-    const int v = base + k * NT + (int)threadIdx.x;
+  for (int k = 0; k < S::CV; ++k) {
+    const int v = base + k * S::NT + (int)threadIdx.x;
     if ((v == 0 && r.shift) || v == r.nvec - 1)
 #pragma unroll
       for (int i = 0; i < E::N; ++i) {
@@ -175,7 +184,7 @@ __device__ __forceinline__ Ref ref_of(float m, float k) {
 }
 
 // Adds a thread's chunk to (m, s).
-template <int DT>
+template <int DT, int CV>
 __device__ __forceinline__ void add(const v4u (&raw)[CV], float k, float& m, float& s) {
   const float top = fmaxf(m, Max<DT, CV>::of(raw));
   const Ref r = ref_of(top, k);
@@ -204,23 +213,25 @@ __device__ __forceinline__ Part join(Part a, float m, float k) {
   return {m, a.s};
 }
 
-// The sum over a row's vectors [v0, v1), of all threads: the same in each of them.
-template <int DT>
+// The sum over a row's vectors [v0, v1), of all threads: the same in each of them. raw: the first chunk. The last
+// one is left in it.
+template <int DT, class S>
 __device__ __forceinline__ Part sum_of(const Args& a, const Row& r, Listed& l, uint32_t owns, int v0,
-                                       int v1) {
+                                       int v1, v4u (&raw)[S::CV]) {
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE);
   float m = -__builtin_inff(), s = 0.f;
   int next = next_of<DT>(l, owns, r.shift, v0);
-  v4u raw[CV], ahead[CV];
-  load<DT>(ahead, r, v0);
-  for (int base = v0; base < v1; base += CHUNK) {
+  for (int base = v0; base < v1; base += S::CHUNK) {
+    v4u x[S::CV];
 #pragma unroll
-    for (int i = 0; i < CV; ++i) raw[i] = ahead[i];
-    if (base + CHUNK < v1) load<DT>(ahead, r, base + CHUNK);
-    if (base == 0 || base + CHUNK >= r.nvec) trim<DT>(raw, r, a.V, base);
-    if (next < base + CHUNK)
-      next = replace<DT>(raw, l, owns, r.shift, base, [](int) { return Elem<DT>::NINF; });
-    add<DT>(raw, a.k, m, s);
+    for (int i = 0; i < S::CV; ++i) x[i] = raw[i];
+    if (base + S::CHUNK < v1) load<DT, S, false>(raw, r, base + S::CHUNK);
+    if (base == 0 || base + S::CHUNK >= r.nvec) trim<DT, S>(x, r, a.V, base);
+    if (next < base + S::CHUNK) {
+      replace<DT, S>(x, l, owns, r.shift, base, [](int) { return Elem<DT>::NINF; });
+      next = next_of<DT>(l, owns, r.shift, base + S::CHUNK);
+    }
+    add<DT>(x, a.k, m, s);
   }
   const float wm = wave_max(m);
   s = wave_add(join({m, s}, wm, a.k).s);
@@ -231,9 +242,9 @@ __device__ __forceinline__ Part sum_of(const Args& a, const Row& r, Listed& l, u
   __syncthreads();
   float top = l.m[0], sum = 0.f;
 #pragma unroll
-  for (int i = 1; i < NW; ++i) top = fmaxf(top, l.m[i]);
+  for (int i = 1; i < S::NW; ++i) top = fmaxf(top, l.m[i]);
 #pragma unroll
-  for (int i = 0; i < NW; ++i) sum += join({l.m[i], l.s[i]}, top, a.k).s;
+  for (int i = 0; i < S::NW; ++i) sum += join({l.m[i], l.s[i]}, top, a.k).s;
   return {top, sum};
 }
 
@@ -343,62 +354,59 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return bits_of<DT>(a) | bits_of<DT>(b) << 16;
 }
 
-// The gradient of a row's vectors [v0, v1).
-template <int DT>
+// The gradient of a row's vectors [v0, v1), the last chunk first: the cache has it still. raw: that chunk.
+template <int DT, class S>
 __device__ __forceinline__ void grad_of(const Args& a, const Row& r, const Listed& l, uint32_t owns,
-                                        int row, int v0, int v1, Coef c) {
+                                        int row, int v0, int v1, Coef c, v4u (&raw)[S::CV]) {
   typedef Elem<DT> E;
   uint8_t* out = a.grad + (size_t)row * a.ldg * E::SIZE - r.shift * E::SIZE;
   const Ref ref = ref_of(c.m, a.k);
   const float f = c.f * __builtin_amdgcn_exp2f(ref.fix);
-  int next = next_of<DT>(l, owns, r.shift, v0);
-  v4u raw[CV], ahead[CV];
-  load<DT>(ahead, r, v0);
-  for (int base = v0; base < v1; base += CHUNK) {
+  for (int base = v0 + (v1 - v0 - 1) / S::CHUNK * S::CHUNK; base >= v0 && v0 < v1; base -= S::CHUNK) {
+    v4u x[S::CV];
 #pragma unroll
-    for (int i = 0; i < CV; ++i) raw[i] = ahead[i];
-    if (base + CHUNK < v1) load<DT>(ahead, r, base + CHUNK);
+    for (int i = 0; i < S::CV; ++i) x[i] = raw[i];
+    if (base > v0) load<DT, S, true>(raw, r, base - S::CHUNK);
 #pragma unroll
-    for (int i = 0; i < CV; ++i) {
+    for (int i = 0; i < S::CV; ++i) {
       float g[E::N];
       if (!ref.far)
 #pragma unroll
         for (int e = 0; e < E::N; ++e)
-          g[e] = f * __builtin_amdgcn_exp2f(fmaf(E::get(raw[i], e), a.k, -ref.c));
+          g[e] = f * __builtin_amdgcn_exp2f(fmaf(E::get(x[i], e), a.k, -ref.c));
       else
 #pragma unroll
         for (int e = 0; e < E::N; ++e)
-          g[e] = f * __builtin_amdgcn_exp2f((E::get(raw[i], e) - ref.m) * a.k);
+          g[e] = f * __builtin_amdgcn_exp2f((E::get(x[i], e) - ref.m) * a.k);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        raw[i][j] = E::SIZE == 4 ? __float_as_uint(g[j]) : pack<DT>(g[2 * j % E::N], g[(2 * j + 1) % E::N]);
+        x[i][j] = E::SIZE == 4 ? __float_as_uint(g[j]) : pack<DT>(g[2 * j % E::N], g[(2 * j + 1) % E::N]);
     }
-    if (next < base + CHUNK)
-      next = replace<DT>(raw, l, owns, r.shift, base, [&](int j) { return bits_of<DT>(l.grad[j]); });
+    if (owns) replace<DT, S>(x, l, owns, r.shift, base, [&](int j) { return bits_of<DT>(l.grad[j]); });
 #pragma unroll
-    for (int k = 0; k < CV; ++k) {
-      const int v = base + k * NT + (int)threadIdx.x;
+    for (int k = 0; k < S::CV; ++k) {
+      const int v = base + k * S::NT + (int)threadIdx.x;
       uint8_t* to = out + (long long)v * 16;
       if ((v == 0 && r.shift) || v == r.nvec - 1) {
 #pragma unroll
         for (int i = 0; i < E::N; ++i) {
           const int j = v * E::N + i - r.shift;
           if (j < 0 || j >= a.V) continue;
-          if (E::SIZE == 4) ((uint32_t*)to)[i] = raw[k][i];
-          else ((uint16_t*)to)[i] = (uint16_t)(raw[k][i / 2] >> i % 2 * 16);
+          if (E::SIZE == 4) ((uint32_t*)to)[i] = x[k][i];
+          else ((uint16_t*)to)[i] = (uint16_t)(x[k][i / 2] >> i % 2 * 16);
         }
       } else if (v < r.nvec) {
-        __builtin_memcpy(to, &raw[k], 16);             // (any element's address)
+        __builtin_nontemporal_store(x[k], (v4ua*)to);
       }
     }
   }
 }
 
-template <int DT>
+template <int DT, class S>
 __device__ __forceinline__ void clear(const Args& a, const Row& r, int row, int v0, int v1) {
   typedef Elem<DT> E;
   uint8_t* out = a.grad + (size_t)row * a.ldg * E::SIZE - r.shift * E::SIZE;
-  for (int v = v0 + (int)threadIdx.x; v < min(v1, r.nvec); v += NT) {
+  for (int v = v0 + (int)threadIdx.x; v < min(v1, r.nvec); v += S::NT) {
     uint8_t* to = out + (long long)v * 16;
     if ((v == 0 && r.shift) || v == r.nvec - 1) {
       for (int i = 0; i < E::N; ++i) {
@@ -420,7 +428,7 @@ struct Own {
   int id;
   bool bad, skip;
 };
-template <int DT, int OP>
+template <int DT, int OP, class S>
 __device__ __forceinline__ Own listed(const Args& a, const Row& r, int row, const float* xs, Listed& l) {
   const int lane = lane_id(), tid = (int)threadIdx.x, top = OP == POLICY ? 1 : a.top;
   Own o = {-__builtin_inff(), -__builtin_inff(), a.weight ? a.weight[row] : 1.f, -1, false, false};
@@ -437,7 +445,7 @@ __device__ __forceinline__ Own listed(const Args& a, const Row& r, int row, cons
   if (tid < MAX_TOP) l.id[tid] = tid < top ? o.id : -1;
   l.owns[tid] = 0;
   __syncthreads();
-  if (tid < WAVE && o.id >= 0) atomicOr(&l.owns[(o.id + r.shift) / Elem<DT>::N % NT], 1u << lane);
+  if (tid < WAVE && o.id >= 0) atomicOr(&l.owns[(o.id + r.shift) / Elem<DT>::N % S::NT], 1u << lane);
   __syncthreads();
   return o;
 }
@@ -452,79 +460,87 @@ __device__ __forceinline__ Coef coef(const Args& a, Part u, const Own& o, int ro
 }
 
 // A workgroup a row: its sum, its loss and, with GRAD, its gradient.
-template <int DT, int OP, bool GRAD>
-__global__ __launch_bounds__(NT) void row_k(Args a) {
+template <int DT, int OP, bool GRAD, class S>
+__global__ __launch_bounds__(S::NT, S::NT == Wide::NT ? 8 : 1) void row_k(Args a) {
   __shared__ Listed l;
   const int row = (int)blockIdx.x;
   const Row r = row_of<DT>(a, row);
-  const Own o = listed<DT, OP>(a, r, row, nullptr, l);
+  v4u raw[S::CV];
+  load<DT, S, !GRAD>(raw, r, 0);
+  const Own o = listed<DT, OP, S>(a, r, row, nullptr, l);
   if (o.skip) {
     if (threadIdx.x == 0) {
       a.loss[row] = 0.f;
       if (OP == POLICY) a.logprob[row] = 0.f;
     }
-    if (GRAD) clear<DT>(a, r, row, 0, r.nvec);
+    if (GRAD) clear<DT, S>(a, r, row, 0, r.nvec);
     return;
   }
   const uint32_t owns = l.owns[threadIdx.x];
-  const Part u = sum_of<DT>(a, r, l, owns, 0, r.nvec);
+  const Part u = sum_of<DT, S>(a, r, l, owns, 0, r.nvec, raw);
   const Coef c = coef<OP>(a, u, o, row, l, true);
-  if (GRAD) grad_of<DT>(a, r, l, owns, row, 0, r.nvec, c);
+  if (GRAD) grad_of<DT, S>(a, r, l, owns, row, 0, r.nvec, c, raw);
 }
 
 // Few rows: a workgroup for each of a row's segments, first their sums, then a launch that joins them and
 // writes the loss and the segments' gradients.
-template <int DT, int OP>
-__global__ __launch_bounds__(NT) void segment_k(Args a, Part* __restrict__ parts,
-                                                float* __restrict__ xs) {
+template <int DT, int OP, class S>
+__global__ __launch_bounds__(S::NT) void segment_k(Args a, Part* __restrict__ parts,
+                                                   float* __restrict__ xs) {
   __shared__ Listed l;
   const int row = (int)(blockIdx.x / (unsigned)a.nseg), seg = (int)(blockIdx.x % (unsigned)a.nseg);
   const Row r = row_of<DT>(a, row);
-  const Own o = listed<DT, OP>(a, r, row, nullptr, l);
+  const int len = ((r.nvec + S::CHUNK - 1) / S::CHUNK + a.nseg - 1) / a.nseg * S::CHUNK;
+  const int v0 = min(seg * len, r.nvec), v1 = min(v0 + len, r.nvec);
+  v4u raw[S::CV];
+  load<DT, S, false>(raw, r, v0);
+  const Own o = listed<DT, OP, S>(a, r, row, nullptr, l);
   if (o.skip) return;
   // (the gradient may take the logits' place while other segments still ask for these)
   if (seg == 0 && (int)threadIdx.x < a.top) xs[(size_t)row * a.top + threadIdx.x] = o.x;
-  const int len = ((r.nvec + CHUNK - 1) / CHUNK + a.nseg - 1) / a.nseg * CHUNK;
-  const int v0 = min(seg * len, r.nvec), v1 = min(v0 + len, r.nvec);
-  const Part u = sum_of<DT>(a, r, l, l.owns[threadIdx.x], v0, v1);
+  const Part u = sum_of<DT, S>(a, r, l, l.owns[threadIdx.x], v0, v1, raw);
   if (threadIdx.x == 0) parts[blockIdx.x] = u;
 }
 
-template <int DT, int OP, bool GRAD>
-__global__ __launch_bounds__(NT) void finish_k(Args a, const Part* __restrict__ parts,
-                                               const float* __restrict__ xs) {
+template <int DT, int OP, bool GRAD, class S>
+__global__ __launch_bounds__(S::NT) void finish_k(Args a, const Part* __restrict__ parts,
+                                                  const float* __restrict__ xs) {
   __shared__ Listed l;
   const unsigned n = GRAD ? (unsigned)a.nseg : 1u;
   const int row = (int)(blockIdx.x / n), seg = (int)(blockIdx.x % n), lane = lane_id();
   const Row r = row_of<DT>(a, row);
-  const Own o = listed<DT, OP>(a, r, row, xs, l);
-  const int len = ((r.nvec + CHUNK - 1) / CHUNK + a.nseg - 1) / a.nseg * CHUNK;
+  const int len = ((r.nvec + S::CHUNK - 1) / S::CHUNK + a.nseg - 1) / a.nseg * S::CHUNK;
   const int v0 = min(seg * len, r.nvec), v1 = min(v0 + len, r.nvec);
+  v4u raw[S::CV];
+  if (GRAD && v0 < v1) load<DT, S, true>(raw, r, v0 + (v1 - v0 - 1) / S::CHUNK * S::CHUNK);
+  Part u = {-__builtin_inff(), 0.f};
+  if (lane < a.nseg) u = parts[(size_t)row * a.nseg + lane];
+  const Own o = listed<DT, OP, S>(a, r, row, xs, l);
   if (o.skip) {
     if (seg == 0 && threadIdx.x == 0) {
       a.loss[row] = 0.f;
       if (OP == POLICY) a.logprob[row] = 0.f;
     }
-    if (GRAD) clear<DT>(a, r, row, v0, v1);
+    if (GRAD) clear<DT, S>(a, r, row, v0, v1);
     return;
   }
-  Part u = {-__builtin_inff(), 0.f};
-  if (lane < a.nseg) u = parts[(size_t)row * a.nseg + lane];
   const float m = wave_max(u.m);
   u = {m, wave_add(join(u, m, a.k).s)};
   const Coef c = coef<OP>(a, u, o, row, l, seg == 0);
-  if (GRAD) grad_of<DT>(a, r, l, l.owns[threadIdx.x], row, v0, v1, c);
+  if (GRAD) grad_of<DT, S>(a, r, l, l.owns[threadIdx.x], row, v0, v1, c, raw);
 }
+
+constexpr int SCALE_NT = 512;
 
 // Rows of a gradient by a factor each; those whose factor is 1 are left as they are.
 template <int DT>
-__global__ __launch_bounds__(NT) void scale_k(Args a, const float* __restrict__ by, long long step) {
+__global__ __launch_bounds__(SCALE_NT) void scale_k(Args a, const float* __restrict__ by, long long step) {
   typedef Elem<DT> E;
   const int row = (int)(blockIdx.x / (unsigned)a.nseg), seg = (int)(blockIdx.x % (unsigned)a.nseg);
   const float f = by[row * step];
   if (f == 1.f) return;
   const Row r = row_of<DT>(a, row);
-  for (int v = seg * NT + (int)threadIdx.x; v < r.nvec; v += a.nseg * NT) {
+  for (int v = seg * SCALE_NT + (int)threadIdx.x; v < r.nvec; v += a.nseg * SCALE_NT) {
     uint8_t* to = (uint8_t*)(r.pv + v);
     if ((v == 0 && r.shift) || v == r.nvec - 1) {      // (the neighbours' elements are theirs)
       for (int i = 0; i < E::N; ++i) {
@@ -547,18 +563,18 @@ __global__ __launch_bounds__(NT) void scale_k(Args a, const float* __restrict__ 
 
 // Segments of a row: one where the rows alone fill the chip.
 static int segments(int dtype, int R, int V) {
-  const int n = dtype == 1 ? 4 : 8;
-  const int chunks = (V + 2 * n - 2) / n / CHUNK + 1;
   if (R >= 256) return 1;
-  const int want = R ? (512 + R - 1) / R : 1;
-  return chunks < want ? (chunks < MAX_SEGS ? chunks : MAX_SEGS) : want < MAX_SEGS ? want : MAX_SEGS;
+  const int n = dtype == 1 ? 4 : 8;
+  const int chunks = (V + 2 * n - 2) / n / Short::CHUNK + 1, want = R ? (768 + R - 1) / R : 1;
+  const int most = chunks < MAX_SEGS ? chunks : MAX_SEGS;
+  return want < most ? want : most;
 }
 
 static int check(const Args& a, int dtype, long long* bytes) {
   if (dtype < 0 || dtype > 2 || a.R < 0 || a.V < 1 || a.V > MAX_V || a.top < 1 || a.top > MAX_TOP)
     return -1;
   const long long segs = (long long)a.R * segments(dtype, a.R, a.V);
-  if (segs > UINT32_MAX / NT) return -1;               // (a launch counts its threads in 32 bits)
+  if (segs > UINT32_MAX / Wide::NT) return -1;         // (a launch counts its threads in 32 bits)
   *bytes = segs * (long long)sizeof(Part) + 4ll * a.R * a.top;
   return 0;
 }
@@ -566,9 +582,7 @@ static int check(const Args& a, int dtype, long long* bytes) {
 template <int OP>
 static int launch(Args a, int dtype, void* ws, hipStream_t stream) {
   long long bytes;
-  if (check(a, dtype, &bytes) || a.ld < 0 || !(a.inv_t > 0.f) ||
-      !(a.k < __builtin_inff()))
-    return -1;
+  if (check(a, dtype, &bytes) || a.ld < 0 || !(a.inv_t > 0.f) || !(a.k < __builtin_inff())) return -1;
   if (a.R == 0) return 0;
   if (!a.logits || !a.loss || !ws) return -1;
   if (a.grad && a.R > 1 && a.ldg < a.V) return -1;
@@ -577,22 +591,34 @@ static int launch(Args a, int dtype, void* ws, hipStream_t stream) {
   Part* parts = (Part*)ws;
   float* xs = (float*)(parts + (size_t)a.R * a.nseg);
   const dim3 rows((unsigned)a.R), all((unsigned)(a.R * a.nseg));
+  // The second read comes from the memory-side cache as long as the rows in flight fit there (256 MB): four
+  // workgroups a CU of rows up to 256 KB. Of longer ones two: float32's with twice the threads, 16-bit ones' kept to
+  // two by LDS that they do not use, as more threads a row leave the vector unit idle between its passes.
+  const bool longer = (long long)a.V * (dtype == 1 ? 4 : 2) > 256 << 10;
+#define RLU_ROW(DT, GRAD, S, LDS) \
+  hipLaunchKernelGGL((row_k<DT, OP, GRAD, S>), rows, dim3(S::NT), LDS, stream, a)
 #define RLU_LOSS(DT)                                                                               \
   do {                                                                                             \
     if (a.nseg == 1) {                                                                             \
-      if (a.grad) hipLaunchKernelGGL((row_k<DT, OP, true>), rows, dim3(NT), 0, stream, a);         \
-      else hipLaunchKernelGGL((row_k<DT, OP, false>), rows, dim3(NT), 0, stream, a);               \
+      if (!a.grad) RLU_ROW(DT, false, Usual, 0);                                                   \
+      else if (!longer) RLU_ROW(DT, true, Usual, 0);                                               \
+      else if (DT == 1) RLU_ROW(1, true, Wide, 0);                                                 \
+      else RLU_ROW(DT, true, Usual, 70 << 10);                                                     \
     } else {                                                                                       \
-      hipLaunchKernelGGL((segment_k<DT, OP>), all, dim3(NT), 0, stream, a, parts, xs);                 \
+      hipLaunchKernelGGL((segment_k<DT, OP, Short>), all, dim3(Short::NT), 0, stream, a, parts, xs); \
       if (a.grad)                                                                                  \
-        hipLaunchKernelGGL((finish_k<DT, OP, true>), all, dim3(NT), 0, stream, a, parts, xs);          \
-      else hipLaunchKernelGGL((finish_k<DT, OP, false>), rows, dim3(NT), 0, stream, a, parts, xs);     \
+        hipLaunchKernelGGL((finish_k<DT, OP, true, Short>), all, dim3(Short::NT), 0, stream, a,    \
+                           parts, xs);                                                             \
+      else                                                                                         \
+        hipLaunchKernelGGL((finish_k<DT, OP, false, Short>), rows, dim3(Short::NT), 0, stream, a,  \
+                           parts, xs);                                                             \
     }                                                                                              \
   } while (0)
   if (dtype == 0) RLU_LOSS(0);
   else if (dtype == 1) RLU_LOSS(1);
   else RLU_LOSS(2);
 #undef RLU_LOSS
+#undef RLU_ROW
   return (int)hipGetLastError();
 }
 
@@ -678,11 +704,11 @@ extern "C" int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, co
   a.ld = ld;
   a.R = R;
   a.V = V;
-  a.nseg = (V + NT * 64 - 1) / (NT * 64);              // (8 to 16 vectors a thread)
-  if ((long long)R * a.nseg > UINT32_MAX / NT) return -1;
+  a.nseg = (V + SCALE_NT * 64 - 1) / (SCALE_NT * 64);              // (8 to 16 vectors a thread)
+  if ((long long)R * a.nseg > UINT32_MAX / SCALE_NT) return -1;
   const dim3 grid((unsigned)(R * a.nseg));
-  if (dtype == 0) hipLaunchKernelGGL((scale_k<0>), grid, dim3(NT), 0, stream, a, by, step);
-  else if (dtype == 1) hipLaunchKernelGGL((scale_k<1>), grid, dim3(NT), 0, stream, a, by, step);
-  else hipLaunchKernelGGL((scale_k<2>), grid, dim3(NT), 0, stream, a, by, step);
+  if (dtype == 0) hipLaunchKernelGGL((scale_k<0>), grid, dim3(SCALE_NT), 0, stream, a, by, step);
+  else if (dtype == 1) hipLaunchKernelGGL((scale_k<1>), grid, dim3(SCALE_NT), 0, stream, a, by, step);
+  else hipLaunchKernelGGL((scale_k<2>), grid, dim3(SCALE_NT), 0, stream, a, by, step);
   return (int)hipGetLastError();
 }
