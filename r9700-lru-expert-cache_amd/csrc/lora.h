@@ -51,11 +51,25 @@ __device__ __forceinline__ uint32_t to_bits(float f) {
   return DT == 0 ? f32_to_bf16(f) : __builtin_bit_cast(uint16_t, (_Float16)f);
 }
 
-// n elements at p (8 or more: eight of them), zeros behind: p at any element's address.
+// Two of them in one word.
+template <int DT>
+__device__ __forceinline__ uint32_t to_bits2(float a, float b) {
+  if (DT == 0) {
+    uint32_t r;
+    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+  }
+  return to_bits<DT>(a) | to_bits<DT>(b) << 16;
+}
+
+// n elements at p (8 or more: eight of them), zeros behind: p at any element's address. ONCE: nobody asks
+// for these again, so they need no place in the cache.
+typedef v4u v4ua __attribute__((aligned(2)));
+template <bool ONCE = false>
 __device__ __forceinline__ v4u load8(const uint16_t* p, int n) {
   v4u v = {};
   if (n >= 8) {
-    __builtin_memcpy(&v, p, 16);
+    v = ONCE ? (v4u)__builtin_nontemporal_load((const v4ua*)p) : (v4u)*(const v4ua*)p;
   } else {
 #pragma unroll
     for (int i = 0; i < 7; ++i)
@@ -63,14 +77,43 @@ __device__ __forceinline__ v4u load8(const uint16_t* p, int n) {
   }
   return v;
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void store8(uint16_t* p, v4u v, int n) {
   if (n >= 8) {
-    __builtin_memcpy(p, &v, 16);
+    if (ONCE) __builtin_nontemporal_store(v, (v4ua*)p);
+    else *(v4ua*)p = v;
   } else {
 #pragma unroll
     for (int i = 0; i < 7; ++i)
       if (i < n) p[i] = (uint16_t)(v[i / 2] >> i % 2 * 16);
   }
+}
+
+typedef v4f v4fa __attribute__((aligned(4)));
+__device__ __forceinline__ void load8(const float* p, int n, float (&h)[8]) {
+  if (n >= 8) {
+    const v4f a = *(const v4fa*)p, b = *(const v4fa*)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = i < 4 ? a[i] : b[i - 4];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = i < n ? p[i] : 0.f;
+  }
+}
+
+// Elements i .. i + 7 of a row of `all`, i a multiple of 8, in two steps: fetch asks for them, keep makes those past the
+// row's end zeros, when they are there. WHOLE: all is a multiple of 8 too, so that eight are there or none: then both go
+// without a branch, and a fetch ahead of its use waits for nothing (where its elements don't matter, keep is left out).
+template <bool WHOLE, bool ONCE = false>
+__device__ __forceinline__ v4u fetch(const uint16_t* p, int i, int all) {
+  return WHOLE ? load8<ONCE>(p + (i < all ? i : 0), 8) : load8<ONCE>(p + i, all - i);
+}
+template <bool WHOLE>
+__device__ __forceinline__ v4u keep(v4u v, int i, int all) {
+  if (WHOLE)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = i < all ? v[e] : 0u;
+  return v;
 }
 
 // Four of 8 consecutive k of a lane's column, from a row-major [k][column] tile in LDS: lanes 4 r .. 4 r + 3 of
@@ -98,34 +141,189 @@ struct Split {
   }
 };
 
-// A row of h or u, R floats, as fragments of both its parts: of the lane's 8 ranks of each 32. Returns by what sums
-// with them are multiplied: float16's were brought into its range by a power of two.
-template <int DT, int KS>
-__device__ __forceinline__ float split_row(const float* row, int R, int g, v4u (&hi)[KS], v4u (&lo)[KS]) {
-  float h[KS][8], m = 0.f;
+// A lane's part of 16 rows from `row` on, 32 of their elements from `k` on, of a row-major tile in LDS.
+template <int LD>
+__device__ __forceinline__ v4u frag(const uint16_t* tile, int row, int k) {
+  const int lane = lane_id();
+  return *(const v4u*)&tile[(row + lane % 16) * LD + k + 8 * (lane / 16)];
+}
+// The same of 16 columns from `c` on, 32 rows from `k` on.
+template <int LD>
+__device__ __forceinline__ v4u frag_tr(const uint16_t* tile, int k, int c) {
+  const int lane = lane_id(), col = lane % 16;
+  const uint16_t* p = &tile[(k + 8 * (lane / 16) + col / 4) * LD + c + col % 4 * 4];
+  return __builtin_bit_cast(v4u, __builtin_shufflevector(read_tr(p), read_tr(p + 4 * LD), 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A tile's rows of h or u, R floats each, as both their 16-bit parts in LDS, and by what sums with them are multiplied:
+// float16's are brought into its range by a power of two a row.
+template <int MT, int KS>
+struct Rows {
+  static constexpr int T = 16 * MT, LD = 32 * KS + 8;
+  uint16_t part[2][T][LD];
+  float back[T];
+};
+template <int DT, int MT, int KS, int NT>
+__device__ __forceinline__ void stage(Rows<MT, KS>& s, const Plan& p, const Tile& t, const float* h, int R) {
+  constexpr int PER = NT / (16 * MT), N = (4 * KS + PER - 1) / PER;    // threads a row, chunks of 8 a thread
+  const int row = (int)threadIdx.x / PER, q = (int)threadIdx.x % PER;
+  const float* from = h + (size_t)p.order[t.start + min(row, t.count - 1)] * R;
+  float v[N][8], m = 0.f;
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+  for (int k = 0; k < N; ++k) {
+    const int c = k * PER + q;
+    load8(from + 8 * c, c < 4 * KS && row < t.count ? R - 8 * c : 0, v[k]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int r = 32 * k + 8 * g + e;
-      h[k][e] = r < R ? row[r] : 0.f;
-      m = fmaxf(m, fabsf(h[k][e]));
-    }
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[k][e]));
+  }
   float by = 1.f;
   if (DT != 0) {
-    m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
+#pragma unroll
+    for (int d = 1; d < PER; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
     by = scale_to(m);
+    if (q == 0) s.back[row] = 1.f / by;
   }
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+  for (int k = 0; k < N; ++k) {
+    const int c = k * PER + q;
+    if (c >= 4 * KS) continue;
+    v4u hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const Split<DT> p(h[k][e] * by), q(h[k][e + 1] * by);
-      hi[k][e / 2] = p.hi | q.hi << 16;
-      lo[k][e / 2] = p.lo | q.lo << 16;
+      const Split<DT> a(v[k][e] * by), b(v[k][e + 1] * by);
+      hi[e / 2] = a.hi | b.hi << 16;
+      lo[e / 2] = a.lo | b.lo << 16;
     }
-  return 1.f / by;
+    *(v4u*)&s.part[0][row][8 * c] = hi;
+    *(v4u*)&s.part[1][row][8 * c] = lo;
+  }
+}
+
+// ---- out = y + h W^T (TR: h W, with W [R][cols]), without y where there is none ------------------------------------
+// A workgroup a tile (or 16 MT of its rows) and a strip of columns, a wave 64 columns at a time: W's part of them as it
+// lies in memory through LDS into registers, then 16 rows after the other. Sums leave the matrix unit with a lane's
+// neighbour another row; through LDS they come in rows of 128 bytes, as y and out are read and written.
+struct Out {
+  const float* h;
+  const uint16_t *w, *y;
+  long long ldy;
+  uint16_t* out;
+  long long ldo;
+  int cols, R;
+};
+constexpr int EXPAND_NT = 256, EXPAND_NW = EXPAND_NT / WAVE;
+template <int MT, int KS, bool TR>
+struct ExpandLds {
+  static constexpr int LD = TR ? 72 : 32 * KS + 8, SUM_LD = 68;
+  static constexpr int W = TR ? 32 * KS * LD : 64 * LD, SUMS = 2 * 16 * SUM_LD;
+  Rows<MT, KS> h;
+  alignas(16) uint16_t wave[EXPAND_NW][W > SUMS ? W : SUMS];           // W, then a block's sums
+};
+
+template <int DT, int MT, int KS, bool WHOLE, bool TR, bool ADD>
+__device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& t, int n0, int n1,
+                                       ExpandLds<MT, KS, TR>& lds) {
+  typedef ExpandLds<MT, KS, TR> L;
+  const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
+  const int r8 = lane / 8, c8 = lane % 8 * 8;
+  size_t row[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) row[i][s] = p.order[t.start + min(16 * i + 8 * s + r8, t.count - 1)];
+  if (ADD && t.adapter == NONE) {
+    if (f.y == f.out && f.ldy == f.ldo) return;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (16 * i + 8 * s + r8 < t.count)
+          for (int c = n0 + w * 64 + c8; c < n1; c += EXPAND_NW * 64)
+            store8(f.out + row[i][s] * f.ldo + c, load8(f.y + row[i][s] * f.ldy + c, f.cols - c), f.cols - c);
+    return;
+  }
+  const uint16_t* weights = f.w + (size_t)max(t.adapter, 0) * f.cols * f.R;       // (BAD: h is NaN)
+  const int ranks = t.adapter == NONE ? 0 : f.R;       // (0 times whatever adapter 0 holds may be NaN)
+  uint16_t* mine = lds.wave[w];
+  float* sums = (float*)mine;
+  stage<DT, MT, KS, EXPAND_NT>(lds.h, p, t, f.h, f.R);
+  __syncthreads();
+  for (int c0 = n0 + w * 64; c0 < n1; c0 += EXPAND_NW * 64) {
+    v4u wr[4 * KS], yv[MT][2];
+#pragma unroll
+    for (int i = 0; i < 4 * KS; ++i) {
+      const int q = i * WAVE + lane;
+      if (TR) wr[i] = fetch<WHOLE>(weights + (size_t)min(q / 8, f.R - 1) * f.cols, c0 + c8, q / 8 < ranks ? f.cols : 0);
+      else wr[i] = fetch<WHOLE>(weights + (size_t)min(c0 + q / (4 * KS), f.cols - 1) * f.R, q % (4 * KS) * 8, ranks);
+    }
+    if (ADD)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) yv[i][s] = fetch<WHOLE>(f.y + row[i][s] * f.ldy, c0 + c8, f.cols);
+#pragma unroll
+    for (int i = 0; i < 4 * KS; ++i) {
+      const int q = i * WAVE + lane;
+      if (TR) *(v4u*)&mine[q / 8 * L::LD + c8] = keep<WHOLE>(wr[i], c0 + c8, q / 8 < ranks ? f.cols : 0);
+      else *(v4u*)&mine[q / (4 * KS) * L::LD + q % (4 * KS) * 8] = keep<WHOLE>(wr[i], q % (4 * KS) * 8, ranks);
+    }
+    wave_lds_sync();
+    v4u wf[4][KS];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        wf[j][k] = TR ? frag_tr<L::LD>(mine, 32 * k, 16 * j) : frag<L::LD>(mine, 16 * j, 32 * k);
+    wave_lds_sync();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      v4f acc[4] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const v4u lo = frag<32 * KS + 8>(lds.h.part[1][0], 16 * i, 32 * k);
+        const v4u hi = frag<32 * KS + 8>(lds.h.part[0][0], 16 * i, 32 * k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[j] = mfma<DT>(wf[j][k], lo, acc[j]);
+          acc[j] = mfma<DT>(wf[j][k], hi, acc[j]);
+        }
+      }
+      if (DT != 0) {
+        const float back = lds.h.back[16 * i + col];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] *= back;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *(v4f*)&sums[col * L::SUM_LD + 16 * j + 4 * g] = acc[j];
+      wave_lds_sync();
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const v4f a = *(const v4f*)&sums[(8 * s + r8) * L::SUM_LD + c8];
+        const v4f b = *(const v4f*)&sums[(8 * s + r8) * L::SUM_LD + c8 + 4];
+        v4u o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = e < 2 ? a[2 * e] : b[2 * e - 4], y = e < 2 ? a[2 * e + 1] : b[2 * e - 3];
+          if (ADD) {
+            x += to_f32<DT>(yv[i][s][e] & 0xffffu);
+            y += to_f32<DT>(yv[i][s][e] >> 16);
+          }
+          o[e] = to_bits2<DT>(x, y);
+        }
+        if (16 * i + 8 * s + r8 < t.count) store8(f.out + row[i][s] * f.ldo + c0 + c8, o, f.cols - c0 - c8);
+      }
+      wave_lds_sync();
+    }
+  }
+}
+
+// Columns of a workgroup: as many as 32768 outputs have, where that leaves two workgroups for every CU.
+static inline int strip_of(long long tiles, int rows, int N) {
+  int strip = 32768 / rows;
+  while (strip > 256 && tiles * ((N + strip - 1) / strip) < 512) strip /= 2;
+  return strip;
 }
 
 static inline bool sizes_ok(int dtype, int rows, int n, int size, int cap, int K, int N, int R) {

@@ -86,15 +86,13 @@ __global__ __launch_bounds__(PLAN_NT) void plan_k(const void* __restrict__ ids, 
   }
 }
 
-// ---- h = s x A^T ------------------------------------------------------------------------------------------
-// A workgroup a tile and 64 ranks: its waves take turns at the depth, and are summed through LDS.
 struct Fwd {
   const uint16_t* x;
   long long ldx;
   const uint16_t *a, *b;
   const float* scale;
   Plan p;
-  int K, N, R;
+  int size, K, N, R;                       // size: rows of a tile
   float* hidden;
   const uint16_t* y;
   long long ldy;
@@ -102,144 +100,142 @@ struct Fwd {
   long long ldo;
 };
 
-template <int DT, int MT, int RB>
-__global__ __launch_bounds__(MT == 1 ? 512 : 256) void shrink_k(Fwd f) {
-  constexpr int NW = MT == 1 ? 8 : 4, T = 16 * MT, W = 16 * RB;
-  __shared__ float sums[NW][T][W];
-  if ((int)blockIdx.x >= f.p.first[f.p.n + 2]) return;
-  const Tile t = f.p.tiles[blockIdx.x];
+// Part `sub` of a tile: 16 MT of its rows. Its tile, and none where it has no rows there.
+template <int MT>
+__device__ __forceinline__ Tile part_of(const Fwd& f, int block) {
+  const int subs = f.size / (16 * MT), tile = block / subs, sub = block % subs;
+  if (tile >= f.p.first[f.p.n + 2]) return {NONE, 0, 0, 0};
+  Tile t = f.p.tiles[tile];
+  t.start += sub * 16 * MT;
+  t.count = min(16 * MT, t.count - sub * 16 * MT);
+  return t;
+}
+
+// ---- h = s x A^T ------------------------------------------------------------------------------------------
+// A workgroup 16 or 32 rows and 64 ranks: its waves take turns at the depth, 64 of it at a time, and are summed through
+// LDS. Rows of x and of A come in pieces of 128 bytes a row and go through LDS: as the matrix unit wants them, with each
+// lane's neighbour in another row, a load would take 64 accesses of 16 bytes.
+constexpr int SHRINK_NT = 512, DEPTH = 2;
+
+template <int DT, int MT, int RB, bool WHOLE>
+__global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
+  constexpr int NW = SHRINK_NT / WAVE, T = 16 * MT, W = 16 * RB, LD = 64;
+  constexpr int TILES = NW * (T + W) * LD, SUMS = 2 * NW * T * W;
+  __shared__ alignas(16) uint16_t lds[TILES > SUMS ? TILES : SUMS];
+  const Tile t = part_of<MT>(f, (int)blockIdx.x);
+  if (t.count <= 0) return;
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
-  const int r0 = (int)blockIdx.y * W;
+  const int r8 = lane / 8, c8 = lane % 8 * 8, r0 = (int)blockIdx.y * W;
   if (t.adapter < 0) {
     const float v = t.adapter == NONE ? 0.f : __builtin_nanf("");
-    for (int i = (int)threadIdx.x; i < t.count * W; i += NW * WAVE)
+    for (int i = (int)threadIdx.x; i < t.count * W; i += SHRINK_NT)
       if (r0 + i % W < f.R)
         f.hidden[(size_t)f.p.order[t.start + i / W] * f.R + r0 + i % W] = v;
     return;
   }
-  const uint16_t *xp[MT], *ap[RB];
+  uint16_t *xt = lds + w * (T + W) * LD, *at = xt + T * LD;
+  const uint16_t *xp[2 * MT], *ap[2 * RB];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)             // (rows past the tile's last: its last again, not stored)
-    xp[i] = f.x + (size_t)f.p.order[t.start + min(16 * i + col, t.count - 1)] * f.ldx;
+  for (int i = 0; i < 2 * MT; ++i)         // (rows past the last: the last again, not stored)
+    xp[i] = f.x + (size_t)f.p.order[t.start + min(8 * i + r8, t.count - 1)] * f.ldx;
 #pragma unroll
-  for (int j = 0; j < RB; ++j)
-    ap[j] = f.a + ((size_t)t.adapter * f.R + min(r0 + 16 * j + col, f.R - 1)) * f.K;
+  for (int j = 0; j < 2 * RB; ++j)
+    ap[j] = f.a + ((size_t)t.adapter * f.R + min(r0 + 8 * j + r8, f.R - 1)) * f.K;
+  v4u xv[DEPTH][2 * MT], av[DEPTH][2 * RB];
+  auto load = [&](int d, int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) xv[d][i] = fetch<WHOLE>(xp[i], k + c8, f.K);
+#pragma unroll
+    for (int j = 0; j < 2 * RB; ++j) av[d][j] = fetch<WHOLE>(ap[j], k + c8, f.K);
+  };
+  // chunks of 16 bytes swapped by the row, so that a fragment's 16 rows lie over all banks
+  const int at16 = (lane % 8 ^ r8) * 8;
+  auto fr = [&](const uint16_t* tile, int row, int k) __attribute__((always_inline)) {
+    return *(const v4u*)&tile[(row + col) * LD + ((k / 8 + g) ^ (col % 8)) * 8];
+  };
   v4f acc[MT][RB] = {};
-#pragma unroll 2
-  for (int k = w * 32; k < f.K; k += NW * 32) {
-    const int kk = k + 8 * g;
-    v4u xv[MT], av[RB];
+  constexpr int STEP = NW * 64;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xv[i] = load8(xp[i] + kk, f.K - kk);
+  for (int d = 0; d < DEPTH; ++d)
+    if (w * 64 + d * STEP < f.K) load(d, w * 64 + d * STEP);
+  for (int k0 = w * 64; k0 < f.K; k0 += DEPTH * STEP)
 #pragma unroll
-    for (int j = 0; j < RB; ++j) av[j] = load8(ap[j] + kk, f.K - kk);
+    for (int d = 0; d < DEPTH; ++d) {
+      const int k = k0 + d * STEP;
+      if (k >= f.K) break;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < 2 * MT; ++i) *(v4u*)&xt[(8 * i + r8) * LD + at16] = keep<WHOLE>(xv[d][i], k + c8, f.K);
 #pragma unroll
-      for (int j = 0; j < RB; ++j) acc[i][j] = mfma<DT>(xv[i], av[j], acc[i][j]);
-  }
+      for (int j = 0; j < 2 * RB; ++j) *(v4u*)&at[(8 * j + r8) * LD + at16] = keep<WHOLE>(av[d][j], k + c8, f.K);
+      wave_lds_sync();
+      if (k + DEPTH * STEP < f.K) load(d, k + DEPTH * STEP);
+#pragma unroll
+      for (int s = 0; s < 64; s += 32) {
+        v4u xf[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[i] = fr(xt, 16 * i, s);
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+          const v4u af = fr(at, 16 * j, s);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[i][j] = mfma<DT>(xf[i], af, acc[i][j]);
+        }
+      }
+      wave_lds_sync();
+    }
+  __syncthreads();
+  float* sums = (float*)lds;               // [NW][T][W]
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < RB; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[w][16 * i + 4 * g + e][16 * j + col] = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) sums[(w * T + 16 * i + 4 * g + e) * W + 16 * j + col] = acc[i][j][e];
   __syncthreads();
   const float s = f.scale[t.adapter];
-  for (int i = (int)threadIdx.x; i < t.count * W; i += NW * WAVE) {
+  for (int i = (int)threadIdx.x; i < t.count * W; i += SHRINK_NT) {
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < NW; ++k) v += sums[k][i / W][i % W];
+    for (int q = 0; q < NW; ++q) v += sums[q * T * W + i];
     if (r0 + i % W < f.R) f.hidden[(size_t)f.p.order[t.start + i / W] * f.R + r0 + i % W] = s * v;
   }
 }
 
-// ---- out = y + h B^T --------------------------------------------------------------------------------------
-// h goes in as a sum of two 16-bit values, so that it is not rounded to the operands' type. Outputs come by four
-// consecutive columns a lane and instruction: with rows of B handed out by fours, two of them make 16 bytes.
-constexpr int STRIP = 512;                 // columns of a workgroup
 
-template <int DT, int MT, int KS>
-__global__ __launch_bounds__(256) void expand_k(Fwd f, int strips) {
-  const int tile = (int)(blockIdx.x / (unsigned)strips), n0 = (int)(blockIdx.x % (unsigned)strips) * STRIP;
+template <int DT, int MT, int KS, bool WHOLE>
+__global__ __launch_bounds__(EXPAND_NT) void expand_k(Fwd f, int strips, int strip) {
+  __shared__ ExpandLds<MT, KS, false> lds;
+  const int tile = (int)(blockIdx.x / (unsigned)strips);
   if (tile >= f.p.first[f.p.n + 2]) return;
   const Tile t = f.p.tiles[tile];
-  const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
-  int row[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) row[i] = f.p.order[t.start + min(16 * i + col, t.count - 1)];
-  if (t.adapter == NONE) {
-    if (f.y == f.out && f.ldy == f.ldo) return;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      if (16 * i + col < t.count)
-        for (int c = n0 + w * 32 + 8 * g; c < min(n0 + STRIP, f.N); c += 128)
-          store8(f.out + (size_t)row[i] * f.ldo + c, load8(f.y + (size_t)row[i] * f.ldy + c, f.N - c),
-                 f.N - c);
-    return;
-  }
-  v4u hi[MT][KS], lo[MT][KS];
-  float back[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-    back[i] = split_row<DT, KS>(f.hidden + (size_t)row[i] * f.R, f.R, g, hi[i], lo[i]);
-  const uint16_t* b = f.b + (size_t)max(t.adapter, 0) * f.N * f.R;       // (BAD: h is NaN)
-  for (int c0 = n0 + w * 32; c0 < min(n0 + STRIP, f.N); c0 += 128) {
-    v4u bv[2][KS];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = min(c0 + col / 4 * 8 + j * 4 + col % 4, f.N - 1);
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        bv[j][k] = load8(b + (size_t)n * f.R + 32 * k + 8 * g, f.R - 32 * k - 8 * g);
-    }
-    const int c = c0 + 8 * g;
-    v4u yv[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      yv[i] = v4u{};
-      if (16 * i + col < t.count) yv[i] = load8(f.y + (size_t)row[i] * f.ldy + c, f.N - c);
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      v4f acc[2] = {};
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[j] = mfma<DT>(bv[j][k], lo[i][k], acc[j]);
-          acc[j] = mfma<DT>(bv[j][k], hi[i][k], acc[j]);
-        }
-      v4u o;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = acc[e / 2][e % 2 * 2], q = acc[e / 2][e % 2 * 2 + 1];
-        o[e] = to_bits<DT>(to_f32<DT>(yv[i][e] & 0xffffu) + (DT == 0 ? p : p * back[i])) |
-               to_bits<DT>(to_f32<DT>(yv[i][e] >> 16) + (DT == 0 ? q : q * back[i])) << 16;
-      }
-      if (16 * i + col < t.count) store8(f.out + (size_t)row[i] * f.ldo + c, o, f.N - c);
-    }
-  }
+  const int n0 = (int)(blockIdx.x % (unsigned)strips) * strip;
+  const Out o = {f.hidden, f.b, f.y, f.ldy, f.out, f.ldo, f.N, f.R};
+  expand<DT, MT, KS, WHOLE, false, true>(o, f.p, t, n0, min(n0 + strip, f.N), lds);
 }
 
-template <int DT, int MT>
+template <int DT, bool WHOLE>
 static void forward(const Fwd& f, hipStream_t stream) {
-  const int strips = (f.N + STRIP - 1) / STRIP;
-  const dim3 tiles((unsigned)f.p.cap), half((unsigned)f.p.cap, 2);
-  const dim3 grid((unsigned)f.p.cap * strips);
-#define RLU_SHRINK(RB, G) \
-  hipLaunchKernelGGL((shrink_k<DT, MT, RB>), G, dim3(MT == 1 ? 512 : 256), 0, stream, f)
-  if (f.R <= 16) RLU_SHRINK(1, tiles);
-  else if (f.R <= 32) RLU_SHRINK(2, tiles);
-  else if (f.R <= 64) RLU_SHRINK(4, tiles);
-  else RLU_SHRINK(4, half);
-#undef RLU_SHRINK
-#define RLU_EXPAND(KS) \
-  hipLaunchKernelGGL((expand_k<DT, MT, KS>), grid, dim3(256), 0, stream, f, strips)
-  if (f.R <= 32) RLU_EXPAND(1);
-  else if (f.R <= 64) RLU_EXPAND(2);
-  else RLU_EXPAND(4);
+  const int strip = strip_of(f.p.cap, f.size, f.N), strips = (f.N + strip - 1) / strip;
+#define RLU_SHRINK(MT, RB, Y)                                                                      \
+  hipLaunchKernelGGL((shrink_k<DT, MT, RB, WHOLE>), dim3(f.p.cap * (f.size / (16 * MT)), Y),       \
+                     dim3(SHRINK_NT), 0, stream, f)
+#define RLU_EXPAND(MT, KS)                                                                         \
+  hipLaunchKernelGGL((expand_k<DT, MT, KS, WHOLE>), dim3(f.p.cap * strips), dim3(EXPAND_NT), 0,    \
+                     stream, f, strips, strip)
+#define RLU_FORWARD(MT, ALL)                                                                       \
+  do {                                                                                             \
+    if (f.R <= 16) RLU_SHRINK(MT, 1, 1);                                                           \
+    else if (f.R <= 32) RLU_SHRINK(MT, 2, 1);                                                      \
+    else RLU_SHRINK(MT, 4, f.R <= 64 ? 1 : 2);                                                     \
+    if (f.R <= 32) RLU_EXPAND(ALL, 1);                                                             \
+    else if (f.R <= 64) RLU_EXPAND(ALL, 2);                                                        \
+    else RLU_EXPAND(ALL, 4);                                                                       \
+  } while (0)
+  if (f.size == 16) RLU_FORWARD(1, 1);
+  else RLU_FORWARD(2, 4);
+#undef RLU_FORWARD
 #undef RLU_EXPAND
+#undef RLU_SHRINK
 }
 
 }  // namespace lora
@@ -268,19 +264,20 @@ extern "C" int rlu_lora_add(const void* x, long long ldx, const void* a, const v
   if (rows == 0) return 0;
   if (!x || !a || !b || !scale || !order || !tiles || !first || !hidden || !y || !out) return -1;
   if (rows > 1 && ldo < N) return -1;
-  if ((long long)cap * ((N + STRIP - 1) / STRIP) > UINT32_MAX / 256 ||
-      (long long)cap > UINT32_MAX / 512)
+  const long long parts = cap * (size / 16ll);
+  if (cap * ((N + 255ll) / 256) > UINT32_MAX / EXPAND_NT || parts > UINT32_MAX / SHRINK_NT)
     return -1;                                         // (a launch counts its threads in 32 bits)
   if (((uintptr_t)x | (uintptr_t)a | (uintptr_t)b | (uintptr_t)y | (uintptr_t)out) % 2 ||
       ((uintptr_t)scale | (uintptr_t)hidden | (uintptr_t)order | (uintptr_t)first) % 4 ||
       (uintptr_t)tiles % 16)
     return -4;
   Fwd f = {(const uint16_t*)x, ldx, (const uint16_t*)a, (const uint16_t*)b, scale,
-           {order, (const Tile*)tiles, first, n, rows, cap}, K, N, R, hidden, (const uint16_t*)y, ldy,
+           {order, (const Tile*)tiles, first, n, rows, cap}, size, K, N, R, hidden, (const uint16_t*)y, ldy,
            (uint16_t*)out, ldo};
-  if (dtype == 0 && size == 16) forward<0, 1>(f, stream);
-  else if (dtype == 0) forward<0, 4>(f, stream);
-  else if (size == 16) forward<2, 1>(f, stream);
-  else forward<2, 4>(f, stream);
+  const bool whole = (K | N | R) % 8 == 0;
+  if (dtype == 0 && whole) forward<0, true>(f, stream);
+  else if (dtype == 0) forward<0, false>(f, stream);
+  else if (whole) forward<2, true>(f, stream);
+  else forward<2, false>(f, stream);
   return (int)hipGetLastError();
 }
