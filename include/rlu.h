@@ -392,7 +392,7 @@ int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* 
 
 /* ---- low-rank adapters ---------------------------------------------------------------------------------
  * No counterpart in the reference: n adapters beside one projection, a [n][R][K], b [n][N][R], scale [n] f32.
- * dtype 0 bf16, 2 f16. 1 <= n <= 1024, 1 <= R <= 128, 1 <= K, N <= 2^24. R columns, K and N may be odd, every 16-bit
+ * dtype 0 bf16, 2 f16. 1 <= n <= 1024, 1 <= R <= 128, 1 <= K, N <= 2^24, rows <= 2^24. R, K and N may be odd, every 16-bit
  * operand lies at any element's address, its rows ld elements apart.
  * rlu_lora_plan: a batch's rows by adapter, once for all its projections. ids [rows] int64 (wide 1) or int32: below
  *   0 none, n or more: the row becomes NaN. size: rows of a tile, 16 or 64. cap = rows / size + min(rows, n + 2).
@@ -401,7 +401,7 @@ int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* 
  *   (y in those), with two launches. out may be y (same address and ld), but overlaps nothing else.
  * rlu_lora_grad: from dy [rows][N] and hidden as rlu_lora_add left it, with u = scale dy b: dx [rows][K] = u a (0 in
  *   rows without an adapter), da = u^T x, db = dy^T hidden of each adapter over its rows (0 for one without rows);
- *   each may be NULL. ws: what rlu_lora_grad_workspace says, 16-byte aligned, used until the kernels end.
+ *   each may be NULL. lddy, ldx < 2^31. ws: what rlu_lora_grad_workspace says, 16-byte aligned, used until the kernels end.
  * rows = 0 launches nothing. Returns -1 (bad sizes, more than 2^32 threads, or a NULL pointer), -4 (misaligned). */
 int rlu_lora_plan(const void* ids, int wide, int rows, int n, int size, int cap, int* order,
                   int* tiles, int* first, hipStream_t stream);

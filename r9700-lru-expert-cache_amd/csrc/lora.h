@@ -135,9 +135,10 @@ template <int DT>
 struct Split {
   uint32_t hi, lo;
   __device__ __forceinline__ explicit Split(float f) {
-    hi = to_bits<DT>(f);
-    const float r = f - to_f32<DT>(hi);
-    lo = to_bits<DT>(r == r ? r : 0.f);                // (an infinity's rest)
+    hi = DT == 0 ? f32_to_bf16_hw(f) : to_bits<DT>(f);
+    float r = f - to_f32<DT>(hi);
+    r = r == r ? r : 0.f;                              // (an infinity's rest)
+    lo = DT == 0 ? f32_to_bf16_hw(r) : to_bits<DT>(r);
   }
 };
 
@@ -327,7 +328,7 @@ static inline int strip_of(long long tiles, int rows, int N) {
 }
 
 static inline bool sizes_ok(int dtype, int rows, int n, int size, int cap, int K, int N, int R) {
-  return (dtype == 0 || dtype == 2) && rows >= 0 && n >= 1 && n <= MAX_ADAPTERS &&
+  return (dtype == 0 || dtype == 2) && rows >= 0 && rows <= 1 << 24 && n >= 1 && n <= MAX_ADAPTERS &&
          (size == 16 || size == 64) && K >= 1 && N >= 1 && K <= 1 << 24 && N <= 1 << 24 && R >= 1 &&
          R <= MAX_RANK && cap == (int)(rows / size + (rows < n + 2 ? rows : n + 2));
 }

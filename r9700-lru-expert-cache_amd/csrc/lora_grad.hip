@@ -28,7 +28,7 @@ struct Bwd {
   long long lddx;
   uint16_t *da, *db;
   // workspace
-  float* upart;                            // [strips of N][rows][R]
+  float* upart;                            // [strips of N][rows R, and 64 that nobody reads]
   float* u;                                // [rows][R]
   float *pa, *pb;                          // [sa][2][R][K], [sb][2][N][R]
   int sa, sb;                              // runs of tiles
@@ -55,24 +55,27 @@ __device__ __forceinline__ Side side_of(const Bwd& f) {
 template <int RB, bool DB>
 struct OuterLds {
   static constexpr int W = 16 * RB;
-  alignas(16) uint16_t v[NW][32 * 72];     // a wave's rows; before them its part of B
+  alignas(16) uint16_t v[NW * 32 * 72];    // the step's rows [32][VLD]; before them each wave's part of B
   alignas(16) uint16_t h[2][W * 40];       // both parts of h or u, [rank][row]
   float u[DB ? NW : 1][DB ? 32 * W : 1];
   float top[NW];
 };
 
 template <int DT, int RB, bool WHOLE, bool DB>
-__global__ __launch_bounds__(NT) void outer_k(Bwd f) {
-  constexpr int W = 16 * RB, EACH = 32 * W / NT, LDB = W + 8;
+__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd f) {
+  constexpr int W = 16 * RB, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
   __shared__ OuterLds<RB, DB> lds;
   const Side o = side_of<DB>(f);
   const int strips = (o.cols + OUTER - 1) / OUTER, run = (int)blockIdx.x / strips, strip = (int)blockIdx.x % strips;
   const int total = f.p.first[f.p.n], per = (total + o.runs - 1) / o.runs;
   const int t0 = run * per, t1 = min(t0 + per, total);
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE), col = lane % 16, g = lane / 16;
-  const int r8 = lane / 8, c8 = lane % 8 * 8, r0 = (int)blockIdx.y * W;
+  const int r0 = (int)blockIdx.y * W;
   const int c0 = strip * OUTER + w * 64;
-  uint16_t* mine = lds.v[w];
+  uint16_t* mine = lds.v + w * 32 * 72;
+  const int vr = w * 8 + lane / 32, vc = strip * OUTER + lane % 32 * 8;        // of the rows this lane brings
+  const uint32_t spare = (uint32_t)f.p.rows * f.R;     // (rows of 64 more behind each strip's part)
+  float* upart = f.upart + (size_t)strip * (spare + WAVE);
   for (int tile = t0; tile < t1;) {
     const int a = f.p.tiles[tile].adapter, first = f.p.first[a], last = f.p.first[a + 1], end = min(last, t1);
     const int p0 = f.p.tiles[tile].start, p1 = f.p.tiles[end - 1].start + f.p.tiles[end - 1].count;
@@ -93,64 +96,82 @@ __global__ __launch_bounds__(NT) void outer_k(Bwd f) {
         for (int j = 0; j < RB; ++j) bu[k][j] = frag_tr<LDB>(mine, 0, 16 * j);
         wave_lds_sync();
       }
+      lds_barrier();                       // (the rows come to the same place)
     }
     const float s = DB ? f.scale[a] : 1.f;
     v4f acc[RB][4] = {};
-    // of the next step: its rows' places, its rows, its h
-    int vrow[4], hrow[EACH];
+    // of the next step: its rows' places, its rows, its h. Places are asked for before the rows of the step before: what
+    // comes back in order is waited for in order.
+    struct Places {
+      int v[4], h[EACH];
+    };
+    auto places = [&](int pos) __attribute__((always_inline)) {        // (past the end: the last row again)
+      Places n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n.v[i] = f.p.order[min(pos + vr + 2 * i, p1 - 1)];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) n.h[i] = f.p.order[min(pos + (tid + i * NT) / W, p1 - 1)];
+      return n;
+    };
+    int hrow[EACH], hcol[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) hcol[i] = min(r0 + (tid + i * NT) % W, f.R - 1);
     v4u vv[4];
     float hv[EACH];
-    auto rows = [&](int pos) __attribute__((always_inline)) {
+    auto load = [&](const Places& at) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vrow[i] = f.p.order[min(pos + 8 * i + r8, p1 - 1)];
+      for (int i = 0; i < 4; ++i) vv[i] = fetch<WHOLE, true>(o.v + (uint64_t)(uint32_t)at.v[i] * (uint32_t)o.ld, vc, o.cols);
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) hrow[i] = f.p.order[min(pos + (tid + i * NT) / W, p1 - 1)];
+      for (int i = 0; i < EACH; ++i) {
+        hrow[i] = at.h[i];
+        hv[i] = o.h[(uint32_t)at.h[i] * (uint32_t)f.R + hcol[i]];
+      }
     };
-    auto load = [&]() __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) vv[i] = fetch<WHOLE>(o.v + (size_t)vrow[i] * o.ld, c0 + c8, o.cols);
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) hv[i] = o.h[(size_t)hrow[i] * f.R + min(r0 + (tid + i * NT) % W, f.R - 1)];
-    };
-    rows(p0);
-    load();
-    int urow[EACH];
+    Places at = places(p0);
+    {
+      const Places next = places(p0 + 32);
+      load(at);
+      at = next;
+    }
     for (int pos = p0; pos < p1; pos += 32) {
+      int urow[EACH];
       float by = 1.f;
       if (DT != 0) {                       // float16: h and u into its range by a power of two a step
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < EACH; ++i) m = fmaxf(m, fabsf(hv[i]));
 #pragma unroll
-        for (int d = 1; d < WAVE; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+        for (int l = 1; l < WAVE; l *= 2) m = fmaxf(m, __shfl_xor(m, l));
         if (lane == 0) lds.top[w] = m;
-        __syncthreads();
+        lds_barrier();
         by = scale_to(fmaxf(fmaxf(lds.top[0], lds.top[1]), fmaxf(lds.top[2], lds.top[3])));
       }
+      if (pos + 32 > p1 || (strip + 1) * OUTER > o.cols)               // zeros past the last row and column
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool in = pos + 8 * i + r8 < p1;         // (rows past the last: zeros)
-        *(v4u*)&mine[(8 * i + r8) * 72 + c8] = in ? keep<WHOLE>(vv[i], c0 + c8, o.cols) : v4u{};
-      }
+        for (int i = 0; i < 4; ++i)
+          vv[i] = pos + vr + 2 * i < p1 ? keep<WHOLE>(vv[i], vc, o.cols) : v4u{};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *(v4u*)&lds.v[(vr + 2 * i) * VLD + lane % 32 * 8] = vv[i];
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int q = tid + i * NT;
-        const bool in = pos + q / W < p1 && r0 + q % W < f.R;
+        const bool in = q / W < p1 - pos && q % W < f.R - r0;
         const Split<DT> p(in ? hv[i] * by : 0.f);
         lds.h[0][q % W * 40 + q / W] = (uint16_t)p.hi;
         lds.h[1][q % W * 40 + q / W] = (uint16_t)p.lo;
         urow[i] = hrow[i];
       }
-      __syncthreads();
-      rows(pos + 32);                      // (past the end: the last row again)
-      load();
+      lds_barrier();
+      const Places next = places(pos + 64);
+      load(at);
+      at = next;
       if (DB) {
         v4f u[2][RB] = {};
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const v4u vf = frag<72>(mine, 16 * i, 32 * k);
+            const v4u vf = frag<VLD>(lds.v, 16 * i, w * 64 + 32 * k);
 #pragma unroll
             for (int j = 0; j < RB; ++j) u[i][j] = mfma<DT>(vf, bu[k][j], u[i][j]);
           }
@@ -169,26 +190,28 @@ __global__ __launch_bounds__(NT) void outer_k(Bwd f) {
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const v4u vf = frag_tr<72>(mine, 0, 16 * c);
+        const v4u vf = frag_tr<VLD>(lds.v, 0, w * 64 + 16 * c);
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
-          v4f d = DT != 0 ? v4f{} : acc[j][c];
-          d = DB ? mfma<DT>(vf, lo[j], d) : mfma<DT>(lo[j], vf, d);
-          d = DB ? mfma<DT>(vf, hi[j], d) : mfma<DT>(hi[j], vf, d);
-          if (DT == 0) acc[j][c] = d;
+          v4f t = DT != 0 ? v4f{} : acc[j][c];
+          t = DB ? mfma<DT>(vf, lo[j], t) : mfma<DT>(lo[j], vf, t);
+          t = DB ? mfma<DT>(vf, hi[j], t) : mfma<DT>(hi[j], vf, t);
+          if (DT == 0) acc[j][c] = t;
           else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][c][e] = fmaf(d[e], 1.f / by, acc[j][c][e]);
+            for (int e = 0; e < 4; ++e) acc[j][c][e] = fmaf(t[e], 1.f / by, acc[j][c][e]);
         }
       }
-      __syncthreads();
+      lds_barrier();
       if (DB) {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
+          // (no branch around the store: the waits after one would be for all that is on its way, this store among
+          // it. What lies past the last row or rank goes to a row that nobody reads.)
           const int q = tid + i * NT;
-          if (pos + q / W < p1 && r0 + q % W < f.R)
-            f.upart[((size_t)strip * f.p.rows + urow[i]) * f.R + r0 + q % W] =
-                s * ((lds.u[0][q] + lds.u[1][q]) + (lds.u[2][q] + lds.u[3][q]));
+          const bool in = q / W < p1 - pos && q % W < f.R - r0;
+          upart[in ? (uint32_t)urow[i] * (uint32_t)f.R + hcol[i] : spare + lane] =
+              s * ((lds.u[0][q] + lds.u[1][q]) + (lds.u[2][q] + lds.u[3][q]));
         }
       }
     }
@@ -245,7 +268,7 @@ __global__ __launch_bounds__(NT) void sum_k(Bwd f) {
   const bool in = i < t.count * f.R;
   const size_t at = in ? (size_t)f.p.order[t.start + i / f.R] * f.R + i % f.R : 0;
   const int strips = (f.N + OUTER - 1) / OUTER;
-  const size_t step = (size_t)f.p.rows * f.R;
+  const size_t step = (size_t)f.p.rows * f.R + WAVE;
   float v = 0.f;
   if (in && t.adapter >= 0)
 #pragma unroll 8
@@ -285,7 +308,7 @@ static void layout(Bwd& f, long long* bytes) {
     return was;
   };
   uint8_t* ws = (uint8_t*)f.upart;
-  f.upart = (float*)(ws + take(4ll * strips * f.p.rows * f.R));
+  f.upart = (float*)(ws + take(4ll * strips * (1ll * f.p.rows * f.R + WAVE)));
   f.u = (float*)(ws + take(4ll * f.p.rows * f.R));
   f.pa = (float*)(ws + take(f.sa > 1 ? 8ll * f.sa * f.R * f.K : 0));
   f.pb = (float*)(ws + take(f.sb > 1 ? 8ll * f.sb * f.R * f.N : 0));
@@ -368,7 +391,9 @@ extern "C" int rlu_lora_grad(const void* dy, long long lddy, const void* x, long
   Bwd f = {};
   f.upart = (float*)ws;
   long long bytes;
-  if (grad_sizes(f, dtype, rows, n, size, cap, K, N, R, &bytes) || lddy < 0 || ldx < 0) return -1;
+  if (grad_sizes(f, dtype, rows, n, size, cap, K, N, R, &bytes) || lddy < 0 || ldx < 0 ||
+      lddy > INT32_MAX || ldx > INT32_MAX)
+    return -1;
   if (rows == 0) return 0;
   if (!dy || !x || !a || !b || !scale || !order || !tiles || !first || !hidden || !ws) return -1;
   if (dx && rows > 1 && lddx < K) return -1;
