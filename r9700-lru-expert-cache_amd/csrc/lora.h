@@ -164,16 +164,17 @@ struct Rows {
   uint16_t part[2][T][LD];
   float back[T];
 };
-template <int DT, int MT, int KS, int NT>
-__device__ __forceinline__ void stage(Rows<MT, KS>& s, const Plan& p, const Tile& t, const float* h, int R) {
+// rows: where the row-th of `count` rows lies
+template <int DT, int MT, int KS, int NT, class At>
+__device__ __forceinline__ void stage(Rows<MT, KS>& s, int count, int R, At rows) {
   constexpr int PER = NT / (16 * MT), N = (4 * KS + PER - 1) / PER;    // threads a row, chunks of 8 a thread
   const int row = (int)threadIdx.x / PER, q = (int)threadIdx.x % PER;
-  const float* from = h + (size_t)p.order[t.start + min(row, t.count - 1)] * R;
+  const float* from = rows(min(row, count - 1));
   float v[N][8], m = 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int c = k * PER + q;
-    load8(from + 8 * c, c < 4 * KS && row < t.count ? R - 8 * c : 0, v[k]);
+    load8(from + 8 * c, c < 4 * KS && row < count ? R - 8 * c : 0, v[k]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[k][e]));
   }
@@ -205,26 +206,38 @@ __device__ __forceinline__ void stage(Rows<MT, KS>& s, const Plan& p, const Tile
 // lies in memory through LDS into registers, then 16 rows after the other. Sums leave the matrix unit with a lane's
 // neighbour another row; through LDS they come in rows of 128 bytes, as y and out are read and written.
 struct Out {
-  const float* h;
   const uint16_t *w, *y;
   long long ldy;
   uint16_t* out;
   long long ldo;
   int cols, R;
 };
-constexpr int EXPAND_NT = 256, EXPAND_NW = EXPAND_NT / WAVE;
-template <int MT, int KS, bool TR>
+constexpr int EXPAND_NT = 256;
+template <int MT, int KS, bool TR, int NT = EXPAND_NT>
 struct ExpandLds {
   static constexpr int LD = TR ? 72 : 32 * KS + 8, SUM_LD = 68;
   static constexpr int W = TR ? 32 * KS * LD : 64 * LD, SUMS = 2 * 16 * SUM_LD;
   Rows<MT, KS> h;
-  alignas(16) uint16_t wave[EXPAND_NW][W > SUMS ? W : SUMS];           // W, then a block's sums
+  alignas(16) uint16_t wave[NT / WAVE][W > SUMS ? W : SUMS];           // W, then a block's sums
 };
 
-template <int DT, int MT, int KS, bool WHOLE, bool TR, bool ADD>
+// Rows without an adapter: out = y.
+template <int NT = EXPAND_NT>
+__device__ __forceinline__ void copy(const Out& f, const Plan& p, const Tile& t, int n0, int n1) {
+  if (f.y == f.out && f.ldy == f.ldo) return;
+  for (int r = (int)threadIdx.x / 32; r < t.count; r += NT / 32) {
+    const size_t row = p.order[t.start + r];
+    for (int c = n0 + (int)threadIdx.x % 32 * 8; c < n1; c += 256)
+      store8(f.out + row * f.ldo + c, load8(f.y + row * f.ldy + c, f.cols - c), f.cols - c);
+  }
+}
+
+// lds.h is staged; its barrier is to come.
+template <int DT, int MT, int KS, bool WHOLE, bool TR, bool ADD, int NT = EXPAND_NT>
 __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& t, int n0, int n1,
-                                       ExpandLds<MT, KS, TR>& lds) {
-  typedef ExpandLds<MT, KS, TR> L;
+                                       ExpandLds<MT, KS, TR, NT>& lds) {
+  typedef ExpandLds<MT, KS, TR, NT> L;
+  constexpr int STEP = NT;                 // columns: 64 a wave
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
   const int r8 = lane / 8, c8 = lane % 8 * 8;
   size_t row[MT][2];
@@ -232,24 +245,12 @@ __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int s = 0; s < 2; ++s) row[i][s] = p.order[t.start + min(16 * i + 8 * s + r8, t.count - 1)];
-  if (ADD && t.adapter == NONE) {
-    if (f.y == f.out && f.ldy == f.ldo) return;
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        if (16 * i + 8 * s + r8 < t.count)
-          for (int c = n0 + w * 64 + c8; c < n1; c += EXPAND_NW * 64)
-            store8(f.out + row[i][s] * f.ldo + c, load8(f.y + row[i][s] * f.ldy + c, f.cols - c), f.cols - c);
-    return;
-  }
   const uint16_t* weights = f.w + (size_t)max(t.adapter, 0) * f.cols * f.R;       // (BAD: h is NaN)
   const int ranks = t.adapter == NONE ? 0 : f.R;       // (0 times whatever adapter 0 holds may be NaN)
   uint16_t* mine = lds.wave[w];
   float* sums = (float*)mine;
-  stage<DT, MT, KS, EXPAND_NT>(lds.h, p, t, f.h, f.R);
   __syncthreads();
-  for (int c0 = n0 + w * 64; c0 < n1; c0 += EXPAND_NW * 64) {
+  for (int c0 = n0 + w * 64; c0 < n1; c0 += STEP) {
     v4u wr[4 * KS], yv[MT][2];
 #pragma unroll
     for (int i = 0; i < 4 * KS; ++i) {

@@ -117,23 +117,21 @@ __device__ __forceinline__ Tile part_of(const Fwd& f, int block) {
 // lane's neighbour in another row, a load would take 64 accesses of 16 bytes.
 constexpr int SHRINK_NT = 512, DEPTH = 2;
 
-template <int DT, int MT, int RB, bool WHOLE>
-__global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
-  constexpr int NW = SHRINK_NT / WAVE, T = 16 * MT, W = 16 * RB, LD = 64;
-  constexpr int TILES = NW * (T + W) * LD, SUMS = 2 * NW * T * W;
-  __shared__ alignas(16) uint16_t lds[TILES > SUMS ? TILES : SUMS];
-  const Tile t = part_of<MT>(f, (int)blockIdx.x);
-  if (t.count <= 0) return;
+template <int MT, int RB>
+struct ShrinkLds {
+  static constexpr int NW = SHRINK_NT / WAVE, T = 16 * MT, W = 16 * RB, LD = 64;
+  static constexpr int TILES = NW * (T + W) * LD, SUMS = 2 * NW * T * W;
+  alignas(16) uint16_t tiles[TILES > SUMS ? TILES : SUMS];             // rows of x and A, then each wave's sums
+};
+
+// Calls put(row, rank, h) for the rows of t and the ranks from r0 on.
+template <int DT, int MT, int RB, bool WHOLE, class Put>
+__device__ __forceinline__ void shrink(const Fwd& f, const Tile& t, int r0, ShrinkLds<MT, RB>& lds, Put put) {
+  typedef ShrinkLds<MT, RB> L;
+  constexpr int NW = L::NW, T = L::T, W = L::W, LD = L::LD;
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
-  const int r8 = lane / 8, c8 = lane % 8 * 8, r0 = (int)blockIdx.y * W;
-  if (t.adapter < 0) {
-    const float v = t.adapter == NONE ? 0.f : __builtin_nanf("");
-    for (int i = (int)threadIdx.x; i < t.count * W; i += SHRINK_NT)
-      if (r0 + i % W < f.R)
-        f.hidden[(size_t)f.p.order[t.start + i / W] * f.R + r0 + i % W] = v;
-    return;
-  }
-  uint16_t *xt = lds + w * (T + W) * LD, *at = xt + T * LD;
+  const int r8 = lane / 8, c8 = lane % 8 * 8;
+  uint16_t *xt = lds.tiles + w * (T + W) * LD, *at = xt + T * LD;
   const uint16_t *xp[2 * MT], *ap[2 * RB];
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i)         // (rows past the last: the last again, not stored)
@@ -184,7 +182,7 @@ __global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
       wave_lds_sync();
     }
   __syncthreads();
-  float* sums = (float*)lds;               // [NW][T][W]
+  float* sums = (float*)lds.tiles;         // [NW][T][W]
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -197,10 +195,27 @@ __global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < NW; ++q) v += sums[q * T * W + i];
-    if (r0 + i % W < f.R) f.hidden[(size_t)f.p.order[t.start + i / W] * f.R + r0 + i % W] = s * v;
+    if (r0 + i % W < f.R) put(i / W, r0 + i % W, s * v);
   }
 }
+// h of rows without an adapter, and of ids past the last
+template <class Put>
+__device__ __forceinline__ void bare(const Fwd& f, const Tile& t, int r0, int ranks, Put put) {
+  const float v = t.adapter == NONE ? 0.f : __builtin_nanf("");
+  for (int i = (int)threadIdx.x; i < t.count * ranks; i += SHRINK_NT)
+    if (r0 + i % ranks < f.R) put(i / ranks, r0 + i % ranks, v);
+}
 
+template <int DT, int MT, int RB, bool WHOLE>
+__global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
+  __shared__ ShrinkLds<MT, RB> lds;
+  const Tile t = part_of<MT>(f, (int)blockIdx.x);
+  if (t.count <= 0) return;
+  const int r0 = (int)blockIdx.y * 16 * RB;
+  auto put = [&](int row, int r, float v) { f.hidden[(size_t)f.p.order[t.start + row] * f.R + r] = v; };
+  if (t.adapter < 0) bare(f, t, r0, 16 * RB, put);
+  else shrink<DT, MT, RB, WHOLE>(f, t, r0, lds, put);
+}
 
 template <int DT, int MT, int KS, bool WHOLE>
 __global__ __launch_bounds__(EXPAND_NT) void expand_k(Fwd f, int strips, int strip) {
@@ -208,13 +223,52 @@ __global__ __launch_bounds__(EXPAND_NT) void expand_k(Fwd f, int strips, int str
   const int tile = (int)(blockIdx.x / (unsigned)strips);
   if (tile >= f.p.first[f.p.n + 2]) return;
   const Tile t = f.p.tiles[tile];
-  const int n0 = (int)(blockIdx.x % (unsigned)strips) * strip;
-  const Out o = {f.hidden, f.b, f.y, f.ldy, f.out, f.ldo, f.N, f.R};
-  expand<DT, MT, KS, WHOLE, false, true>(o, f.p, t, n0, min(n0 + strip, f.N), lds);
+  const int n0 = (int)(blockIdx.x % (unsigned)strips) * strip, n1 = min(n0 + strip, f.N);
+  const Out o = {f.b, f.y, f.ldy, f.out, f.ldo, f.N, f.R};
+  if (t.adapter == NONE) return copy(o, f.p, t, n0, n1);
+  stage<DT, MT, KS, EXPAND_NT>(lds.h, t.count, f.R, [&](int row) {
+    return f.hidden + (size_t)f.p.order[t.start + row] * f.R;
+  });
+  expand<DT, MT, KS, WHOLE, false, true>(o, f.p, t, n0, n1, lds);
+}
+
+// Both in one launch where the tiles' strips have a CU each: every strip's workgroup works h out for itself.
+constexpr int BOTH_STRIP = SHRINK_NT;      // columns: 64 a wave
+template <int DT, int RB, bool WHOLE>
+__global__ __launch_bounds__(SHRINK_NT) void both_k(Fwd f, int strips) {
+  constexpr int KS = (RB + 1) / 2, LD = 16 * RB + 4;
+  __shared__ union {
+    ShrinkLds<1, RB> first;
+    ExpandLds<1, KS, false, SHRINK_NT> then;
+  } lds;
+  __shared__ float h[16 * LD];
+  const int tile = (int)(blockIdx.x / (unsigned)strips), strip = (int)(blockIdx.x % (unsigned)strips);
+  if (tile >= f.p.first[f.p.n + 2]) return;
+  const Tile t = f.p.tiles[tile];
+  const int n0 = strip * BOTH_STRIP, n1 = min(n0 + BOTH_STRIP, f.N);
+  const Out o = {f.b, f.y, f.ldy, f.out, f.ldo, f.N, f.R};
+  auto put = [&](int row, int r, float v) {
+    h[row * LD + r] = v;
+    if (strip == 0) f.hidden[(size_t)f.p.order[t.start + row] * f.R + r] = v;
+  };
+  if (t.adapter < 0) bare(f, t, 0, 16 * RB, put);
+  else shrink<DT, 1, RB, WHOLE>(f, t, 0, lds.first, put);
+  if (t.adapter == NONE) return copy<SHRINK_NT>(o, f.p, t, n0, n1);
+  __syncthreads();
+  stage<DT, 1, KS, SHRINK_NT>(lds.then.h, t.count, f.R, [&](int row) { return (const float*)h + row * LD; });
+  expand<DT, 1, KS, WHOLE, false, true, SHRINK_NT>(o, f.p, t, n0, n1, lds.then);
 }
 
 template <int DT, bool WHOLE>
 static void forward(const Fwd& f, hipStream_t stream) {
+  const int two = (f.N + BOTH_STRIP - 1) / BOTH_STRIP;
+  if (f.size == 16 && f.R <= 64 && (long long)f.p.cap * two <= 256) {
+    const dim3 grid(f.p.cap * two), block(SHRINK_NT);
+    if (f.R <= 16) hipLaunchKernelGGL((both_k<DT, 1, WHOLE>), grid, block, 0, stream, f, two);
+    else if (f.R <= 32) hipLaunchKernelGGL((both_k<DT, 2, WHOLE>), grid, block, 0, stream, f, two);
+    else hipLaunchKernelGGL((both_k<DT, 4, WHOLE>), grid, block, 0, stream, f, two);
+    return;
+  }
   const int strip = strip_of(f.p.cap, f.size, f.N), strips = (f.N + strip - 1) / strip;
 #define RLU_SHRINK(MT, RB, Y)                                                                      \
   hipLaunchKernelGGL((shrink_k<DT, MT, RB, WHOLE>), dim3(f.p.cap * (f.size / (16 * MT)), Y),       \

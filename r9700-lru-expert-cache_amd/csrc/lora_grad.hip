@@ -288,8 +288,12 @@ __global__ __launch_bounds__(EXPAND_NT) void dx_k(Bwd f, int strips, int strip) 
   const int tile = (int)(blockIdx.x / (unsigned)strips);
   if (tile >= f.p.first[f.p.n + 2]) return;
   const int n0 = (int)(blockIdx.x % (unsigned)strips) * strip;
-  const Out o = {f.u, f.a, nullptr, 0, f.dx, f.lddx, f.K, f.R};
-  expand<DT, MT, KS, WHOLE, true, false>(o, f.p, f.p.tiles[tile], n0, min(n0 + strip, f.K), lds);
+  const Tile t = f.p.tiles[tile];
+  const Out o = {f.a, nullptr, 0, f.dx, f.lddx, f.K, f.R};
+  stage<DT, MT, KS, EXPAND_NT>(lds.h, t.count, f.R, [&](int row) {
+    return f.u + (size_t)f.p.order[t.start + row] * f.R;
+  });
+  expand<DT, MT, KS, WHOLE, true, false>(o, f.p, t, n0, min(n0 + strip, f.K), lds);
 }
 
 // Runs: workgroups for every CU, twice over, of 128 rows at least.

@@ -83,7 +83,7 @@ def plan_rows(ids: torch.Tensor, n: int) -> LoraRows:
     size = 16 if rows < 1024 else 64
     cap = rows // size + min(rows, n + 2)
     order = torch.empty(rows, dtype=torch.int32, device=dev)
-    tiles = torch.empty((cap, 4), dtype=torch.int32, device=dev)
+    tiles = torch.empty(cap, 4, dtype=torch.int32, device=dev)
     first = torch.empty(n + 3, dtype=torch.int32, device=dev)
     with on_device(dev):
         rc = lib().rlu_lora_plan(ids.data_ptr(), int(ids.dtype == torch.int64), rows, n, size, cap,
@@ -94,13 +94,13 @@ def plan_rows(ids: torch.Tensor, n: int) -> LoraRows:
 
 def _check_rows(name: str, what: str, t: torch.Tensor, rows: int, cols: int, w: LoraStack) -> None:
     if t.shape != (rows, cols) or t.dtype != w.a.dtype or t.device != w.a.device or \
-            (cols > 1 and t.stride(1) != 1):
+            (t.stride()[1] != 1 and cols > 1):
         raise ValueError(f"{name}: {what} must be {w.a.dtype} [{rows}, {cols}] beside the adapters, a row's elements "
                          "next to each other")
 
 
 def _check_batch(name: str, w: LoraStack, rows: LoraRows) -> None:
-    if rows.n != w.n or rows.order.device != w.a.device:
+    if rows.n != w.a.shape[0] or rows.order.device != w.a.device:
         raise ValueError(f"{name}: rows planned for {rows.n} adapters on {rows.order.device}, a stack of {w.n} "
                          f"on {w.a.device}")
 
@@ -123,17 +123,20 @@ def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
 
 
 def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride()[0] if rows > 1 else cols
 
 
 def _forward(y, x, w, rows, hidden, out) -> None:
     if rows.rows == 0:
         return
+    a, b = w.a, w.b
+    n, rank, K = a.shape
     with on_device(x.device):
         rc = lib().rlu_lora_add(
-            x.data_ptr(), _ld(x), w.a.data_ptr(), w.b.data_ptr(), w.scale.data_ptr(),
+            x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), w.scale.data_ptr(),
             _DTYPE_CODE[x.dtype], rows.order.data_ptr(), rows.tiles.data_ptr(), rows.first.data_ptr(),
-            rows.rows, w.n, rows.size, rows.tiles.shape[0], x.shape[1], y.shape[1], w.rank,
+            rows.rows, n, rows.size, rows.tiles.shape[0], K, y.shape[1], rank,
             hidden.data_ptr(), y.data_ptr(), _ld(y), out.data_ptr(), _ld(out), stream_ptr())
     check(rc, "rlu_lora_add")
 
@@ -144,29 +147,34 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
     x a^T in float32, rounded once. Rows may be apart (x, y and out of any stride). A row without an adapter is y's.
     out: where the result goes, y itself among others; a new tensor without it.
     hidden: float32 [rows, rank] that receives scale x a^T, for add_lora_grad."""
+    a, b, M = w.a, w.b, rows.rows
     _check_batch("add_lora", w, rows)
-    _check_rows("add_lora", "x", x, rows.rows, w.a.shape[2], w)
-    _check_rows("add_lora", "y", y, rows.rows, w.b.shape[1], w)
+    _check_rows("add_lora", "x", x, M, a.shape[2], w)
+    _check_rows("add_lora", "y", y, M, b.shape[1], w)
     if hidden is not None:
-        _check_hidden("add_lora", hidden, rows.rows, w)
+        _check_hidden("add_lora", hidden, M, w)
+    grad = (x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad) and \
+        torch.is_grad_enabled()
+    if grad and (out is not None or hidden is not None):
+        raise ValueError("add_lora: autograd keeps its own hidden and makes its own out; detach the operands for a "
+                         "gradient by hand")
     if out is not None:
-        _check_rows("add_lora", "out", out, rows.rows, w.b.shape[1], w)
-        if rows.rows > 1 and out.stride(0) < out.shape[1]:
+        _check_rows("add_lora", "out", out, M, b.shape[1], w)
+        if M > 1 and out.stride()[0] < out.shape[1]:
             raise ValueError("add_lora: out's rows overlap")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("add_lora: out asks for a gradient")
         same = out.data_ptr() == y.data_ptr() and _ld(out) == _ld(y)
         if (not same and _overlap(out, y)) or _overlap(out, x):
             raise ValueError("add_lora: out overlaps y or x (it may be y, or apart from both)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, y, w.a, w.b)):
-        if out is not None or hidden is not None:
-            raise ValueError("add_lora: autograd keeps its own hidden and makes its own out; detach the operands "
-                             "for a gradient by hand")
+    if grad:
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("add_lora: a captured graph takes add_lora_grad, without autograd")
-        return _AddLora.apply(y, x, w.a, w.b, w, rows)
+        return _AddLora.apply(y, x, a, b, w, rows)
     if hidden is None:
-        hidden = torch.empty((rows.rows, w.rank), dtype=torch.float32, device=x.device)
+        hidden = torch.empty(M * a.shape[1], dtype=torch.float32, device=x.device)
     if out is None:
-        out = torch.empty((rows.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+        out = torch.empty(M, b.shape[1], dtype=y.dtype, device=y.device)
     _forward(y, x, w, rows, hidden, out)
     return out
 
@@ -181,24 +189,25 @@ def _grad_workspace(dtype: int, rows: int, n: int, size: int, cap: int, K: int, 
 
 
 def _backward(dy, x, w, rows, hidden, need):
-    K, N, dev = w.a.shape[2], w.b.shape[1], x.device
-    make = torch.empty if rows.rows else torch.zeros
-    dx = torch.empty((rows.rows, K), dtype=x.dtype, device=dev) if need[0] else None
-    da = make(w.a.shape, dtype=x.dtype, device=dev) if need[1] else None
-    db = make(w.b.shape, dtype=x.dtype, device=dev) if need[2] else None
-    if rows.rows and any(need):
+    a, b, M, dev = w.a, w.b, rows.rows, x.device
+    n, rank, K = a.shape
+    N = b.shape[1]
+    make = torch.empty if M else torch.zeros
+    dx = torch.empty(M, K, dtype=x.dtype, device=dev) if need[0] else None
+    da = make(n, rank, K, dtype=x.dtype, device=dev) if need[1] else None
+    db = make(n, N, rank, dtype=x.dtype, device=dev) if need[2] else None
+    if M and (need[0] or need[1] or need[2]):
         code, cap = _DTYPE_CODE[x.dtype], rows.tiles.shape[0]
         # taken and given back on the current stream: calls on two streams, or two captured graphs, have their own
-        ws = torch.empty(_grad_workspace(code, rows.rows, w.n, rows.size, cap, K, N, w.rank),
-                         dtype=torch.uint8, device=dev)
+        ws = torch.empty(_grad_workspace(code, M, n, rows.size, cap, K, N, rank), dtype=torch.uint8,
+                         device=dev)
         with on_device(dev):
             rc = lib().rlu_lora_grad(
-                dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), w.a.data_ptr(), w.b.data_ptr(),
+                dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(),
                 w.scale.data_ptr(), code, rows.order.data_ptr(), rows.tiles.data_ptr(),
-                rows.first.data_ptr(), rows.rows, w.n, rows.size, cap, K, N, w.rank, hidden.data_ptr(),
-                *[0 if dx is None else dx.data_ptr(), K], *[0 if t is None else t.data_ptr()
-                                                            for t in (da, db)],
-                ws.data_ptr(), stream_ptr())
+                rows.first.data_ptr(), M, n, rows.size, cap, K, N, rank, hidden.data_ptr(),
+                0 if dx is None else dx.data_ptr(), K, 0 if da is None else da.data_ptr(),
+                0 if db is None else db.data_ptr(), ws.data_ptr(), stream_ptr())
         check(rc, "rlu_lora_grad")
     return dx, da, db
 
@@ -214,7 +223,8 @@ def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRow
     _check_hidden("add_lora_grad", hidden, rows.rows, w)
     if len(need) != 3:
         raise ValueError("add_lora_grad: need says whether dx, da and db are wanted")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (dy, x, w.a, w.b)):
+    if (dy.requires_grad or x.requires_grad or w.a.requires_grad or w.b.requires_grad) and \
+            torch.is_grad_enabled():
         raise ValueError("add_lora_grad returns the gradients itself: detach its operands")
     return _backward(dy, x, w, rows, hidden, need)
 
@@ -222,8 +232,8 @@ def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRow
 class _AddLora(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, a, b, w, rows):
-        hidden = torch.empty((rows.rows, w.rank), dtype=torch.float32, device=x.device)
-        out = torch.empty((rows.rows, y.shape[1]), dtype=y.dtype, device=y.device)
+        hidden = torch.empty(rows.rows, a.shape[1], dtype=torch.float32, device=x.device)
+        out = torch.empty(rows.rows, y.shape[1], dtype=y.dtype, device=y.device)
         _forward(y, x, w, rows, hidden, out)
         ctx.save_for_backward(x, a, b, hidden)
         ctx.w, ctx.rows = w, rows

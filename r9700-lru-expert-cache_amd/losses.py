@@ -40,30 +40,30 @@ def _check_logits(name: str, logits: torch.Tensor) -> None:
     vocab = logits.shape[1]
     if not 1 <= vocab <= MAX_VOCAB:
         raise ValueError(f"{name}: a vocabulary of {vocab} is outside 1..{MAX_VOCAB}")
-    if vocab > 1 and logits.stride(1) != 1:
+    if vocab > 1 and logits.stride()[1] != 1:
         raise ValueError(f"{name}: a row's logits must lie next to each other")
 
 
 def _check_beside(name: str, what: str, t, shape, dtypes, logits) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or not t.is_contiguous() or \
-            t.device != logits.device:
+    if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != logits.device:
         raise ValueError(f"{name}: {what} must be contiguous {' or '.join(str(d)[6:] for d in dtypes)} "
                          f"{list(shape)} beside the logits")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient of {what}: detach it")
 
 
-_F32 = (torch.float32,)
+_F32, _I32, _IDS = (torch.float32,), (torch.int32,), (torch.int64, torch.int32)
 
 
 def _grad_like(logits: torch.Tensor) -> torch.Tensor:
     """A buffer for the gradient whose rows start at the same place within 16 bytes as the logits'."""
     rows, vocab = logits.shape
-    n = 16 // logits.element_size()
-    ld = vocab + ((logits.stride(0) - vocab) % n if rows > 1 else 0)
-    off = logits.data_ptr() // logits.element_size() % n
+    size = logits.element_size()
+    n = 16 // size
+    ld = vocab + ((logits.stride()[0] - vocab) % n if rows > 1 else 0)
+    off = logits.data_ptr() // size % n
     if ld == vocab and off == 0:
-        return torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        return torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
     return torch.empty(off + rows * ld, dtype=logits.dtype, device=logits.device).as_strided(
         (rows, vocab), (ld, 1), off)
 
@@ -96,9 +96,9 @@ def _call(logits, grad, top, fn, before, after) -> torch.Tensor:
     ws = torch.empty(_workspace(code, rows, vocab, top), dtype=torch.uint8, device=dev)
     with on_device(dev):
         rc = getattr(lib(), fn)(
-            logits.data_ptr(), code, logits.stride(0), rows, vocab, *before, loss.data_ptr(), *after,
+            logits.data_ptr(), code, logits.stride()[0], rows, vocab, *before, loss.data_ptr(), *after,
             0 if grad is None else grad.data_ptr(),
-            0 if grad is None else grad.stride(0) if rows > 1 else vocab, ws.data_ptr(), stream_ptr())
+            0 if grad is None else grad.stride()[0] if rows > 1 else vocab, ws.data_ptr(), stream_ptr())
     check(rc, fn)
     return loss
 
@@ -133,11 +133,13 @@ def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, 
                   temperature) -> None:
     _check_logits(name, logits)
     rows = (logits.shape[0],)
-    _check_beside(name, "tokens", tokens, rows, (torch.int64, torch.int32), logits)
-    for what, t in (("old_logprobs", old_logprobs), ("advantages", advantages),
-                    ("ref_logprobs", ref_logprobs), ("weight", weight)):
-        if t is not None:
-            _check_beside(name, what, t, rows, _F32, logits)
+    _check_beside(name, "tokens", tokens, rows, _IDS, logits)
+    _check_beside(name, "old_logprobs", old_logprobs, rows, _F32, logits)
+    _check_beside(name, "advantages", advantages, rows, _F32, logits)
+    if ref_logprobs is not None:
+        _check_beside(name, "ref_logprobs", ref_logprobs, rows, _F32, logits)
+    if weight is not None:
+        _check_beside(name, "weight", weight, rows, _F32, logits)
     if len(clip) != 2 or not 0 <= clip[0] <= 1 or not 0 <= clip[1] < float("inf"):
         raise ValueError(f"{name}: clip={clip}, not (below, above) with 0 <= below <= 1 and above >= 0")
     if not 0 <= kl <= 1e30:
@@ -150,9 +152,9 @@ def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, 
 def _check_distill(name, logits, top_ids, top_logprobs, weight, temperature) -> None:
     _check_logits(name, logits)
     rows = logits.shape[0]
-    if top_ids.ndim != 2 or not 1 <= top_ids.shape[1] <= MAX_TOP:
+    if top_ids.ndim != 2 or top_ids.shape[0] != rows or not 1 <= top_ids.shape[1] <= MAX_TOP:
         raise ValueError(f"{name}: top_ids must be [{rows}, 1..{MAX_TOP}]")
-    _check_beside(name, "top_ids", top_ids, (rows, top_ids.shape[1]), (torch.int32,), logits)
+    _check_beside(name, "top_ids", top_ids, top_ids.shape, _I32, logits)
     _check_beside(name, "top_logprobs", top_logprobs, top_ids.shape, _F32, logits)
     if weight is not None:
         _check_beside(name, "weight", weight, (rows,), _F32, logits)

@@ -119,6 +119,7 @@ SIZES = [  # rows, K, N, R, n
     (1, 2560, 2560, 16, 1), (1, 1, 1, 1, 1), (2, 7, 5, 3, 2), (5, 33, 31, 8, 3), (16, 128, 512, 16, 1),
     (17, 100, 513, 17, 40), (63, 768, 1543, 8, 12), (64, 256, 100, 24, 2), (100, 31, 33, 33, 5),
     (200, 512, 640, 64, 64), (300, 129, 257, 100, 7), (129, 264, 1030, 128, 3), (1023, 136, 72, 16, 1000),
+    (600, 136, 700, 16, 300), (500, 72, 1030, 40, 400), (40, 200, 150000, 24, 3),
     (1024, 136, 72, 16, 1024), (1100, 65, 515, 32, 9), (2050, 128, 130, 128, 1), (3000, 40, 48, 65, 30)]
 
 
