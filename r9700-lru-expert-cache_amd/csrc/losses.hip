@@ -110,6 +110,7 @@ struct Listed {
   int id[MAX_TOP];
   float grad[MAX_TOP];
   float m[MOST_NW], s[MOST_NW];
+  Coef coef;
   uint32_t owns[MOST_NW * WAVE];           // bit j: the thread's vectors hold id[j]
 };
 
@@ -248,8 +249,7 @@ __device__ __forceinline__ Part sum_of(const Args& a, const Row& r, Listed& l, u
   return {top, sum};
 }
 
-// The loss and its coefficients from the unlisted logits' part, by each wave alone; the listed ones'
-// gradients go to LDS, of wave 0.
+// The loss and its coefficients from the unlisted logits' part, by the first wave; the listed ones' gradients go to LDS.
 __device__ __forceinline__ Coef policy(const Args& a, Part u, float x, int row, float weight,
                                        bool bad, Listed& l, bool store) {
   const float inf = __builtin_inff(), nan = __builtin_nanf("");
@@ -315,10 +315,10 @@ __device__ __forceinline__ Coef distill(const Args& a, Part u, float x, float v,
   }
   // an id listed twice has its probabilities' sum and counts once
   float own = q;
-  for (int j = 0; j < a.top; ++j) {
-    const bool same = in && __builtin_amdgcn_readlane(id, j) == id && j != lane;
-    own += same ? lane_f(q, j) : 0.f;
-    first = first && !(same && j < lane);
+  const uint64_t alike = match_any(id, in, 19);        // (MAX_V < 2^19)
+  if (__ballot(alike & (alike - 1))) {
+    first = in && __ffsll((unsigned long long)alike) - 1 == lane;
+    for (int j = 0; j < a.top; ++j) own += alike >> j & 1 && j != lane ? lane_f(q, j) : 0.f;
   }
   const float xm = wave_max(in ? x : -inf), m = fmaxf(u.m, xm);
   bad |= m == inf || __ballot(in && q != q);
@@ -438,9 +438,11 @@ __device__ __forceinline__ Own listed(const Args& a, const Row& r, int row, cons
   o.bad = __ballot(id >= a.V);
   o.skip = o.weight == 0.f || (OP == POLICY && __ballot(id >= 0) == 0);
   o.id = id >= 0 && id < a.V ? (int)id : -1;
+  float v = 0.f;
+  if (OP == DISTILL && lane < top) v = a.vals[(size_t)row * top + lane];
   if (o.id >= 0) {
     o.x = xs ? xs[(size_t)row * top + lane] : load_one<DT>(r.p, o.id);
-    if (OP == DISTILL) o.v = a.vals[(size_t)row * top + lane];
+    if (OP == DISTILL) o.v = v;
   }
   if (tid < MAX_TOP) l.id[tid] = tid < top ? o.id : -1;
   l.owns[tid] = 0;
@@ -453,10 +455,14 @@ __device__ __forceinline__ Own listed(const Args& a, const Row& r, int row, cons
 template <int OP>
 __device__ __forceinline__ Coef coef(const Args& a, Part u, const Own& o, int row, Listed& l,
                                      bool store) {
-  const Coef c = OP == POLICY ? policy(a, u, o.x, row, o.weight, o.bad, l, store)
-                              : distill(a, u, o.x, o.v, o.id, row, o.weight, o.bad, l, store);
+  // (one wave for all: it is a thousand instructions)
+  if (threadIdx.x < WAVE) {
+    const Coef c = OP == POLICY ? policy(a, u, o.x, row, o.weight, o.bad, l, store)
+                                : distill(a, u, o.x, o.v, o.id, row, o.weight, o.bad, l, store);
+    if (threadIdx.x == 0) l.coef = c;
+  }
   __syncthreads();
-  return c;
+  return l.coef;
 }
 
 // A workgroup a row: its sum, its loss and, with GRAD, its gradient.
