@@ -238,6 +238,7 @@ __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& 
                                        ExpandLds<MT, KS, TR, NT>& lds) {
   typedef ExpandLds<MT, KS, TR, NT> L;
   constexpr int STEP = NT;                 // columns: 64 a wave
+  constexpr bool ONCE = ADD && NT == EXPAND_NT;        // (what is more than a few tiles' outputs passes the cache by)
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
   const int r8 = lane / 8, c8 = lane % 8 * 8;
   size_t row[MT][2];
@@ -262,7 +263,7 @@ __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& 
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) yv[i][s] = fetch<WHOLE>(f.y + row[i][s] * f.ldy, c0 + c8, f.cols);
+        for (int s = 0; s < 2; ++s) yv[i][s] = fetch<WHOLE, ONCE>(f.y + row[i][s] * f.ldy, c0 + c8, f.cols);
 #pragma unroll
     for (int i = 0; i < 4 * KS; ++i) {
       const int q = i * WAVE + lane;
@@ -314,7 +315,7 @@ __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& 
           }
           o[e] = to_bits2<DT>(x, y);
         }
-        if (16 * i + 8 * s + r8 < t.count) store8(f.out + row[i][s] * f.ldo + c0 + c8, o, f.cols - c0 - c8);
+        if (16 * i + 8 * s + r8 < t.count) store8<ONCE>(f.out + row[i][s] * f.ldo + c0 + c8, o, f.cols - c0 - c8);
       }
       wave_lds_sync();
     }

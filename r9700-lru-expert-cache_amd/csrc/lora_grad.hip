@@ -62,15 +62,13 @@ struct OuterLds {
 };
 
 template <int DT, int RB, bool WHOLE, bool DB>
-__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd f) {
+__device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<RB, DB>& lds) {
   constexpr int W = 16 * RB, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
-  __shared__ OuterLds<RB, DB> lds;
   const Side o = side_of<DB>(f);
-  const int strips = (o.cols + OUTER - 1) / OUTER, run = (int)blockIdx.x / strips, strip = (int)blockIdx.x % strips;
+  const int strips = (o.cols + OUTER - 1) / OUTER, run = block / strips, strip = block % strips;
   const int total = f.p.first[f.p.n], per = (total + o.runs - 1) / o.runs;
   const int t0 = run * per, t1 = min(t0 + per, total);
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE), col = lane % 16, g = lane / 16;
-  const int r0 = (int)blockIdx.y * W;
   const int c0 = strip * OUTER + w * 64;
   uint16_t* mine = lds.v + w * 32 * 72;
   const int vr = w * 8 + lane / 32, vc = strip * OUTER + lane % 32 * 8;        // of the rows this lane brings
@@ -235,14 +233,20 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd
   }
 }
 
-// Adapters that go over several runs: their parts, in order; those without rows: zeros.
+template <int DT, int RB, bool WHOLE>
+__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd f) {
+  __shared__ OuterLds<RB, true> lds;
+  outer<DT, RB, WHOLE, true>(f, (int)blockIdx.x, (int)blockIdx.y * 16 * RB, lds);
+}
+
+// Adapters that go over several runs: their parts, in order; those without rows: zeros. (zeros alone with only)
 template <int DT, bool DB>
-__device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks) {
+__device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks, bool only) {
   const Side o = side_of<DB>(f);
   const int total = f.p.first[f.p.n], per = (total + o.runs - 1) / o.runs;
   const int first = f.p.first[a], last = f.p.first[a + 1];
   const int s0 = first < last ? first / per : 0, s1 = first < last ? (last - 1) / per : -1;
-  if (s0 == s1) return;
+  if (s0 == s1 || (only && first < last)) return;
   const size_t one = (size_t)f.R * o.cols;
   uint16_t* out = o.out + a * one;
   for (size_t i = (size_t)block * NT + threadIdx.x; i < one; i += (size_t)blocks * NT) {
@@ -254,8 +258,7 @@ __device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks)
 }
 template <int DT>
 __global__ __launch_bounds__(NT) void join_k(Bwd f) {
-  if (blockIdx.z == 0 && f.da) join<DT, false>(f, (int)blockIdx.y, (int)blockIdx.x, (int)gridDim.x);
-  if (blockIdx.z == 1 && f.db) join<DT, true>(f, (int)blockIdx.y, (int)blockIdx.x, (int)gridDim.x);
+  join<DT, false>(f, (int)blockIdx.y, (int)blockIdx.x, (int)gridDim.x, false);
 }
 
 // ---- u over the strips --------------------------------------------------------------------------------------
@@ -281,19 +284,41 @@ __global__ __launch_bounds__(NT) void sum_k(Bwd f) {
   f.u[at] = t.adapter == BAD ? __builtin_nanf("") : v;
 }
 
-// ---- dx = u A ---------------------------------------------------------------------------------------------
-template <int DT, int MT, int KS, bool WHOLE>
-__global__ __launch_bounds__(EXPAND_NT) void dx_k(Bwd f, int strips, int strip) {
-  __shared__ ExpandLds<MT, KS, true> lds;
-  const int tile = (int)(blockIdx.x / (unsigned)strips);
-  if (tile >= f.p.first[f.p.n + 2]) return;
-  const int n0 = (int)(blockIdx.x % (unsigned)strips) * strip;
-  const Tile t = f.p.tiles[tile];
-  const Out o = {f.a, nullptr, 0, f.dx, f.lddx, f.K, f.R};
-  stage<DT, MT, KS, EXPAND_NT>(lds.h, t.count, f.R, [&](int row) {
-    return f.u + (size_t)f.p.order[t.start + row] * f.R;
-  });
-  expand<DT, MT, KS, WHOLE, true, false>(o, f.p, t, n0, min(n0 + strip, f.K), lds);
+// ---- what needs u, and what dB's launch left -------------------------------------------------------------------------
+// dx, a tile and strip a workgroup; dA's strips and runs; dB's parts and both gradients' zeros, `joins` workgroups an
+// adapter: one launch of work that does not wait for one another.
+struct Last {
+  int dx, da, joins;                       // workgroups (joins: of an adapter)
+  int strips, strip;                       // of dx
+};
+template <int DT, int MT, int RB, int KS, bool WHOLE>
+__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void last_k(Bwd f, Last l) {
+  __shared__ union {
+    ExpandLds<MT, KS, true> dx;
+    OuterLds<RB, false> da;
+  } lds;
+  int block = (int)blockIdx.x;
+  if (block < l.dx) {
+    const int tile = block / l.strips, n0 = block % l.strips * l.strip;
+    if (tile >= f.p.first[f.p.n + 2]) return;
+    const Tile t = f.p.tiles[tile];
+    const Out o = {f.a, nullptr, 0, f.dx, f.lddx, f.K, f.R};
+    stage<DT, MT, KS, EXPAND_NT>(lds.dx.h, t.count, f.R, [&](int row) {
+      return f.u + (size_t)f.p.order[t.start + row] * f.R;
+    });
+    expand<DT, MT, KS, WHOLE, true, false>(o, f.p, t, n0, min(n0 + l.strip, f.K), lds.dx);
+    return;
+  }
+  block -= l.dx;
+  if (block < l.da) {
+    const int pass = l.da / (KS == 4 ? 2 : 1);
+    outer<DT, RB, WHOLE, false>(f, block % pass, block / pass * 16 * RB, lds.da);
+    return;
+  }
+  block -= l.da;
+  const int a = block / l.joins;
+  if (f.db) join<DT, true>(f, a, block % l.joins, l.joins, false);
+  if (f.da) join<DT, false>(f, a, block % l.joins, l.joins, true);
 }
 
 // Runs: workgroups for every CU, twice over, of 128 rows at least.
@@ -320,48 +345,40 @@ static void layout(Bwd& f, long long* bytes) {
 }
 
 template <int DT, bool WHOLE>
-static void backward(const Bwd& f, hipStream_t stream) {
+static void backward(const Bwd& f, const Last& l, hipStream_t stream) {
   const unsigned cap = (unsigned)f.p.cap;
-  const int ba = (f.K + OUTER - 1) / OUTER * f.sa, bb = (f.N + OUTER - 1) / OUTER * f.sb;
-#define RLU_OUTER(RB, DB, Y)                                                                      \
-  hipLaunchKernelGGL((outer_k<DT, RB, WHOLE, DB>), dim3(DB ? bb : ba, Y), dim3(NT), 0, stream, f)
-#define RLU_SIDE(DB)                          \
-  do {                                        \
-    if (f.R <= 16) RLU_OUTER(1, DB, 1);       \
-    else if (f.R <= 32) RLU_OUTER(2, DB, 1);  \
-    else RLU_OUTER(4, DB, f.R <= 64 ? 1 : 2); \
-  } while (0)
-  RLU_SIDE(true);
+  const int bb = (f.N + OUTER - 1) / OUTER * f.sb;
+#define RLU_OUTER(RB, Y) hipLaunchKernelGGL((outer_k<DT, RB, WHOLE>), dim3(bb, Y), dim3(NT), 0, stream, f)
+  if (f.R <= 16) RLU_OUTER(1, 1);
+  else if (f.R <= 32) RLU_OUTER(2, 1);
+  else RLU_OUTER(4, f.R <= 64 ? 1 : 2);
+#undef RLU_OUTER
   if (f.dx || f.da)
     hipLaunchKernelGGL(sum_k, dim3(cap, (f.size * f.R + 31) / 32), dim3(NT), 0, stream, f);
-  if (f.dx) {
-    const int strip = strip_of(f.p.cap, f.size, f.K), strips = (f.K + strip - 1) / strip;
-#define RLU_DX(MT, KS)                                                                               \
-  hipLaunchKernelGGL((dx_k<DT, MT, KS, WHOLE>), dim3(cap * strips), dim3(EXPAND_NT), 0, stream, f, strips, strip)
-#define RLU_DX_OF(MT)                   \
-  do {                                  \
-    if (f.R <= 32) RLU_DX(MT, 1);       \
-    else if (f.R <= 64) RLU_DX(MT, 2);  \
-    else RLU_DX(MT, 4);                 \
+  const dim3 all((unsigned)(l.dx + l.da + l.joins * f.p.n));
+#define RLU_LAST(MT, RB, KS) \
+  hipLaunchKernelGGL((last_k<DT, MT, RB, KS, WHOLE>), all, dim3(NT), 0, stream, f, l)
+#define RLU_LAST_OF(MT)                    \
+  do {                                     \
+    if (f.R <= 16) RLU_LAST(MT, 1, 1);     \
+    else if (f.R <= 32) RLU_LAST(MT, 2, 1); \
+    else if (f.R <= 64) RLU_LAST(MT, 4, 2); \
+    else RLU_LAST(MT, 4, 4);               \
   } while (0)
-    if (f.size == 16) RLU_DX_OF(1);
-    else RLU_DX_OF(4);
-#undef RLU_DX_OF
-#undef RLU_DX
+  if (f.size == 16) RLU_LAST_OF(1);
+  else RLU_LAST_OF(4);
+#undef RLU_LAST_OF
+#undef RLU_LAST
+  if (f.da && f.sa > 1) {
+    const long long per = ((long long)f.R * f.K + NT * 4 - 1) / (NT * 4);
+    hipLaunchKernelGGL((join_k<DT>), dim3(per < 512 ? per : 512, f.p.n), dim3(NT), 0, stream, f);
   }
-  if (f.da) RLU_SIDE(false);
-#undef RLU_SIDE
-#undef RLU_OUTER
-  if (!f.da && !f.db) return;
-  const long long one = (long long)f.R * (f.N > f.K ? f.N : f.K);
-  const int per = (int)((one + NT * 4 - 1) / (NT * 4));
-  hipLaunchKernelGGL((join_k<DT>), dim3(per < 512 ? per : 512, f.p.n, 2), dim3(NT), 0, stream, f);
 }
 
 }  // namespace lora
 }  // namespace rlu
 
-static int grad_sizes(rlu::lora::Bwd& f, int dtype, int rows, int n, int size, int cap, int K, int N, int R,
+static int grad_sizes(rlu::lora::Bwd& f, rlu::lora::Last& l, int dtype, int rows, int n, int size, int cap, int K, int N, int R,
                       long long* bytes) {
   using namespace rlu::lora;
   if (!sizes_ok(dtype, rows, n, size, cap, K, N, R)) return -1;
@@ -373,9 +390,14 @@ static int grad_sizes(rlu::lora::Bwd& f, int dtype, int rows, int n, int size, i
   f.N = N;
   f.R = R;
   layout(f, bytes);
-  const long long blocks = 2ll * ((N + OUTER - 1) / OUTER) * f.sb, more = 2ll * ((K + OUTER - 1) / OUTER) * f.sa;
-  if (blocks > UINT32_MAX / NT || more > UINT32_MAX / NT || 4ll * cap * R * (size / 16) > UINT32_MAX / NT ||
-      cap * ((K + 255ll) / 256) > UINT32_MAX / EXPAND_NT)
+  const int strip = strip_of(cap, size, K);
+  const long long strips = (K + strip - 1) / strip, most = (long long)R * (N > K ? N : K);
+  const long long joins = (most + NT * 4 - 1) / (NT * 4);
+  const long long blocks = 2ll * ((N + OUTER - 1) / OUTER) * f.sb, dx = cap * strips,
+                  da = ((K + OUTER - 1) / OUTER) * (R > 64 ? 2ll : 1ll) * f.sa;
+  l = {(int)dx, (int)da, (int)(joins < 512 ? joins : 512), (int)strips, strip};
+  if (blocks > UINT32_MAX / NT || dx + da + (long long)l.joins * n > UINT32_MAX / NT ||
+      4ll * cap * R * (size / 16) > UINT32_MAX / NT)
     return -1;                                         // (a launch counts its threads in 32 bits)
   return 0;
 }
@@ -383,7 +405,8 @@ static int grad_sizes(rlu::lora::Bwd& f, int dtype, int rows, int n, int size, i
 extern "C" int rlu_lora_grad_workspace(int dtype, int rows, int n, int size, int cap, int K, int N, int R,
                                        long long* bytes) {
   rlu::lora::Bwd f = {};
-  return bytes ? grad_sizes(f, dtype, rows, n, size, cap, K, N, R, bytes) : -1;
+  rlu::lora::Last l;
+  return bytes ? grad_sizes(f, l, dtype, rows, n, size, cap, K, N, R, bytes) : -1;
 }
 
 extern "C" int rlu_lora_grad(const void* dy, long long lddy, const void* x, long long ldx, const void* a,
@@ -395,7 +418,8 @@ extern "C" int rlu_lora_grad(const void* dy, long long lddy, const void* x, long
   Bwd f = {};
   f.upart = (float*)ws;
   long long bytes;
-  if (grad_sizes(f, dtype, rows, n, size, cap, K, N, R, &bytes) || lddy < 0 || ldx < 0 ||
+  Last l;
+  if (grad_sizes(f, l, dtype, rows, n, size, cap, K, N, R, &bytes) || lddy < 0 || ldx < 0 ||
       lddy > INT32_MAX || ldx > INT32_MAX)
     return -1;
   if (rows == 0) return 0;
@@ -421,10 +445,12 @@ extern "C" int rlu_lora_grad(const void* dy, long long lddy, const void* x, long
   f.lddx = lddx;
   f.da = (uint16_t*)da;
   f.db = (uint16_t*)db;
+  if (!dx) l.dx = 0;
+  if (!da) l.da = 0;
   const bool whole = (K | N | R) % 8 == 0;
-  if (dtype == 0 && whole) backward<0, true>(f, stream);
-  else if (dtype == 0) backward<0, false>(f, stream);
-  else if (whole) backward<2, true>(f, stream);
-  else backward<2, false>(f, stream);
+  if (dtype == 0 && whole) backward<0, true>(f, l, stream);
+  else if (dtype == 0) backward<0, false>(f, l, stream);
+  else if (whole) backward<2, true>(f, l, stream);
+  else backward<2, false>(f, l, stream);
   return (int)hipGetLastError();
 }
