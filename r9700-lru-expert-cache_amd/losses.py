@@ -44,8 +44,8 @@ def _check_logits(name: str, logits: torch.Tensor) -> None:
         raise ValueError(f"{name}: a row's logits must lie next to each other")
 
 
-def _check_beside(name: str, what: str, t, shape, dtypes, logits) -> None:
-    if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != logits.device:
+def _check_beside(name: str, what: str, t, shape, dtypes, dev) -> None:
+    if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{name}: {what} must be contiguous {' or '.join(str(d)[6:] for d in dtypes)} "
                          f"{list(shape)} beside the logits")
     if t.requires_grad and torch.is_grad_enabled():
@@ -132,14 +132,14 @@ def _check_temperature(name: str, temperature) -> None:
 def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
                   temperature) -> None:
     _check_logits(name, logits)
-    rows = (logits.shape[0],)
-    _check_beside(name, "tokens", tokens, rows, _IDS, logits)
-    _check_beside(name, "old_logprobs", old_logprobs, rows, _F32, logits)
-    _check_beside(name, "advantages", advantages, rows, _F32, logits)
+    rows, dev = (logits.shape[0],), logits.device
+    _check_beside(name, "tokens", tokens, rows, _IDS, dev)
+    _check_beside(name, "old_logprobs", old_logprobs, rows, _F32, dev)
+    _check_beside(name, "advantages", advantages, rows, _F32, dev)
     if ref_logprobs is not None:
-        _check_beside(name, "ref_logprobs", ref_logprobs, rows, _F32, logits)
+        _check_beside(name, "ref_logprobs", ref_logprobs, rows, _F32, dev)
     if weight is not None:
-        _check_beside(name, "weight", weight, rows, _F32, logits)
+        _check_beside(name, "weight", weight, rows, _F32, dev)
     if len(clip) != 2 or not 0 <= clip[0] <= 1 or not 0 <= clip[1] < float("inf"):
         raise ValueError(f"{name}: clip={clip}, not (below, above) with 0 <= below <= 1 and above >= 0")
     if not 0 <= kl <= 1e30:
@@ -151,13 +151,13 @@ def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, 
 
 def _check_distill(name, logits, top_ids, top_logprobs, weight, temperature) -> None:
     _check_logits(name, logits)
-    rows = logits.shape[0]
+    rows, dev = logits.shape[0], logits.device
     if top_ids.ndim != 2 or top_ids.shape[0] != rows or not 1 <= top_ids.shape[1] <= MAX_TOP:
         raise ValueError(f"{name}: top_ids must be [{rows}, 1..{MAX_TOP}]")
-    _check_beside(name, "top_ids", top_ids, top_ids.shape, _I32, logits)
-    _check_beside(name, "top_logprobs", top_logprobs, top_ids.shape, _F32, logits)
+    _check_beside(name, "top_ids", top_ids, top_ids.shape, _I32, dev)
+    _check_beside(name, "top_logprobs", top_logprobs, top_ids.shape, _F32, dev)
     if weight is not None:
-        _check_beside(name, "weight", weight, (rows,), _F32, logits)
+        _check_beside(name, "weight", weight, (rows,), _F32, dev)
     _check_temperature(name, temperature)
 
 
