@@ -396,7 +396,7 @@ int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* 
  * operand lies at any element's address, its rows ld elements apart.
  * rlu_lora_plan: a batch's rows by adapter, once for all its projections. ids [rows] int64 (wide 1) or int32: below
  *   0 none, n or more: the row becomes NaN. size: rows of a tile, 16 or 64. cap = rows / size + min(rows, n + 2).
- *   order [rows], tiles [cap][4] (16-byte aligned), first [n + 3]: for the calls below, which trust them.
+ *   order [rows], tiles [cap][4] (16-byte aligned), first [n + 5]: for the calls below, which trust them.
  * rlu_lora_add: hidden [rows][R] f32 = scale x a^T (0 in rows without an adapter), out [rows][N] = y + hidden b^T
  *   (y in those), with two launches. out may be y (same address and ld), but overlaps nothing else.
  * rlu_lora_grad: from dy [rows][N] and hidden as rlu_lora_add left it, with u = scale dy b: dx [rows][K] = u a (0 in

@@ -27,7 +27,8 @@ constexpr int NONE = -1, BAD = -2;
 struct Plan {
   const int* order;
   const Tile* tiles;
-  const int* first;                        // [n + 3]: an adapter's first tile; NONE's, BAD's, and their number
+  const int* first;                        // [n + 5]: an adapter's first tile; NONE's, BAD's, their number; adapters
+                                           // with rows, and the rows that have one
   int n, rows, cap;                        // cap: tiles that there are at most
 };
 

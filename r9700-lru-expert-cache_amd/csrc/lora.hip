@@ -45,7 +45,7 @@ __global__ __launch_bounds__(PLAN_NT) void plan_k(const void* __restrict__ ids, 
   }
   __syncthreads();
   if (w == 0) {                            // totals to starts, rows and tiles
-    int at = 0, tile = 0;
+    int at = 0, tile = 0, live = 0;
     for (int g0 = 0; g0 < groups; g0 += WAVE) {
       const int g = g0 + lane, c = g < groups ? start[g] : 0, t = (c + size - 1) / size;
       const int sc = wave_incl_scan(c), st = wave_incl_scan(t);
@@ -54,11 +54,14 @@ __global__ __launch_bounds__(PLAN_NT) void plan_k(const void* __restrict__ ids, 
         tile0[g] = tile + st - t;
         first[g] = tile + st - t;
       }
+      live += (int)__popcll(__ballot(c > 0 && g < n));
       at += readlane(sc, WAVE - 1);
       tile += readlane(st, WAVE - 1);
     }
     if (lane == 0) {
       first[groups] = tile;
+      first[groups + 1] = live;
+      first[groups + 2] = start[n];
       tile0[groups] = tile;
     }
   }

@@ -52,12 +52,20 @@ __device__ __forceinline__ Side side_of(const Bwd& f) {
             : Side{f.x, f.ldx, f.K, f.sa, f.u, f.da, f.pa};
 }
 
+// Tiles of a run: as many runs as there is work for, adapters of their own or 128 rows.
+__device__ __forceinline__ int tiles_a_run(const Plan& p, int runs) {
+  const int total = p.first[p.n], live = p.first[p.n + 3], rows = p.first[p.n + 4];
+  const int use = max(1, min(runs, max(live, rows / 128)));
+  return max(1, (total + use - 1) / use);
+}
+
 template <int RB, bool DB>
 struct OuterLds {
   static constexpr int W = 16 * RB;
   alignas(16) uint16_t v[NW * 32 * 72];    // the step's rows [32][VLD]; before them each wave's part of B
   alignas(16) uint16_t h[2][W * 40];       // both parts of h or u, [rank][row]
   float u[DB ? NW : 1][DB ? 32 * W : 1];
+  int row[2][DB ? 32 : 1];                 // where the rows of this step and of the one before lie
   float top[NW];
 };
 
@@ -66,7 +74,7 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
   constexpr int W = 16 * RB, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
   const Side o = side_of<DB>(f);
   const int strips = (o.cols + OUTER - 1) / OUTER, run = block / strips, strip = block % strips;
-  const int total = f.p.first[f.p.n], per = (total + o.runs - 1) / o.runs;
+  const int total = f.p.first[f.p.n], per = tiles_a_run(f.p, o.runs);
   const int t0 = run * per, t1 = min(t0 + per, total);
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE), col = lane % 16, g = lane / 16;
   const int c0 = strip * OUTER + w * 64;
@@ -111,19 +119,18 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
       for (int i = 0; i < EACH; ++i) n.h[i] = f.p.order[min(pos + (tid + i * NT) / W, p1 - 1)];
       return n;
     };
-    int hrow[EACH], hcol[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) hcol[i] = min(r0 + (tid + i * NT) % W, f.R - 1);
+    const int hcol = min(r0 + tid % W, f.R - 1);       // (NT is a multiple of W)
+    int vrow[4], odd = 0;
     v4u vv[4];
     float hv[EACH];
     auto load = [&](const Places& at) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vv[i] = fetch<WHOLE, true>(o.v + (uint64_t)(uint32_t)at.v[i] * (uint32_t)o.ld, vc, o.cols);
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        hrow[i] = at.h[i];
-        hv[i] = o.h[(uint32_t)at.h[i] * (uint32_t)f.R + hcol[i]];
+      for (int i = 0; i < 4; ++i) {
+        vrow[i] = at.v[i];
+        vv[i] = fetch<WHOLE, true>(o.v + (uint64_t)(uint32_t)at.v[i] * (uint32_t)o.ld, vc, o.cols);
       }
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) hv[i] = o.h[(uint32_t)at.h[i] * (uint32_t)f.R + hcol];
     };
     Places at = places(p0);
     {
@@ -132,7 +139,6 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
       at = next;
     }
     for (int pos = p0; pos < p1; pos += 32) {
-      int urow[EACH];
       float by = 1.f;
       if (DT != 0) {                       // float16: h and u into its range by a power of two a step
         float m = 0.f;
@@ -157,43 +163,41 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
         const Split<DT> p(in ? hv[i] * by : 0.f);
         lds.h[0][q % W * 40 + q / W] = (uint16_t)p.hi;
         lds.h[1][q % W * 40 + q / W] = (uint16_t)p.lo;
-        urow[i] = hrow[i];
+      }
+      if (DB && lane % 32 == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds.row[odd][vr + 2 * i] = vrow[i];
       }
       lds_barrier();
       const Places next = places(pos + 64);
       load(at);
       at = next;
-      if (DB) {
-        v4f u[2][RB] = {};
+      if (DB)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int i = 0; i < 2; ++i) {
+          v4f u[RB] = {};
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int k = 0; k < 2; ++k) {
             const v4u vf = frag<VLD>(lds.v, 16 * i, w * 64 + 32 * k);
 #pragma unroll
-            for (int j = 0; j < RB; ++j) u[i][j] = mfma<DT>(vf, bu[k][j], u[i][j]);
+            for (int j = 0; j < RB; ++j) u[j] = mfma<DT>(vf, bu[k][j], u[j]);
           }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < RB; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) lds.u[w][(16 * i + 4 * g + e) * W + 16 * j + col] = u[i][j][e];
-      }
-      v4u hi[RB], lo[RB];
+            for (int e = 0; e < 4; ++e) lds.u[w][(16 * i + 4 * g + e) * W + 16 * j + col] = u[j][e];
+        }
+      v4u vf[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) vf[c] = frag_tr<VLD>(lds.v, 0, w * 64 + 16 * c);
 #pragma unroll
       for (int j = 0; j < RB; ++j) {
-        hi[j] = frag<40>(lds.h[0], 16 * j, 0);
-        lo[j] = frag<40>(lds.h[1], 16 * j, 0);
-      }
+        const v4u hi = frag<40>(lds.h[0], 16 * j, 0), lo = frag<40>(lds.h[1], 16 * j, 0);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const v4u vf = frag_tr<VLD>(lds.v, 0, w * 64 + 16 * c);
-#pragma unroll
-        for (int j = 0; j < RB; ++j) {
+        for (int c = 0; c < 4; ++c) {
           v4f t = DT != 0 ? v4f{} : acc[j][c];
-          t = DB ? mfma<DT>(vf, lo[j], t) : mfma<DT>(lo[j], vf, t);
-          t = DB ? mfma<DT>(vf, hi[j], t) : mfma<DT>(hi[j], vf, t);
+          t = DB ? mfma<DT>(vf[c], lo, t) : mfma<DT>(lo, vf[c], t);
+          t = DB ? mfma<DT>(vf[c], hi, t) : mfma<DT>(hi, vf[c], t);
           if (DT == 0) acc[j][c] = t;
           else
 #pragma unroll
@@ -208,33 +212,55 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
           // it. What lies past the last row or rank goes to a row that nobody reads.)
           const int q = tid + i * NT;
           const bool in = q / W < p1 - pos && q % W < f.R - r0;
-          upart[in ? (uint32_t)urow[i] * (uint32_t)f.R + hcol[i] : spare + lane] =
+          upart[in ? (uint32_t)lds.row[odd][q / W] * (uint32_t)f.R + hcol : spare + lane] =
               s * ((lds.u[0][q] + lds.u[1][q]) + (lds.u[2][q] + lds.u[3][q]));
         }
       }
+      odd ^= 1;
     }
-    if (!o.out) continue;
+    // 16 ranks at a time through the wave's part of LDS, then eight of the gradient's consecutive elements a lane
     const bool whole = first >= t0 && last <= t1;
     const size_t one = (size_t)f.R * o.cols;
     uint16_t* out = o.out + a * one;
     float* part = o.parts + ((size_t)run * 2 + (first >= t0)) * one;
+    float* t = (float*)mine;
 #pragma unroll
-    for (int j = 0; j < RB; ++j)
+    for (int j = 0; j < RB; ++j) {
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = r0 + 16 * j + (DB ? col : 4 * g + e), cc = c0 + 16 * c + (DB ? 4 * g + e : col);
-          if (r >= f.R || cc >= o.cols) continue;
-          const size_t at = DB ? (size_t)cc * f.R + r : (size_t)r * o.cols + cc;
-          if (whole) out[at] = (uint16_t)to_bits<DT>(acc[j][c][e]);
-          else part[at] = acc[j][c][e];
+        for (int e = 0; e < 4; ++e)
+          t[DB ? (16 * c + 4 * g + e) * 16 + col : (4 * g + e) * 68 + 16 * c + col] = acc[j][c][e];
+      wave_lds_sync();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = i * WAVE + lane, r = r0 + 16 * j + (DB ? q % 2 * 8 : q / 8), cc = c0 + (DB ? q / 2 : q % 8 * 8);
+        const v4f x = *(const v4f*)&t[DB ? q * 8 : q / 8 * 68 + q % 8 * 8];
+        const v4f y = *(const v4f*)&t[DB ? q * 8 + 4 : q / 8 * 68 + q % 8 * 8 + 4];
+        if (r >= f.R || cc >= o.cols || !o.out) continue;
+        const size_t at = DB ? (size_t)cc * f.R + r : (size_t)r * o.cols + cc;
+        const int n = DB ? f.R - r : o.cols - cc;
+        if (whole) {
+          const v4u v = {to_bits2<DT>(x[0], x[1]), to_bits2<DT>(x[2], x[3]), to_bits2<DT>(y[0], y[1]),
+                         to_bits2<DT>(y[2], y[3])};
+          store8(out + at, v, n);
+        } else if (n >= 8) {
+          *(v4fa*)(part + at) = x;
+          *(v4fa*)(part + at + 4) = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 7; ++e)
+            if (e < n) part[at + e] = e < 4 ? x[e] : y[e - 4];
         }
+      }
+      wave_lds_sync();
+    }
+    lds_barrier();                         // (the next adapter's rows come to the same place)
   }
 }
 
 template <int DT, int RB, bool WHOLE>
-__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd f) {
+__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 4 && DT != 0 ? 1 : 2) void outer_k(Bwd f) {
   __shared__ OuterLds<RB, true> lds;
   outer<DT, RB, WHOLE, true>(f, (int)blockIdx.x, (int)blockIdx.y * 16 * RB, lds);
 }
@@ -243,7 +269,7 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void outer_k(Bwd
 template <int DT, bool DB>
 __device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks, bool only) {
   const Side o = side_of<DB>(f);
-  const int total = f.p.first[f.p.n], per = (total + o.runs - 1) / o.runs;
+  const int per = tiles_a_run(f.p, o.runs);
   const int first = f.p.first[a], last = f.p.first[a + 1];
   const int s0 = first < last ? first / per : 0, s1 = first < last ? (last - 1) / per : -1;
   if (s0 == s1 || (only && first < last)) return;
@@ -292,7 +318,7 @@ struct Last {
   int strips, strip;                       // of dx
 };
 template <int DT, int MT, int RB, int KS, bool WHOLE>
-__global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void last_k(Bwd f, Last l) {
+__global__ __launch_bounds__(NT, RB == 1 ? 3 : 2) void last_k(Bwd f, Last l) {
   __shared__ union {
     ExpandLds<MT, KS, true> dx;
     OuterLds<RB, false> da;
@@ -321,15 +347,15 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 2 ? 2 : 1) void last_k(Bwd 
   if (f.da) join<DT, false>(f, a, block % l.joins, l.joins, true);
 }
 
-// Runs: workgroups for every CU, twice over, of 128 rows at least.
-static int runs_of(int strips, int rows) {
-  const int want = (512 + strips - 1) / strips, most = rows / 128;
+// Runs, at most: workgroups for every CU, twice over; see tiles_a_run.
+static int runs_of(int strips, int rows, int n) {
+  const int want = (512 + strips - 1) / strips, most = rows / 128 > n ? rows / 128 : rows < n ? rows : n;
   return want < most ? want : most > 1 ? most : 1;
 }
 static void layout(Bwd& f, long long* bytes) {
   const int strips = (f.N + OUTER - 1) / OUTER;
-  f.sa = runs_of((f.K + OUTER - 1) / OUTER, f.p.rows);
-  f.sb = runs_of(strips, f.p.rows);
+  f.sa = runs_of((f.K + OUTER - 1) / OUTER, f.p.rows, f.p.n);
+  f.sb = runs_of(strips, f.p.rows, f.p.n);
   long long at = 0;
   auto take = [&](long long n) {
     const long long was = at;

@@ -62,7 +62,7 @@ class LoraRows:
     """A batch's rows by adapter, as the kernels read them (plan_rows makes it)."""
     order: torch.Tensor    # int32 [rows]: the rows of adapter 0, of adapter 1, ...; without one; ids past the last
     tiles: torch.Tensor    # int32 [cap, 4]
-    first: torch.Tensor    # int32 [n + 3]
+    first: torch.Tensor    # int32 [n + 5]
     rows: int
     n: int                 # adapters that the ids count
     size: int              # rows of a tile
@@ -84,7 +84,7 @@ def plan_rows(ids: torch.Tensor, n: int) -> LoraRows:
     cap = rows // size + min(rows, n + 2)
     order = torch.empty(rows, dtype=torch.int32, device=dev)
     tiles = torch.empty(cap, 4, dtype=torch.int32, device=dev)
-    first = torch.empty(n + 3, dtype=torch.int32, device=dev)
+    first = torch.empty(n + 5, dtype=torch.int32, device=dev)
     with on_device(dev):
         rc = lib().rlu_lora_plan(ids.data_ptr(), int(ids.dtype == torch.int64), rows, n, size, cap,
                                  order.data_ptr(), tiles.data_ptr(), first.data_ptr(), stream_ptr())

@@ -162,7 +162,8 @@ def test_plan(lora, rows, n, ids64):
         count = torch.bincount(key, minlength=n + 2)
         tiles = (count + p.size - 1) // p.size
         first = torch.cat([torch.zeros(1, dtype=tiles.dtype), tiles.cumsum(0)])
-        assert torch.equal(p.first.cpu().long(), first) and first[-1] <= p.tiles.shape[0]
+        live = (count[:n] > 0).sum().view(1)
+        assert torch.equal(p.first.cpu().long(), torch.cat([first, live, count[:n].sum().view(1)])) and first[-1] <= p.tiles.shape[0]
         start, want = 0, []
         for k in range(n + 2):
             for at in range(0, int(count[k]), p.size):
@@ -346,13 +347,13 @@ def test_gradients(lora, dtype, rows, K, N, R, n, pad, offset):
 
 
 @pytest.mark.parametrize("rows,n,ids", [
-    (2000, 3, "one"), (2000, 70, "few"), (1500, 2, "none"), (90, 5, "runs"), (5000, 6, "runs"), (700, 1024, "few"),
+    (2000, 3, "one"), (2000, 70, "few"), (64, 64, "each"), (300, 64, "each"), (1500, 2, "none"), (90, 5, "runs"), (5000, 6, "runs"), (700, 1024, "few"),
     (129, 2, "one")])
 def test_gradients_of_uneven_batches(lora, rows, n, ids):
     """One adapter with every row, over many runs of tiles; most without any; no row with one; ids in runs."""
     g = torch.Generator(DEV).manual_seed(rows)
     of = {"one": torch.full((rows,), n - 1, device=DEV), "none": torch.full((rows,), -1, device=DEV),
-          "few": torch.randint(3, (rows,), generator=g, device=DEV) * (n // 3),
+          "each": torch.arange(rows, device=DEV) % n, "few": torch.randint(3, (rows,), generator=g, device=DEV) * (n // 3),
           "runs": torch.randint(-1, n, (rows,), generator=g, device=DEV).sort().values}[ids].int()
     for K, N, R in ((200, 264, 16), (72, 40, 40)):
         c = Case(lora, rows, K, N, R, n, "bf16", ids=of)

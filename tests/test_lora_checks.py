@@ -38,7 +38,7 @@ def stack(lora, e, n=3, R=8, K=32, N=40, dtype=BF):
 
 
 def planned(lora, e, rows=5, n=3):
-    return lora.LoraRows(e(rows, dtype=I32), e(rows, 4, dtype=I32), e(n + 3, dtype=I32), rows, n, 16)
+    return lora.LoraRows(e(rows, dtype=I32), e(rows, 4, dtype=I32), e(n + 5, dtype=I32), rows, n, 16)
 
 
 @pytest.mark.parametrize("bad", [
