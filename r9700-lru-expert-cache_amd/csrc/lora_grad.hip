@@ -316,6 +316,7 @@ __global__ __launch_bounds__(NT) void sum_k(Bwd f) {
 struct Last {
   int dx, da, joins;                       // workgroups (joins: of an adapter)
   int strips, strip;                       // of dx
+  int passes;                              // of dA, 64 ranks each
 };
 template <int DT, int MT, int RB, int KS, bool WHOLE>
 __global__ __launch_bounds__(NT, RB == 1 ? 3 : 2) void last_k(Bwd f, Last l) {
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : 2) void last_k(Bwd f, Last l) {
   }
   block -= l.dx;
   if (block < l.da) {
-    const int pass = l.da / (KS == 4 ? 2 : 1);
+    const int pass = l.da / l.passes;
     outer<DT, RB, WHOLE, false>(f, block % pass, block / pass * 16 * RB, lds.da);
     return;
   }
@@ -381,15 +382,23 @@ static void backward(const Bwd& f, const Last& l, hipStream_t stream) {
 #undef RLU_OUTER
   if (f.dx || f.da)
     hipLaunchKernelGGL(sum_k, dim3(cap, (f.size * f.R + 31) / 32), dim3(NT), 0, stream, f);
-  const dim3 all((unsigned)(l.dx + l.da + l.joins * f.p.n));
-#define RLU_LAST(MT, RB, KS) \
-  hipLaunchKernelGGL((last_k<DT, MT, RB, KS, WHOLE>), all, dim3(NT), 0, stream, f, l)
-#define RLU_LAST_OF(MT)                    \
-  do {                                     \
-    if (f.R <= 16) RLU_LAST(MT, 1, 1);     \
-    else if (f.R <= 32) RLU_LAST(MT, 2, 1); \
-    else if (f.R <= 64) RLU_LAST(MT, 4, 2); \
-    else RLU_LAST(MT, 4, 4);               \
+  const auto blocks = [&](const Last& l) { return dim3((unsigned)(l.dx + l.da + l.joins * f.p.n)); };
+#define RLU_LAST(MT, RB, KS, L) \
+  hipLaunchKernelGGL((last_k<DT, MT, RB, KS, WHOLE>), blocks(L), dim3(NT), 0, stream, f, L)
+#define RLU_LAST_OF(MT)                                                                         \
+  do {                                                                                          \
+    if (f.R <= 16) {                                                                            \
+      RLU_LAST(MT, 1, 1, l);                                                                    \
+    } else if (f.R <= 32) {                                                                     \
+      RLU_LAST(MT, 2, 1, l);                                                                    \
+    } else if (f.R <= 64) {                                                                     \
+      RLU_LAST(MT, 4, 2, l);                                                                    \
+    } else { /* (dx's 108 KB of LDS would leave dA one workgroup a CU: 531 us, 450 apart) */        \
+      Last dx = l, rest = l;                                                                    \
+      dx.da = dx.joins = rest.dx = 0;                                                           \
+      if (dx.dx) RLU_LAST(MT, 4, 4, dx);                                                        \
+      RLU_LAST(MT, 4, 2, rest);                                                                 \
+    }                                                                                           \
   } while (0)
   if (f.size == 16) RLU_LAST_OF(1);
   else RLU_LAST_OF(4);
@@ -418,10 +427,13 @@ static int grad_sizes(rlu::lora::Bwd& f, rlu::lora::Last& l, int dtype, int rows
   layout(f, bytes);
   const int strip = strip_of(cap, size, K);
   const long long strips = (K + strip - 1) / strip, most = (long long)R * (N > K ? N : K);
+  // Workgroups for an adapter's parts: those of an adapter without any end at once, and of 64 adapters with 512 each that
+  // took 50 us; with 32 each, one that has all of 8192 rows at R = 64 took 90 us more than with 128.
+  const long long each = 8192 / n > 1 ? (8192 / n < 512 ? 8192 / n : 512) : 1;
   const long long joins = (most + NT * 4 - 1) / (NT * 4);
   const long long blocks = 2ll * ((N + OUTER - 1) / OUTER) * f.sb, dx = cap * strips,
                   da = ((K + OUTER - 1) / OUTER) * (R > 64 ? 2ll : 1ll) * f.sa;
-  l = {(int)dx, (int)da, (int)(joins < 512 ? joins : 512), (int)strips, strip};
+  l = {(int)dx, (int)da, (int)(joins < each ? joins : each), (int)strips, strip, R > 64 ? 2 : 1};
   if (blocks > UINT32_MAX / NT || dx + da + (long long)l.joins * n > UINT32_MAX / NT ||
       4ll * cap * R * (size / 16) > UINT32_MAX / NT)
     return -1;                                         // (a launch counts its threads in 32 bits)

@@ -387,6 +387,22 @@ def test_gradients_asked_for_one_by_one(lora):
                 assert torch.equal(t, u) if n else t is None
 
 
+@pytest.mark.parametrize("R", [65, 128])
+@pytest.mark.parametrize("rows,n", [(70, 40), (1100, 3)])
+def test_gradients_of_high_ranks_one_by_one(lora, rows, n, R):
+    """Over 64 ranks, where dx has a launch of its own."""
+    c = Case(lora, rows, 264, 520, R, n, "bf16")
+    gpu_case(f"lora grad need rows={rows} R={R}")
+    want = both(lora, c)
+    torch.cuda.synchronize()
+    c.check_grad(*want)
+    for need in ((True, False, False), (False, True, False), (False, False, True)):
+        got = both(lora, c, need)
+        torch.cuda.synchronize()
+        for t, u, n in zip(got, want, need):
+            assert torch.equal(t, u) if n else t is None
+
+
 @pytest.mark.parametrize("rows", [45, 1300])
 def test_gradients_of_ids_past_the_last_and_nan(lora, rows):
     """A bad row has no part in the adapters' gradients; a NaN in a row goes to that row and to its adapter alone;
