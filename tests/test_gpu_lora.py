@@ -365,6 +365,19 @@ def test_gradients_of_uneven_batches(lora, rows, n, ids):
         assert (got[1][empty] == 0).all() and (got[2][empty] == 0).all()
 
 
+@pytest.mark.parametrize("counts", [
+    [10, 600, 200, 1, 0, 7], [0, 256, 257, 16, 17, 300], [10, 900, 250, 1, 0, 300, 256, 257, 64, 65], [1200, 0, 1, 700, 192, 193]])
+def test_gradients_of_small_beside_large_adapters(lora, counts):
+    """Adapters on both sides of the rows that one workgroup takes alone, in any order of the rows."""
+    ids = torch.cat([torch.full((c,), i) for i, c in enumerate(counts)] + [torch.full((9,), -1)]).int()
+    ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(len(ids)))].to(DEV)
+    c = Case(lora, len(ids), 264, 200, 24, len(counts), "bf16", ids=ids)
+    gpu_case(f"lora grad rows of {counts}")
+    got = both(lora, c)
+    torch.cuda.synchronize()
+    c.check_grad(*got)
+
+
 @pytest.mark.parametrize("rows,K,N,R", [(96, 2560, 2560, 16), (40, 136, 50000, 16), (1030, 512, 20000, 64)])
 def test_gradients_of_long_products(lora, rows, K, N, R):
     c = Case(lora, rows, K, N, R, 2, "bf16")
@@ -476,6 +489,20 @@ def test_gradients_against_differences(lora):
     by = (c.dy.double() * torch.bmm(c.of(step), h.double()[:, :, None])[:, :, 0]).sum()
     size = (db.double().abs() * step.abs()).sum()
     assert (by - (db.double() * step).sum()).abs() <= (c.eps + 600 * STEP) * size
+
+
+def test_autograd_refuses_operands_written_to(lora):
+    for which in ("a", "b", "scale"):
+        c = Case(lora, 20, 64, 72, 8, 2, "bf16")
+        a, b, scale = c.w.a.clone().requires_grad_(), c.w.b.clone(), c.w.scale.clone()
+        w = lora.LoraStack(a, b, scale)
+        gpu_case(f"lora autograd, {which} written to")
+        out = lora.add_lora(c.y, c.x, w, c.rows)
+        with torch.no_grad():
+            getattr(w, which).mul_(2)
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.sum().backward()
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
