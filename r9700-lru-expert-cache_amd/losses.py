@@ -280,7 +280,7 @@ def distill_top(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch
 
     A negative id is none, with its value. One past the vocabulary, a NaN or +inf give a row of NaN. A weight of 0
     gives 0 and no gradient; the logits of such a row may be anything. An id listed twice has a term for each, and
-    where probabilities sum to more than 1 there is no rest. Where all that is not listed is at -inf, or nothing is, the
+    where probabilities sum to 1 or more there is no rest (the gradient takes an excess of up to 2^-16 for rounding). Where all that is not listed is at -inf, or nothing is, the
     rest's term is left out of the loss, and the listed tokens' gradient is p_j - q_j. Weight, backward: as policy_loss."""
     _check_distill("distill_top", logits, top_ids, top_logprobs, weight, temperature)
     if not _differentiable("distill_top", logits):

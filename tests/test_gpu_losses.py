@@ -374,6 +374,33 @@ def test_an_id_listed_twice(losses):
         torch.testing.assert_close(grad, want[rows], rtol=2 * SUM, atol=200 * STEP)
 
 
+@pytest.mark.parametrize("R", [5, 300])
+def test_probabilities_of_more_than_one(losses, R):
+    """A teacher's certain token at 0 after rounding, or a little above: the gradient is p - q. Above by more: S p - q."""
+    x = torch.zeros(R, 2001, device=DEV)
+    x[:, 7] = 30.0
+    ids = torch.tensor([[7, 3]], dtype=torch.int32, device=DEV).expand(R, 2).contiguous()
+    w = torch.ones(R, device=DEV)
+    p = torch.softmax(x.double(), 1)[0]
+    for top in (0.0, 1e-6, 1e-5, 1e-4, 0.3):
+        v = torch.tensor([[top, -12.0]], device=DEV).expand(R, 2).contiguous()
+        gpu_case(f"distill R={R} with a log probability of {top}")
+        loss, grad = losses.distill_top_grad(x, ids, v, w)
+        torch.cuda.synchronize()
+        q = v[0].double().exp()
+        S = q.sum() if q.sum() > 1 + 2.0 ** -16 else 1.0               # (at 1e-5 it is: e^-12 = 0.6e-5 comes on top)
+        want = S * p
+        want[7] -= q[0]
+        want[3] -= q[1]
+        # at 7 an exponential, S, their product and difference (2, 3, 1 and 1 steps of at most 1.4), at 3 the exponential
+        # alone, the others an exponential of -30
+        limit = 220 * STEP * p
+        limit[7], limit[3] = 10 * STEP, 10 * STEP * q[1]
+        near(grad, want.expand(R, -1), limit, "grad")
+        cost = q * (v[0].double() - torch.log(p[[7, 3]]))
+        near(loss, cost.sum().expand(R), 10 * STEP * cost.abs().sum(), "loss")
+
+
 def test_where_everything_is_listed(losses):
     x, _ = rows_of(300, 20, "f32", 3)
     ids = torch.stack([torch.randperm(20, device=DEV) for _ in range(300)]).int()
