@@ -367,7 +367,7 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
  *   distill_top: top_ids [R, top] int32 (below 0: none; >= V: NaN row), top_logprobs [R, top].
  *     rest 1: q = e^top_logprobs and one outcome more, all tokens not listed, of probability 1 - sum q (0 where
  *     that is negative): loss = weight sum q ln(q / p) over the listed and that one. Where no unlisted token has a
- *     probability the last has no term.
+ *     probability the last has no term. grad of a listed token: p - q, or sum(q) p - q where the sum is over 1 + 2^-16.
  *     rest 0: q = softmax(top_logprobs / temperature) over the listed, which may be logits.
  *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf: NaN throughout.
  * 0 <= clip_low <= 1, clip_high >= 0, 0 <= kl < inf, temperature > 0 and 1 / temperature finite, 1 <= top <= 32. ws:
@@ -398,7 +398,7 @@ int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* 
  *   0 none, n or more: the row becomes NaN. size: rows of a tile, 16 or 64. cap = rows / size + min(rows, n + 2).
  *   order [rows], tiles [cap][4] (16-byte aligned), first [n + 5]: for the calls below, which trust them.
  * rlu_lora_add: hidden [rows][R] f32 = scale x a^T (0 in rows without an adapter), out [rows][N] = y + hidden b^T
- *   (y in those), with two launches. out may be y (same address and ld), but overlaps nothing else.
+ *   (y in those), in one launch or two. out may be y (same address and ld), but overlaps nothing else.
  * rlu_lora_grad: from dy [rows][N] and hidden as rlu_lora_add left it, with u = scale dy b: dx [rows][K] = u a (0 in
  *   rows without an adapter), da = u^T x, db = dy^T hidden of each adapter over its rows (0 for one without rows);
  *   each may be NULL. lddy, ldx < 2^31. ws: what rlu_lora_grad_workspace says, 16-byte aligned, used until the kernels end.

@@ -13,7 +13,8 @@ namespace rlu {
 namespace lora {
 
 // ---- rows by adapter: a stable counting sort in one workgroup ---------------------------------------------
-// Each wave counts and later places a run of the rows, 64 at a time in order, so the order is the same on every run.
+// Each wave counts and later places a run of the rows, 64 at a time in order, so the order is the same on every run. One
+// workgroup's chain of loads and barriers: 3 - 4 us up to 8192 rows, once for all the projections of a batch.
 constexpr int PLAN_NT = 1024, PLAN_NW = PLAN_NT / WAVE;
 
 __device__ __forceinline__ int key_of(const void* ids, int wide, int row, int n) {
@@ -117,7 +118,9 @@ __device__ __forceinline__ Tile part_of(const Fwd& f, int block) {
 // ---- h = s x A^T ------------------------------------------------------------------------------------------
 // A workgroup 16 or 32 rows and 64 ranks: its waves take turns at the depth, 64 of it at a time, and are summed through
 // LDS. Rows of x and of A come in pieces of 128 bytes a row and go through LDS: as the matrix unit wants them, with each
-// lane's neighbour in another row, a load would take 64 accesses of 16 bytes.
+// lane's neighbour in another row, a load would take 64 accesses of 16 bytes (measured: 64 cache accesses a load).
+// Bound by x: 8192 x 2560 with ranks of 64 22 us, 1.9 TB/s of x's 42 MB, and 18.6 where nothing is written before it (28 - 40
+// with other depths, threads or rows a workgroup); 160 x 2560, R = 16, 32 adapters 5 - 6 us, a chain of five steps.
 constexpr int SHRINK_NT = 512, DEPTH = 2;
 
 template <int MT, int RB>
