@@ -416,6 +416,24 @@ def test_gradients_of_high_ranks_one_by_one(lora, rows, n, R):
             assert torch.equal(t, u) if n else t is None
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,K,N,R", [(30, 256, 320, 16), (1100, 129, 65, 40), (1100, 128, 264, 8)])
+def test_factors_at_any_address(lora, dtype, rows, K, N, R):
+    """Adapters, their scale and hidden one element behind an aligned address: the same bits."""
+    c = Case(lora, rows, K, N, R, 3, dtype)
+    off = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)     # noqa: E731
+    w = lora.LoraStack(off(c.w.a), off(c.w.b), off(c.w.scale))
+    assert w.a.data_ptr() % 16 and w.b.data_ptr() % 16 and w.scale.data_ptr() % 16
+    h, g = torch.empty(rows, R, device=DEV), off(torch.full((rows, R), NAN, device=DEV))
+    gpu_case(f"lora {dtype} factors at odd addresses rows={rows}")
+    want = lora.add_lora(c.y, c.x, c.w, c.rows, hidden=h)
+    got = lora.add_lora(c.y, c.x, w, c.rows, hidden=g)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(g, h)
+    for t, u in zip(lora.add_lora_grad(c.dy, c.x, w, c.rows, g), lora.add_lora_grad(c.dy, c.x, c.w, c.rows, h)):
+        assert torch.equal(t, u)
+
+
 @pytest.mark.parametrize("rows", [45, 1300])
 def test_gradients_of_ids_past_the_last_and_nan(lora, rows):
     """A bad row has no part in the adapters' gradients; a NaN in a row goes to that row and to its adapter alone;
