@@ -69,6 +69,11 @@ struct Args {
 typedef Shape<512, 4> Usual;
 typedef Shape<1024, 4> Wide;
 typedef Shape<256, 2> Short;
+// Rows that one chunk of these holds: the work that a row costs whatever its length, one wave's coefficients and the waits
+// around them, then leaves the CU to more rows. (distill with 20 listed, bf16, in shapes of 512 / 256 / 64 threads, us: 40000
+// x 500 418 / 215 / 87, 4476 x 1666 55 / 34 / 19; 4096 x 8000 57 / 35 / 39, 1159 x 8000 21.4 / 14.6 / 23)
+typedef Shape<256, 4> Medium;
+typedef Shape<64, 4> Small;
 
 // The maximum of a row's unlisted logits and sum e^((x - m) / T) over them. Nothing: -inf, 0.
 struct Part {
@@ -614,13 +619,18 @@ static int launch(Args a, int dtype, void* ws, hipStream_t stream) {
   // The second read comes from the memory-side cache as long as the rows in flight fit there (256 MB): four
   // workgroups a CU of rows up to 256 KB. Of longer ones two: float32's with twice the threads, 16-bit ones' kept to
   // two by LDS that they do not use, as more threads a row leave the vector unit idle between its passes.
+  const long long vecs = (long long)a.V * (dtype == 1 ? 4 : 2) / 16 + 1;
   const bool longer = (long long)a.V * (dtype == 1 ? 4 : 2) > 256 << 10;
 #define RLU_ROW(DT, GRAD, S, LDS) \
   hipLaunchKernelGGL((row_k<DT, OP, GRAD, S>), rows, dim3(S::NT), LDS, stream, a)
 #define RLU_LOSS(DT)                                                                               \
   do {                                                                                             \
     if (a.nseg == 1) {                                                                             \
-      if (!a.grad) RLU_ROW(DT, false, Usual, 0);                                                   \
+      if (vecs <= Small::CHUNK && a.grad) RLU_ROW(DT, true, Small, 0);                             \
+      else if (vecs <= Small::CHUNK) RLU_ROW(DT, false, Small, 0);                                 \
+      else if (vecs <= Medium::CHUNK && a.grad) RLU_ROW(DT, true, Medium, 0);                      \
+      else if (vecs <= Medium::CHUNK) RLU_ROW(DT, false, Medium, 0);                               \
+      else if (!a.grad) RLU_ROW(DT, false, Usual, 0);                                              \
       else if (!longer) RLU_ROW(DT, true, Usual, 0);                                               \
       else if (DT == 1) RLU_ROW(1, true, Wide, 0);                                                 \
       else RLU_ROW(DT, true, Usual, 70 << 10);                                                     \

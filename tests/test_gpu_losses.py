@@ -180,7 +180,9 @@ def check_distill(loss, grad, x, ids, v, w, rest=True, T=1.0):
 SIZES = [(3, 1, 0, 0), (5, 2, 1, 1), (4, 5, 0, 3), (7, 33, 2, 0), (9, 255, 0, 1), (2, 256, 0, 0),
          (6, 2047, 3, 2), (6, 4097, 7, 1), (4, 16384, 0, 0), (3, 16391, 5, 3), (17, 32003, 2, 5),
          (2, 65537, 0, 1), (1, 151936, 0, 0), (20, 151936, 0, 0), (255, 9001, 0, 0), (256, 9001, 0, 0),
-         (300, 50001, 3, 1), (2, 499999, 1, 1), (1, 500000, 0, 0), (40000, 9, 0, 0)]
+         (300, 50001, 3, 1), (2, 499999, 1, 1), (1, 500000, 0, 0), (40000, 9, 0, 0),
+         (200, 1020, 1, 1), (200, 1030, 0, 0), (1000, 2040, 3, 7), (1000, 2049, 0, 0), (300, 4093, 5, 2), (400, 8185, 3, 1),
+         (200, 8200, 0, 0)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
