@@ -372,7 +372,7 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
  *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf: NaN throughout.
  * 0 <= clip_low <= 1, clip_high >= 0, 0 <= kl < inf, temperature > 0 and 1 / temperature finite, 1 <= top <= 32. ws:
  * what the first call says (top 1 for the policy loss), 8-byte aligned, used until the call's kernels end.
- * R = 0 launches nothing. Returns -1 (bad sizes or arguments, more than 2^23 - 1 workgroups, or a NULL pointer),
+ * R = 0 launches nothing. Returns -1 (bad sizes or arguments, more than 2^22 - 1 workgroups, or a NULL pointer),
  * -4 (misaligned logits, grad or ws). */
 int rlu_loss_workspace(int dtype, int R, int V, int top, long long* bytes);
 int rlu_policy_loss(const void* logits, int dtype, long long ld, int R, int V, const void* tokens,
