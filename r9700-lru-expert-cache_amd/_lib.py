@@ -116,6 +116,13 @@ def on_device(device):
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def written(t) -> None:
+    """For a caller's tensor that a kernel is about to write: autograd then refuses a backward pass that had
+    saved it, as after torch's own in-place operations."""
+    import torch
+    torch.autograd.graph.increment_version(t)
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed rc={rc}")

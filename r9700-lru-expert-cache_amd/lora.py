@@ -16,7 +16,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, lib, on_device, stream_ptr
+from ._lib import check, lib, on_device, stream_ptr, written
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 2}
 MAX_RANK = 128
@@ -177,6 +177,8 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
         hidden = torch.empty(M * a.shape[1], dtype=torch.float32, device=x.device)
     if out is None:
         out = torch.empty(M, b.shape[1], dtype=y.dtype, device=y.device)
+    else:
+        written(out)
     _forward(y, x, w, rows, hidden, out)
     return out
 

@@ -16,7 +16,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import check, lib, on_device, stream_ptr
+from ._lib import check, lib, on_device, stream_ptr, written
 from .logprobs import _DTYPE_CODE, MAX_VOCAB
 
 MAX_TOP = 32
@@ -181,6 +181,7 @@ def policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: t
         out = _grad_like(logits)
     else:
         _check_out(name, out, logits)
+        written(out)
     return _policy(logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
                    temperature, out), out
 
@@ -198,6 +199,7 @@ def distill_top_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: 
         out = _grad_like(logits)
     else:
         _check_out(name, out, logits)
+        written(out)
     return _distill(logits, top_ids, top_logprobs, weight, rest, temperature, out), out
 
 

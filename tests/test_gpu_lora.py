@@ -509,6 +509,22 @@ def test_gradients_against_differences(lora):
     assert (by - (db.double() * step).sum()).abs() <= (c.eps + 600 * STEP) * size
 
 
+def test_autograd_notices_an_output_that_was_written_over(lora):
+    c = Case(lora, 20, 64, 72, 8, 2, "bf16")
+    leaf = c.y.detach().clone().requires_grad_()
+    for out in (None, "y"):
+        y = torch.sigmoid(leaf)                                      # (whose backward pass asks for y)
+        gpu_case(f"lora into {out} beside autograd")
+        with torch.no_grad():
+            lora.add_lora(y, c.x, c.w, c.rows, out=out and y)
+        if out:
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.sum().backward()
+        else:
+            y.sum().backward()
+    torch.cuda.synchronize()
+
+
 def test_autograd_refuses_operands_written_to(lora):
     for which in ("a", "b", "scale"):
         c = Case(lora, 20, 64, 72, 8, 2, "bf16")

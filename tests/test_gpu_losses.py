@@ -559,6 +559,25 @@ def test_autograd(losses, dtype, R):
         assert not losses.distill_top(leaf, ids, v, w).requires_grad
 
 
+def test_autograd_notices_logits_that_were_written_over(losses):
+    h = torch.randn(5, 500, device=DEV, requires_grad=True)
+    tok = torch.randint(500, (5,), device=DEV)
+    old, adv = torch.full((5,), -6.0, device=DEV), torch.ones(5, device=DEV)
+    gpu_case("losses' gradient in place of logits that autograd has saved")
+    x = torch.tanh(h)                                                # (whose backward pass asks for x)
+    lg = x.detach()
+    _, g = losses.policy_loss_grad(lg, tok, old, adv, out=lg)
+    with pytest.raises(RuntimeError, match="inplace"):
+        x.backward(g)
+    x = 2 * h
+    lg = x.detach()
+    _, want = losses.policy_loss_grad(lg, tok, old, adv)
+    _, g = losses.policy_loss_grad(lg, tok, old, adv, out=lg)
+    x.backward(g)
+    torch.cuda.synchronize()
+    assert torch.equal(h.grad, 2 * want)
+
+
 def test_autograd_through_a_head(losses):
     """The loss's gradient goes on to a trainable head, as float32 autograd has it."""
     g = torch.Generator(DEV).manual_seed(1)
