@@ -290,11 +290,25 @@ __device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks,
   if (s0 == s1 || (first < last && (only || in_one(f, a)))) return;
   const size_t one = (size_t)f.R * o.cols;
   uint16_t* out = o.out + a * one;
-  for (size_t i = (size_t)block * NT + threadIdx.x; i < one; i += (size_t)blocks * NT) {
-    float v = 0.f;
+  for (size_t i = 8 * ((size_t)block * NT + threadIdx.x); i < one; i += (size_t)blocks * NT * 8) {
+    if (i + 8 <= one) {
+      v4f x = {}, y = {};
 #pragma unroll 4
-    for (int s = s0; s <= s1; ++s) v += o.parts[((size_t)s * 2 + (s == s0)) * one + i];
-    out[i] = (uint16_t)to_bits<DT>(v);
+      for (int s = s0; s <= s1; ++s) {
+        const float* p = o.parts + ((size_t)s * 2 + (s == s0)) * one + i;
+        x += *(const v4fa*)p;
+        y += *(const v4fa*)(p + 4);
+      }
+      const v4u v = {to_bits2<DT>(x[0], x[1]), to_bits2<DT>(x[2], x[3]), to_bits2<DT>(y[0], y[1]),
+                     to_bits2<DT>(y[2], y[3])};
+      store8(out + i, v, 8);
+    } else {
+      for (size_t e = i; e < one; ++e) {
+        float v = 0.f;
+        for (int s = s0; s <= s1; ++s) v += o.parts[((size_t)s * 2 + (s == s0)) * one + e];
+        out[e] = (uint16_t)to_bits<DT>(v);
+      }
+    }
   }
 }
 template <int DT>
@@ -303,26 +317,30 @@ __global__ __launch_bounds__(NT) void join_k(Bwd f) {
 }
 
 // ---- u over the strips --------------------------------------------------------------------------------------
-// 32 values of a tile a workgroup, eight threads each.
+// 32 times four ranks of a tile a workgroup, eight threads each.
 __global__ __launch_bounds__(NT) void sum_k(Bwd f) {
-  __shared__ float sums[8][32];
+  __shared__ v4f sums[8][32];
   if ((int)blockIdx.x >= f.p.first[f.p.n + 2]) return;
   const Tile t = f.p.tiles[blockIdx.x];
   const int e = (int)threadIdx.x % 32, q = (int)threadIdx.x / 32, i = (int)blockIdx.y * 32 + e;
-  const bool in = i < t.count * f.R;
-  const size_t at = in ? (size_t)f.p.order[t.start + i / f.R] * f.R + i % f.R : 0;
+  const int fours = (f.R + 3) / 4, r = i % fours * 4;
+  const bool in = i < t.count * fours;
+  const size_t at = in ? (size_t)f.p.order[t.start + i / fours] * f.R + r : 0;
   const int strips = (f.N + OUTER - 1) / OUTER;
   const size_t step = (size_t)f.p.rows * f.R + WAVE;
-  float v = 0.f;
-  if (in && t.adapter >= 0)
+  v4f v = {};
+  if (in && t.adapter >= 0)                            // (past the last rank: the next row's, or what is behind the last)
 #pragma unroll 8
-    for (int k = q; k < strips; k += 8) v += f.upart[k * step + at];
+    for (int k = q; k < strips; k += 8) v += *(const v4fa*)(f.upart + k * step + at);
   sums[q][e] = v;
   __syncthreads();
   if (q || !in) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) v += sums[k][e];
-  f.u[at] = t.adapter == BAD ? __builtin_nanf("") : v;
+  if (t.adapter == BAD) v = v4f{} + __builtin_nanf("");
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (r + k < f.R) f.u[at + k] = v[k];
 }
 
 // ---- what needs u, and what dB's launch left -------------------------------------------------------------------------
@@ -396,7 +414,7 @@ static void backward(const Bwd& f, const Last& l, hipStream_t stream) {
   else RLU_OUTER(4, f.R <= 64 ? 1 : 2);
 #undef RLU_OUTER
   if (f.dx || f.da)
-    hipLaunchKernelGGL(sum_k, dim3(cap, (f.size * f.R + 31) / 32), dim3(NT), 0, stream, f);
+    hipLaunchKernelGGL(sum_k, dim3(cap, (f.size * ((f.R + 3) / 4) + 31) / 32), dim3(NT), 0, stream, f);
   const auto blocks = [&](const Last& l) { return dim3((unsigned)(l.dx + l.da + l.joins * f.p.n)); };
 #define RLU_LAST(MT, RB, KS, L) \
   hipLaunchKernelGGL((last_k<DT, MT, RB, KS, WHOLE>), blocks(L), dim3(NT), 0, stream, f, L)
@@ -420,7 +438,7 @@ static void backward(const Bwd& f, const Last& l, hipStream_t stream) {
 #undef RLU_LAST_OF
 #undef RLU_LAST
   if (f.da && f.sa > 1) {
-    const long long per = ((long long)f.R * f.K + NT * 4 - 1) / (NT * 4);
+    const long long per = ((long long)f.R * f.K + NT * 8 - 1) / (NT * 8);
     hipLaunchKernelGGL((join_k<DT>), dim3(per < 512 ? per : 512, f.p.n), dim3(NT), 0, stream, f);
   }
 }
@@ -445,12 +463,12 @@ static int grad_sizes(rlu::lora::Bwd& f, rlu::lora::Last& l, int dtype, int rows
   // Workgroups for an adapter's parts: those of an adapter without any end at once, and of 64 adapters with 512 each that
   // took 50 us; with 32 each, one that has all of 8192 rows at R = 64 took 90 us more than with 128.
   const long long each = 8192 / n > 1 ? (8192 / n < 512 ? 8192 / n : 512) : 1;
-  const long long joins = (most + NT * 4 - 1) / (NT * 4);
+  const long long joins = (most + NT * 8 - 1) / (NT * 8);
   const long long blocks = 2ll * ((N + OUTER - 1) / OUTER) * f.sb, dx = cap * strips,
                   da = ((K + OUTER - 1) / OUTER) * (R > 64 ? 2ll : 1ll) * f.sa;
   l = {(int)dx, (int)da, (int)(joins < each ? joins : each), (int)strips, strip, R > 64 ? 2 : 1};
   if (blocks > UINT32_MAX / NT || dx + da + (long long)l.joins * n > UINT32_MAX / NT ||
-      4ll * cap * R * (size / 16) > UINT32_MAX / NT)
+      (long long)cap * ((size * ((R + 3) / 4) + 31) / 32) > UINT32_MAX / NT)
     return -1;                                         // (a launch counts its threads in 32 bits)
   return 0;
 }
