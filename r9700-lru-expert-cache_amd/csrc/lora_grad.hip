@@ -77,17 +77,17 @@ __device__ __forceinline__ int run_start(const Bwd& f, int tile) {
 
 template <int RB, bool DB>
 struct OuterLds {
-  static constexpr int W = 16 * RB;
+  static constexpr int W = 16 * RB, UW = W + 4;       // (four rows apart lie 16 banks apart)
   alignas(16) uint16_t v[NW * 32 * 72];    // the step's rows [32][VLD]; before them each wave's part of B
   alignas(16) uint16_t h[2][W * 40];       // both parts of h or u, [rank][row]
-  float u[DB ? NW : 1][DB ? 32 * W : 1];
+  float u[DB ? NW : 1][DB ? 32 * UW : 1];
   int row[2][DB ? 32 : 1];                 // where the rows of this step and of the one before lie
   float top[NW];
 };
 
 template <int DT, int RB, bool WHOLE, bool DB>
 __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<RB, DB>& lds) {
-  constexpr int W = 16 * RB, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
+  constexpr int W = 16 * RB, UW = W + 4, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
   const Side o = side_of<DB>(f);
   const int strips = (o.cols + OUTER - 1) / OUTER, run = block / strips, strip = block % strips;
   const int per = tiles_a_run(f.p, o.runs), t0 = run_start(f, run * per), t1 = run_start(f, (run + 1) * per);
@@ -126,12 +126,13 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
     struct Places {
       int v[4], h[EACH];
     };
+    const int hrow = tid / W * 2;          // (two rows of h, one below the other, a thread)
     auto places = [&](int pos) __attribute__((always_inline)) {        // (past the end: the last row again)
       Places n;
 #pragma unroll
       for (int i = 0; i < 4; ++i) n.v[i] = f.p.order[min(pos + vr + 2 * i, p1 - 1)];
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) n.h[i] = f.p.order[min(pos + (tid + i * NT) / W, p1 - 1)];
+      for (int i = 0; i < EACH; ++i) n.h[i] = f.p.order[min(pos + hrow + i % 2 + i / 2 * (2 * NT / W), p1 - 1)];
       return n;
     };
     const int hcol = min(r0 + tid % W, f.R - 1);       // (NT is a multiple of W)
@@ -172,12 +173,11 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
 #pragma unroll
       for (int i = 0; i < 4; ++i) *(v4u*)&lds.v[(vr + 2 * i) * VLD + lane % 32 * 8] = vv[i];
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        const int q = tid + i * NT;
-        const bool in = q / W < p1 - pos && q % W < f.R - r0;
-        const Split<DT> p(in ? hv[i] * by : 0.f);
-        lds.h[0][q % W * 40 + q / W] = (uint16_t)p.hi;
-        lds.h[1][q % W * 40 + q / W] = (uint16_t)p.lo;
+      for (int i = 0; i < EACH; i += 2) {
+        const int row = hrow + i * (NT / W), n = tid % W < f.R - r0 ? p1 - pos - row : 0;
+        const Split<DT> p(n > 0 ? hv[i] * by : 0.f), q(n > 1 ? hv[i + 1] * by : 0.f);
+        *(uint32_t*)&lds.h[0][tid % W * 40 + row] = p.hi | q.hi << 16;
+        *(uint32_t*)&lds.h[1][tid % W * 40 + row] = p.lo | q.lo << 16;
       }
       if (DB && lane % 32 == 0) {
 #pragma unroll
@@ -200,7 +200,7 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
 #pragma unroll
           for (int j = 0; j < RB; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) lds.u[w][(16 * i + 4 * g + e) * W + 16 * j + col] = u[j][e];
+            for (int e = 0; e < 4; ++e) lds.u[w][(16 * i + 4 * g + e) * UW + 16 * j + col] = u[j][e];
         }
       v4u vf[4];
 #pragma unroll
@@ -227,8 +227,9 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
           // it. What lies past the last row or rank goes to a row that nobody reads.)
           const int q = tid + i * NT;
           const bool in = q / W < p1 - pos && q % W < f.R - r0;
+          const int at = q / W * UW + q % W;
           upart[in ? (uint32_t)lds.row[odd][q / W] * (uint32_t)f.R + hcol : spare + lane] =
-              s * ((lds.u[0][q] + lds.u[1][q]) + (lds.u[2][q] + lds.u[3][q]));
+              s * ((lds.u[0][at] + lds.u[1][at]) + (lds.u[2][at] + lds.u[3][at]));
         }
       }
       odd ^= 1;
