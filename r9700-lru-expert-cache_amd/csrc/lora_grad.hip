@@ -59,20 +59,26 @@ __device__ __forceinline__ Side side_of(const Bwd& f) {
             : Side{f.x, f.ldx, f.K, f.sa, f.u, f.da, f.pa};
 }
 
-// Tiles of a run: as many runs as there is work for, adapters of their own or 128 rows.
-__device__ __forceinline__ int tiles_a_run(const Plan& p, int runs) {
-  const int total = p.first[p.n], live = p.first[p.n + 3], rows = p.first[p.n + 4];
-  const int use = max(1, min(runs, max(live, rows / 128)));
-  return max(1, (total + use - 1) / use);
+// Runs: one for each adapter that has rows, or for 128 rows; for 64 rows where that leaves CUs without a workgroup (256 rows
+// of one adapter, [2560 -> 2560], R = 64, us: in two of 128 44, in four of 64 27, in eight of 32 28). Adapters of up to twice
+// that are not cut by a run's end: their parts and the join cost more than uneven runs (256 rows of 8 adapters over [2560 ->
+// 10240], R = 16: 27 us cut, 20 not).
+constexpr int FEWEST = 64;
+struct Runs {
+  int per, whole;                          // tiles of a run; tiles of an adapter that is not cut
+};
+__device__ __forceinline__ Runs runs_of(const Bwd& f, const Side& o) {
+  const int total = f.p.first[f.p.n], live = f.p.first[f.p.n + 3], rows = f.p.first[f.p.n + 4];
+  const int strips = (o.cols + OUTER - 1) / OUTER, each = strips * max(live, rows / 128) >= 256 ? 128 : FEWEST;
+  const int use = max(1, min(o.runs, max(live, rows / each)));
+  return {max(1, (total + use - 1) / use), 2 * each / f.size};
 }
-// Adapters of few rows are not cut by a run's end: their parts and the join cost more than uneven runs (256 rows of 8
-// adapters over [2560 -> 10240], R = 16: 27 us cut, 20 not).
-__device__ __forceinline__ bool in_one(const Bwd& f, int a) { return (f.p.first[a + 1] - f.p.first[a]) * f.size <= 256; }
-__device__ __forceinline__ int run_start(const Bwd& f, int tile) {
+__device__ __forceinline__ bool in_one(const Bwd& f, const Runs& r, int a) { return f.p.first[a + 1] - f.p.first[a] <= r.whole; }
+__device__ __forceinline__ int run_start(const Bwd& f, const Runs& r, int tile) {
   const int total = f.p.first[f.p.n];
   if (tile >= total) return total;
   const int a = f.p.tiles[tile].adapter;
-  return in_one(f, a) ? f.p.first[a] : tile;
+  return in_one(f, r, a) ? f.p.first[a] : tile;
 }
 
 template <int RB, bool DB>
@@ -90,7 +96,8 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
   constexpr int W = 16 * RB, UW = W + 4, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
   const Side o = side_of<DB>(f);
   const int strips = (o.cols + OUTER - 1) / OUTER, run = block / strips, strip = block % strips;
-  const int per = tiles_a_run(f.p, o.runs), t0 = run_start(f, run * per), t1 = run_start(f, (run + 1) * per);
+  const Runs r = runs_of(f, o);
+  const int t0 = run_start(f, r, run * r.per), t1 = run_start(f, r, (run + 1) * r.per);
   const int lane = lane_id(), tid = (int)threadIdx.x, w = uniform(tid / WAVE), col = lane % 16, g = lane / 16;
   const int c0 = strip * OUTER + w * 64;
   uint16_t* mine = lds.v + w * 32 * 72;
@@ -285,10 +292,10 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 4 && DT != 0 ? 1 : 2) void 
 template <int DT, bool DB>
 __device__ __forceinline__ void join(const Bwd& f, int a, int block, int blocks, bool only) {
   const Side o = side_of<DB>(f);
-  const int per = tiles_a_run(f.p, o.runs);
+  const Runs r = runs_of(f, o);
   const int first = f.p.first[a], last = f.p.first[a + 1];
-  const int s0 = first < last ? first / per : 0, s1 = first < last ? (last - 1) / per : -1;
-  if (s0 == s1 || (first < last && (only || in_one(f, a)))) return;
+  const int s0 = first < last ? first / r.per : 0, s1 = first < last ? (last - 1) / r.per : -1;
+  if (s0 == s1 || (first < last && (only || in_one(f, r, a)))) return;
   const size_t one = (size_t)f.R * o.cols;
   uint16_t* out = o.out + a * one;
   for (size_t i = 8 * ((size_t)block * NT + threadIdx.x); i < one; i += (size_t)blocks * NT * 8) {
@@ -382,15 +389,18 @@ __global__ __launch_bounds__(NT, RB == 1 ? 3 : 2) void last_k(Bwd f, Last l) {
   if (f.da) join<DT, false>(f, a, block % l.joins, l.joins, true);
 }
 
-// Runs, at most: workgroups for every CU, twice over; see tiles_a_run.
-static int runs_of(int strips, int rows, int n) {
-  const int want = (512 + strips - 1) / strips, most = rows / 128 > n ? rows / 128 : rows < n ? rows : n;
+// Runs, at most: as many workgroups as the CUs take at a time, two each, and three of up to 16 ranks. (strips: of all passes
+// over the ranks. 8192 rows of [2560 -> 10240], us: R = 64 with 240 workgroups 190, 480 162, 760 178; R = 128 with 480 277, 560
+// 314; 512 rows of 64 adapters, R = 16, with 480 47, 760 43)
+static int runs_at_most(int strips, int rows, int n, int R) {
+  const int slots = R <= 16 ? 768 : 512, want = strips < slots ? slots / strips : 1;
+  const int most = rows / FEWEST > n ? rows / FEWEST : rows < n ? rows : n;
   return want < most ? want : most > 1 ? most : 1;
 }
 static void layout(Bwd& f, long long* bytes) {
-  const int strips = (f.N + OUTER - 1) / OUTER;
-  f.sa = runs_of((f.K + OUTER - 1) / OUTER, f.p.rows, f.p.n);
-  f.sb = runs_of(strips, f.p.rows, f.p.n);
+  const int strips = (f.N + OUTER - 1) / OUTER, passes = f.R > 64 ? 2 : 1;
+  f.sa = runs_at_most((f.K + OUTER - 1) / OUTER * passes, f.p.rows, f.p.n, f.R);
+  f.sb = runs_at_most(strips * passes, f.p.rows, f.p.n, f.R);
   long long at = 0;
   auto take = [&](long long n) {
     const long long was = at;
