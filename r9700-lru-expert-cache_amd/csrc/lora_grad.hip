@@ -4,8 +4,9 @@
 // they lie in memory: their tiles go through LDS as they are and are read transposed. h and u take part as sums of two
 // 16-bit values each.
 //
-// Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 78 - 84 us for u and dB, then 9.4 for u over the strips, 9.4 for
-// dx, dA and dB's parts, 5.7 for dA's. 96 x 2560 x 2560 with one adapter: 7, 3, 5 us, each launch a chain of a few loads.
+// Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 79 - 83 us for u and dB, then 10 for u over the strips, 8 for dx,
+// dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 45 + 8 + 15 + 5, R = 64 83 + 15 + 45 + 7, where the
+// registers leave two workgroups a CU. 96 x 2560 x 2560 with one adapter: 7, 3, 4 us, each launch a chain of a few loads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -325,7 +326,8 @@ __global__ __launch_bounds__(NT) void join_k(Bwd f) {
 }
 
 // ---- u over the strips --------------------------------------------------------------------------------------
-// 32 times four ranks of a tile a workgroup, eight threads each.
+// 32 times four ranks of a tile a workgroup, eight threads each. (8192 rows, 40 strips, R = 64: 25 us with a rank a thread, 15;
+// 16 times four by 16 threads 16, 8 by 32 22)
 __global__ __launch_bounds__(NT) void sum_k(Bwd f) {
   __shared__ v4f sums[8][32];
   if ((int)blockIdx.x >= f.p.first[f.p.n + 2]) return;
