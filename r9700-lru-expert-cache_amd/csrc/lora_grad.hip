@@ -5,7 +5,7 @@
 // 16-bit values each.
 //
 // Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 79 - 83 us for u and dB, then 10 for u over the strips, 8 for dx,
-// dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 45 + 8 + 15 + 5, R = 64 83 + 15 + 45 + 7, where the
+// dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 46 + 8 + 26 + 5, R = 64 83 - 91 + 16 + 48 + 7, where the
 // registers leave two workgroups a CU. 96 x 2560 x 2560 with one adapter: 7, 3, 4 us, each launch a chain of a few loads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
