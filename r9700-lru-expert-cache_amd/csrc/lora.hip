@@ -119,21 +119,21 @@ __device__ __forceinline__ Tile part_of(const Fwd& f, int block) {
 // A workgroup 16 or 32 rows and 64 ranks: its waves take turns at the depth, 64 of it at a time, and are summed through
 // LDS. Rows of x and of A come in pieces of 128 bytes a row and go through LDS: as the matrix unit wants them, with each
 // lane's neighbour in another row, a load would take 64 accesses of 16 bytes (measured: 64 cache accesses a load).
-// Bound by x: 8192 x 2560 with ranks of 64 22 us, 1.9 TB/s of x's 42 MB, and 18.6 where nothing is written before it (28 - 40
-// with other depths, threads or rows a workgroup); 160 x 2560, R = 16, 32 adapters 5 - 6 us, a chain of five steps.
+// Bound by x: 8192 x 2560 with ranks of 64 19 - 20 us, 2.2 TB/s of x's 42 MB behind the writes of what ran before (three steps
+// ahead 24, 16 rows a workgroup 20.5); 160 x 2560, R = 16, 32 adapters 5 - 6 us, a chain of five steps.
 constexpr int SHRINK_NT = 512, DEPTH = 2;
 
-template <int MT, int RB>
+template <int MT, int RB, int NT>
 struct ShrinkLds {
-  static constexpr int NW = SHRINK_NT / WAVE, T = 16 * MT, W = 16 * RB, LD = 64;
+  static constexpr int NW = NT / WAVE, T = 16 * MT, W = 16 * RB, LD = 64;
   static constexpr int TILES = NW * (T + W) * LD, SUMS = 2 * NW * T * W;
   alignas(16) uint16_t tiles[TILES > SUMS ? TILES : SUMS];             // rows of x and A, then each wave's sums
 };
 
 // Calls put(row, rank, h) for the rows of t and the ranks from r0 on.
-template <int DT, int MT, int RB, bool WHOLE, class Put>
-__device__ __forceinline__ void shrink(const Fwd& f, const Tile& t, int r0, ShrinkLds<MT, RB>& lds, Put put) {
-  typedef ShrinkLds<MT, RB> L;
+template <int DT, int MT, int RB, bool WHOLE, int NT, class Put>
+__device__ __forceinline__ void shrink(const Fwd& f, const Tile& t, int r0, ShrinkLds<MT, RB, NT>& lds, Put put) {
+  typedef ShrinkLds<MT, RB, NT> L;
   constexpr int NW = L::NW, T = L::T, W = L::W, LD = L::LD;
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
   const int r8 = lane / 8, c8 = lane % 8 * 8;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void shrink(const Fwd& f, const Tile& t, int r0, Shri
       for (int e = 0; e < 4; ++e) sums[(w * T + 16 * i + 4 * g + e) * W + 16 * j + col] = acc[i][j][e];
   __syncthreads();
   const float s = f.scale[t.adapter];
-  for (int i = (int)threadIdx.x; i < t.count * W; i += SHRINK_NT) {
+  for (int i = (int)threadIdx.x; i < t.count * W; i += NT) {
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < NW; ++q) v += sums[q * T * W + i];
@@ -205,22 +205,22 @@ __device__ __forceinline__ void shrink(const Fwd& f, const Tile& t, int r0, Shri
   }
 }
 // h of rows without an adapter, and of ids past the last
-template <class Put>
+template <int NT, class Put>
 __device__ __forceinline__ void bare(const Fwd& f, const Tile& t, int r0, int ranks, Put put) {
   const float v = t.adapter == NONE ? 0.f : __builtin_nanf("");
-  for (int i = (int)threadIdx.x; i < t.count * ranks; i += SHRINK_NT)
+  for (int i = (int)threadIdx.x; i < t.count * ranks; i += NT)
     if (r0 + i % ranks < f.R) put(i / ranks, r0 + i % ranks, v);
 }
 
-template <int DT, int MT, int RB, bool WHOLE>
-__global__ __launch_bounds__(SHRINK_NT) void shrink_k(Fwd f) {
-  __shared__ ShrinkLds<MT, RB> lds;
+template <int DT, int MT, int RB, bool WHOLE, int NT>
+__global__ __launch_bounds__(NT) void shrink_k(Fwd f) {
+  __shared__ ShrinkLds<MT, RB, NT> lds;
   const Tile t = part_of<MT>(f, (int)blockIdx.x);
   if (t.count <= 0) return;
   const int r0 = (int)blockIdx.y * 16 * RB;
   auto put = [&](int row, int r, float v) { f.hidden[(size_t)f.p.order[t.start + row] * f.R + r] = v; };
-  if (t.adapter < 0) bare(f, t, r0, 16 * RB, put);
-  else shrink<DT, MT, RB, WHOLE>(f, t, r0, lds, put);
+  if (t.adapter < 0) bare<NT>(f, t, r0, 16 * RB, put);
+  else shrink<DT, MT, RB, WHOLE, NT>(f, t, r0, lds, put);
 }
 
 template <int DT, int MT, int KS, bool WHOLE>
@@ -246,7 +246,7 @@ template <int DT, int RB, bool WHOLE>
 __global__ __launch_bounds__(SHRINK_NT) void both_k(Fwd f, int strips) {
   constexpr int KS = (RB + 1) / 2, LD = 16 * RB + 4;
   __shared__ union {
-    ShrinkLds<1, RB> first;
+    ShrinkLds<1, RB, SHRINK_NT> first;
     ExpandLds<1, KS, false, SHRINK_NT> then;
   } lds;
   __shared__ float h[16 * LD];
@@ -259,8 +259,8 @@ __global__ __launch_bounds__(SHRINK_NT) void both_k(Fwd f, int strips) {
     h[row * LD + r] = v;
     if (strip == 0) f.hidden[(size_t)f.p.order[t.start + row] * f.R + r] = v;
   };
-  if (t.adapter < 0) bare(f, t, 0, 16 * RB, put);
-  else shrink<DT, 1, RB, WHOLE>(f, t, 0, lds.first, put);
+  if (t.adapter < 0) bare<SHRINK_NT>(f, t, 0, 16 * RB, put);
+  else shrink<DT, 1, RB, WHOLE, SHRINK_NT>(f, t, 0, lds.first, put);
   if (t.adapter == NONE) return copy<SHRINK_NT>(o, f.p, t, n0, n1);
   __syncthreads();
   stage<DT, 1, KS, SHRINK_NT>(lds.then.h, t.count, f.R, [&](int row) { return (const float*)h + row * LD; });
@@ -278,9 +278,12 @@ static void forward(const Fwd& f, hipStream_t stream) {
     return;
   }
   const int strip = strip_of(f.p.cap, f.size, f.N), strips = (f.N + strip - 1) / strip;
+  // 64 ranks of 32 rows: half the threads, as the others' LDS (98 KB) would leave them a workgroup a CU and some CUs a second
+  // one after it (8192 x 2560: 22.4 us, 19.5 so; 16 ranks of 1024 rows 8.3 and 9.4)
 #define RLU_SHRINK(MT, RB, Y)                                                                      \
-  hipLaunchKernelGGL((shrink_k<DT, MT, RB, WHOLE>), dim3(f.p.cap * (f.size / (16 * MT)), Y),       \
-                     dim3(SHRINK_NT), 0, stream, f)
+  hipLaunchKernelGGL((shrink_k<DT, MT, RB, WHOLE, MT * RB == 8 ? SHRINK_NT / 2 : SHRINK_NT>),      \
+                     dim3(f.p.cap * (f.size / (16 * MT)), Y),                                      \
+                     dim3(MT * RB == 8 ? SHRINK_NT / 2 : SHRINK_NT), 0, stream, f)
 #define RLU_EXPAND(MT, KS)                                                                         \
   hipLaunchKernelGGL((expand_k<DT, MT, KS, WHOLE>), dim3(f.p.cap * strips), dim3(EXPAND_NT), 0,    \
                      stream, f, strips, strip)
