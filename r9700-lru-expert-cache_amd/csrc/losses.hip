@@ -585,10 +585,14 @@ __global__ __launch_bounds__(SCALE_NT) void scale_k(Args a, const float* __restr
   }
 }
 
-// Segments of a row: one where the rows alone fill the chip. (bf16 rows of 151936, policy, us: 16 rows 8.5 in segments, 26
-// whole; 128 24.4 and 30.5; 192 33.8 and 33.3; 255 42.3 and 39.4)
+// Vectors of a row, but for what its address adds.
+static long long vectors(int dtype, int V) { return (long long)V * (dtype == 1 ? 4 : 2) / 16 + 1; }
+
+// Segments of a row: one where the rows alone fill the chip, or a workgroup holds a row in its registers. (bf16, policy, us:
+// 16 rows of 151936 8.5 in segments, 26 whole; 128 24.4 and 30.5; 192 33.8 and 33.3; 255 42.3 and 39.4; 8 of 15000 7.2 and 6.5
+// and a launch less, 150 of them 9.1 and 7.3)
 static int segments(int dtype, int R, int V) {
-  if (R >= 192) return 1;
+  if (R >= 192 || vectors(dtype, V) <= Usual::CHUNK) return 1;
   const int n = dtype == 1 ? 4 : 8;
   const int chunks = (V + 2 * n - 2) / n / Short::CHUNK + 1, want = R ? (768 + R - 1) / R : 1;
   const int most = chunks < MAX_SEGS ? chunks : MAX_SEGS;
@@ -619,7 +623,7 @@ static int launch(Args a, int dtype, void* ws, hipStream_t stream) {
   // The second read comes from the memory-side cache as long as the rows in flight fit there (256 MB): four
   // workgroups a CU of rows up to 256 KB. Of longer ones two: float32's with twice the threads, 16-bit ones' kept to
   // two by LDS that they do not use, as more threads a row leave the vector unit idle between its passes.
-  const long long vecs = (long long)a.V * (dtype == 1 ? 4 : 2) / 16 + 1;
+  const long long vecs = vectors(dtype, a.V);
   const bool longer = (long long)a.V * (dtype == 1 ? 4 : 2) > 256 << 10;
 #define RLU_ROW(DT, GRAD, S, LDS) \
   hipLaunchKernelGGL((row_k<DT, OP, GRAD, S>), rows, dim3(S::NT), LDS, stream, a)
