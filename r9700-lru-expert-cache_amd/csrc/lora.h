@@ -131,15 +131,19 @@ __device__ __forceinline__ float scale_to(float m) {
   return __builtin_ldexpf(1.f, max(-100, min(100, 137 - ex)));
 }
 
-// f as the sum of two 16-bit values: 16 bits of it (22 in float16), for products with 8 (11)
+// f as the sum of 16-bit values, the largest first, for products with 16-bit ones: all of its 24 bits in three of bf16; in
+// two of float16 22, half a step of which is 2^-23 of f, no more than one addition of the float32 sums around it may lose.
 template <int DT>
 struct Split {
-  uint32_t hi, lo;
+  static constexpr int N = DT == 0 ? 3 : 2;
+  uint32_t part[N];
   __device__ __forceinline__ explicit Split(float f) {
-    hi = DT == 0 ? f32_to_bf16_hw(f) : to_bits<DT>(f);
-    float r = f - to_f32<DT>(hi);
-    r = r == r ? r : 0.f;                              // (an infinity's rest)
-    lo = DT == 0 ? f32_to_bf16_hw(r) : to_bits<DT>(r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      part[i] = DT == 0 ? f32_to_bf16_hw(f) : to_bits<DT>(f);
+      f -= to_f32<DT>(part[i]);
+      f = f == f ? f : 0.f;                            // (an infinity's rest)
+    }
   }
 };
 
@@ -157,17 +161,17 @@ __device__ __forceinline__ v4u frag_tr(const uint16_t* tile, int k, int c) {
   return __builtin_bit_cast(v4u, __builtin_shufflevector(read_tr(p), read_tr(p + 4 * LD), 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// A tile's rows of h or u, R floats each, as both their 16-bit parts in LDS, and by what sums with them are multiplied:
+// A tile's rows of h or u, R floats each, as their 16-bit parts in LDS, and by what sums with them are multiplied:
 // float16's are brought into its range by a power of two a row.
-template <int MT, int KS>
+template <int DT, int MT, int KS>
 struct Rows {
-  static constexpr int T = 16 * MT, LD = 32 * KS + 8;
-  uint16_t part[2][T][LD];
+  static constexpr int T = 16 * MT, LD = 32 * KS + 8, PARTS = Split<DT>::N;
+  uint16_t part[PARTS][T][LD];
   float back[T];
 };
 // rows: where the row-th of `count` rows lies
 template <int DT, int MT, int KS, int NT, class At>
-__device__ __forceinline__ void stage(Rows<MT, KS>& s, int count, int R, At rows) {
+__device__ __forceinline__ void stage(Rows<DT, MT, KS>& s, int count, int R, At rows) {
   constexpr int PER = NT / (16 * MT), N = (4 * KS + PER - 1) / PER;    // threads a row, chunks of 8 a thread
   const int row = (int)threadIdx.x / PER, q = (int)threadIdx.x % PER;
   const float* from = rows(min(row, count - 1));
@@ -190,15 +194,15 @@ __device__ __forceinline__ void stage(Rows<MT, KS>& s, int count, int R, At rows
   for (int k = 0; k < N; ++k) {
     const int c = k * PER + q;
     if (c >= 4 * KS) continue;
-    v4u hi, lo;
+    v4u p[Split<DT>::N];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const Split<DT> a(v[k][e] * by), b(v[k][e + 1] * by);
-      hi[e / 2] = a.hi | b.hi << 16;
-      lo[e / 2] = a.lo | b.lo << 16;
+#pragma unroll
+      for (int i = 0; i < Split<DT>::N; ++i) p[i][e / 2] = a.part[i] | b.part[i] << 16;
     }
-    *(v4u*)&s.part[0][row][8 * c] = hi;
-    *(v4u*)&s.part[1][row][8 * c] = lo;
+#pragma unroll
+    for (int i = 0; i < Split<DT>::N; ++i) *(v4u*)&s.part[i][row][8 * c] = p[i];
   }
 }
 
@@ -218,11 +222,11 @@ struct Out {
   int cols, R;
 };
 constexpr int EXPAND_NT = 256;
-template <int MT, int KS, bool TR, int NT = EXPAND_NT>
+template <int DT, int MT, int KS, bool TR, int NT = EXPAND_NT>
 struct ExpandLds {
   static constexpr int LD = TR ? 72 : 32 * KS + 8, SUM_LD = 68;
   static constexpr int W = TR ? 32 * KS * LD : 64 * LD, SUMS = 2 * 16 * SUM_LD;
-  Rows<MT, KS> h;
+  Rows<DT, MT, KS> h;
   alignas(16) uint16_t wave[NT / WAVE][W > SUMS ? W : SUMS];           // W, then a block's sums
 };
 
@@ -240,8 +244,8 @@ __device__ __forceinline__ void copy(const Out& f, const Plan& p, const Tile& t,
 // lds.h is staged; its barrier is to come.
 template <int DT, int MT, int KS, bool WHOLE, bool TR, bool ADD, int NT = EXPAND_NT>
 __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& t, int n0, int n1,
-                                       ExpandLds<MT, KS, TR, NT>& lds) {
-  typedef ExpandLds<MT, KS, TR, NT> L;
+                                       ExpandLds<DT, MT, KS, TR, NT>& lds) {
+  typedef ExpandLds<DT, MT, KS, TR, NT> L;
   constexpr int STEP = NT;                 // columns: 64 a wave
   constexpr bool ONCE = ADD && NT == EXPAND_NT;        // (what is more than a few tiles' outputs passes the cache by)
   const int lane = lane_id(), w = uniform((int)threadIdx.x / WAVE), col = lane % 16, g = lane / 16;
@@ -287,15 +291,13 @@ __device__ __forceinline__ void expand(const Out& f, const Plan& p, const Tile& 
     for (int i = 0; i < MT; ++i) {
       v4f acc[4] = {};
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const v4u lo = frag<32 * KS + 8>(lds.h.part[1][0], 16 * i, 32 * k);
-        const v4u hi = frag<32 * KS + 8>(lds.h.part[0][0], 16 * i, 32 * k);
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[j] = mfma<DT>(wf[j][k], lo, acc[j]);
-          acc[j] = mfma<DT>(wf[j][k], hi, acc[j]);
+        for (int p = Split<DT>::N - 1; p >= 0; --p) {
+          const v4u h = frag<32 * KS + 8>(lds.h.part[p][0], 16 * i, 32 * k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = mfma<DT>(wf[j][k], h, acc[j]);
         }
-      }
       if (DT != 0) {
         const float back = lds.h.back[16 * i + col];
 #pragma unroll

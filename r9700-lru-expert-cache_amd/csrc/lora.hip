@@ -225,7 +225,7 @@ __global__ __launch_bounds__(NT) void shrink_k(Fwd f) {
 
 template <int DT, int MT, int KS, bool WHOLE>
 __global__ __launch_bounds__(EXPAND_NT) void expand_k(Fwd f, int strips, int strip) {
-  __shared__ ExpandLds<MT, KS, false> lds;
+  __shared__ ExpandLds<DT, MT, KS, false> lds;
   const int tile = (int)(blockIdx.x / (unsigned)strips);
   if (tile >= f.p.first[f.p.n + 2]) return;
   const Tile t = f.p.tiles[tile];
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(SHRINK_NT) void both_k(Fwd f, int strips) {
   constexpr int KS = (RB + 1) / 2, LD = 16 * RB + 4;
   __shared__ union {
     ShrinkLds<1, RB, SHRINK_NT> first;
-    ExpandLds<1, KS, false, SHRINK_NT> then;
+    ExpandLds<DT, 1, KS, false, SHRINK_NT> then;
   } lds;
   __shared__ float h[16 * LD];
   const int tile = (int)(blockIdx.x / (unsigned)strips), strip = (int)(blockIdx.x % (unsigned)strips);

@@ -1,8 +1,8 @@
 // The backward pass of out = y + h B^T, h = s x A^T, from dy [rows, N] and h as the forward pass left it:
 //   u = s dy B, dx = u A; of each adapter over its own rows dA = u^T x, dB = dy^T h.
 // dy is read once, for u and for dB. Products over the rows (dA, dB) and over the rank (dx) need operands across the way
-// they lie in memory: their tiles go through LDS as they are and are read transposed. h and u take part as sums of two
-// 16-bit values each.
+// they lie in memory: their tiles go through LDS as they are and are read transposed. h and u take part as sums of 16-bit
+// values each (Split).
 //
 // Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 79 - 83 us for u and dB, then 10 for u over the strips, 8 for dx,
 // dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 46 + 8 + 26 + 5, R = 64 83 - 91 + 16 + 48 + 7, where the
@@ -82,18 +82,18 @@ __device__ __forceinline__ int run_start(const Bwd& f, const Runs& r, int tile) 
   return in_one(f, r, a) ? f.p.first[a] : tile;
 }
 
-template <int RB, bool DB>
+template <int DT, int RB, bool DB>
 struct OuterLds {
   static constexpr int W = 16 * RB, UW = W + 4;       // (four rows apart lie 16 banks apart)
   alignas(16) uint16_t v[NW * 32 * 72];    // the step's rows [32][VLD]; before them each wave's part of B
-  alignas(16) uint16_t h[2][W * 40];       // both parts of h or u, [rank][row]
+  alignas(16) uint16_t h[Split<DT>::N][W * 40];       // the parts of h or u, [rank][row]
   float u[DB ? NW : 1][DB ? 32 * UW : 1];
   int row[2][DB ? 32 : 1];                 // where the rows of this step and of the one before lie
   float top[NW];
 };
 
 template <int DT, int RB, bool WHOLE, bool DB>
-__device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<RB, DB>& lds) {
+__device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<DT, RB, DB>& lds) {
   constexpr int W = 16 * RB, UW = W + 4, EACH = 32 * W / NT, LDB = W + 8, VLD = OUTER + 8;
   const Side o = side_of<DB>(f);
   const int strips = (o.cols + OUTER - 1) / OUTER, run = block / strips, strip = block % strips;
@@ -184,8 +184,9 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
       for (int i = 0; i < EACH; i += 2) {
         const int row = hrow + i * (NT / W), n = tid % W < f.R - r0 ? p1 - pos - row : 0;
         const Split<DT> p(n > 0 ? hv[i] * by : 0.f), q(n > 1 ? hv[i + 1] * by : 0.f);
-        *(uint32_t*)&lds.h[0][tid % W * 40 + row] = p.hi | q.hi << 16;
-        *(uint32_t*)&lds.h[1][tid % W * 40 + row] = p.lo | q.lo << 16;
+#pragma unroll
+        for (int k = 0; k < Split<DT>::N; ++k)
+          *(uint32_t*)&lds.h[k][tid % W * 40 + row] = p.part[k] | q.part[k] << 16;
       }
       if (DB && lane % 32 == 0) {
 #pragma unroll
@@ -215,17 +216,19 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
       for (int c = 0; c < 4; ++c) vf[c] = frag_tr<VLD>(lds.v, 0, w * 64 + 16 * c);
 #pragma unroll
       for (int j = 0; j < RB; ++j) {
-        const v4u hi = frag<40>(lds.h[0], 16 * j, 0), lo = frag<40>(lds.h[1], 16 * j, 0);
+        v4f sums[4] = {};
+        v4f(&t)[4] = DT != 0 ? sums : acc[j];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          v4f t = DT != 0 ? v4f{} : acc[j][c];
-          t = DB ? mfma<DT>(vf[c], lo, t) : mfma<DT>(lo, vf[c], t);
-          t = DB ? mfma<DT>(vf[c], hi, t) : mfma<DT>(hi, vf[c], t);
-          if (DT == 0) acc[j][c] = t;
-          else
+        for (int k = Split<DT>::N - 1; k >= 0; --k) {
+          const v4u h = frag<40>(lds.h[k], 16 * j, 0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][c][e] = fmaf(t[e], 1.f / by, acc[j][c][e]);
+          for (int c = 0; c < 4; ++c) t[c] = DB ? mfma<DT>(vf[c], h, t[c]) : mfma<DT>(h, vf[c], t[c]);
         }
+        if (DT != 0)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][c][e] = fmaf(t[c][e], 1.f / by, acc[j][c][e]);
       }
       lds_barrier();
       if (DB) {
@@ -285,7 +288,7 @@ __device__ __forceinline__ void outer(const Bwd& f, int block, int r0, OuterLds<
 
 template <int DT, int RB, bool WHOLE>
 __global__ __launch_bounds__(NT, RB == 1 ? 3 : RB == 4 && DT != 0 ? 1 : 2) void outer_k(Bwd f) {
-  __shared__ OuterLds<RB, true> lds;
+  __shared__ OuterLds<DT, RB, true> lds;
   outer<DT, RB, WHOLE, true>(f, (int)blockIdx.x, (int)blockIdx.y * 16 * RB, lds);
 }
 
@@ -364,8 +367,8 @@ struct Last {
 template <int DT, int MT, int RB, int KS, bool WHOLE>
 __global__ __launch_bounds__(NT, RB == 1 ? 3 : 2) void last_k(Bwd f, Last l) {
   __shared__ union {
-    ExpandLds<MT, KS, true> dx;
-    OuterLds<RB, false> da;
+    ExpandLds<DT, MT, KS, true> dx;
+    OuterLds<DT, RB, false> da;
   } lds;
   int block = (int)blockIdx.x;
   if (block < l.dx) {

@@ -146,7 +146,7 @@ def _forward(y, x, w, rows, hidden, out) -> None:
 def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
              out: torch.Tensor | None = None, hidden: torch.Tensor | None = None) -> torch.Tensor:
     """y [rows, N] + scale (x [rows, K] a^T) b^T with each row's adapter, all of the stack's type; sums and
-    x a^T in float32, rounded once. Rows may be apart (x, y and out of any stride). A row without an adapter is y's.
+    x a^T in float32 (of which float16's second product takes 22 bits), rounded once. Rows may be apart (x, y and out of any stride). A row without an adapter is y's.
     out: where the result goes, y itself among others; a new tensor without it.
     hidden: float32 [rows, rank] that receives scale x a^T, for add_lora_grad."""
     a, b, M = w.a, w.b, rows.rows
