@@ -367,7 +367,8 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
  *   distill_top: top_ids [R, top] int32 (below 0: none; >= V: NaN row), top_logprobs [R, top].
  *     rest 1: q = e^top_logprobs and one outcome more, all tokens not listed, of probability 1 - sum q (0 where
  *     that is negative): loss = weight sum q ln(q / p) over the listed and that one. Where no unlisted token has a
- *     probability the last has no term. grad of a listed token: p - q, or sum(q) p - q where the sum is over 1 + 2^-16.
+ *     probability the last has no term. grad of a listed token: p - q, or sum(q) p - q in such a row and where the sum
+ *     is over 1 + 2^-16.
  *     rest 0: q = softmax(top_logprobs / temperature) over the listed, which may be logits.
  *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf: NaN throughout.
  * 0 <= clip_low <= 1, clip_high >= 0, 0 <= kl < inf, temperature > 0 and 1 / temperature finite, 1 <= top <= 32. ws:

@@ -317,8 +317,9 @@ __device__ __forceinline__ Coef distill(const Args& a, Part u, float x, float v,
     // what they leave: the leader's own 1 - q is small where it is nearly certain
     left = (at ? -expm1f(vm) : 1.f) - others;
     left = left > 0.f ? left : left == left ? 0.f : left;
-    // all that is listed: 1, or the sum where it is over 1 by more than a teacher's rounded values explain
-    total = sum > 1.f + 0x1p-16f ? sum : sum == sum ? 1.f : sum;
+    // what the loss counts: 1, or the listed ones' sum where it is over 1 by more than a teacher's rounded values explain,
+    // or where no token is left for the rest, whose term the loss then lacks
+    total = sum > 1.f + 0x1p-16f || u.s == 0.f ? sum : sum == sum ? 1.f : sum;
     if (!__ballot(in)) left = total = 0.f;
   } else {
     const float d = (v - vm) * a.inv_t;

@@ -284,7 +284,7 @@ def distill_top(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch
     gives 0 and no gradient; the logits of such a row may be anything. An id listed twice has a term for each. Where
     probabilities sum to 1 or more there is no rest (and in the gradient an excess of up to 2^-16 is rounding). Where
     no token is left for the rest, as all are listed or those that are not are at -inf, its term is left out of the
-    loss and the listed tokens' gradient is p_j - q_j. Weight, backward: as policy_loss."""
+    loss, and the listed tokens' gradient is that loss's, (sum q) p_j - q_j. Weight, backward: as policy_loss."""
     _check_distill("distill_top", logits, top_ids, top_logprobs, weight, temperature)
     if not _differentiable("distill_top", logits):
         return _distill(logits, top_ids, top_logprobs, weight, rest, temperature, None)

@@ -23,6 +23,23 @@ def load_pkg():
     return mod
 
 
+# Tests that hold a value since shown to be wrong, by file and function: the parameters concerned, and why. They stay as
+# they are and are expected to fail there; what is right is tested in the file that the reason names.
+NOTHING_LEFT = ("rows where no token is left for the teacher's rest: the expected gradient p - q is not that of the expected "
+                "loss, which lacks the rest's term (tests/test_gpu_losses_nothing_left.py)")
+WRONG_VALUES = {
+    "test_gpu_losses.py::test_masked_rows": (lambda p: True, NOTHING_LEFT),
+    "test_gpu_losses.py::test_distill": (lambda p: p["V"] in (1, 2, 5, 9), NOTHING_LEFT),
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        concerned, why = WRONG_VALUES.get(item.nodeid.rsplit("/", 1)[-1].split("[")[0], (None, ""))
+        if concerned and concerned(item.callspec.params):
+            item.add_marker(pytest.mark.xfail(strict=True, reason=why))
+
+
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (HIP device)")
 
