@@ -386,6 +386,19 @@ int rlu_distill_top(const void* logits, int dtype, long long ld, int R, int V, c
                     float temperature, float* loss, void* grad, long long ldg, void* ws,
                     hipStream_t stream);
 
+/* After one of those with a 16-bit gradient (dtype 0, 2), for a caller that has factors by[r * step] for the rows afterwards: the rows of grad
+ * whose factor is not 1 are written again, from the same logits and with weight times the factor, rounded to the logits'
+ * type once; the others are not touched. grad must not be NULL nor overlap the logits. ws as above; returns as those. */
+int rlu_policy_grad_by(const void* logits, int dtype, long long ld, int R, int V, const void* tokens,
+                       int wide, const float* old_logprobs, const float* advantages,
+                       const float* ref_logprobs, const float* weight, float clip_low,
+                       float clip_high, float kl, float temperature, const float* by, long long step,
+                       void* grad, long long ldg, void* ws, hipStream_t stream);
+int rlu_distill_top_grad_by(const void* logits, int dtype, long long ld, int R, int V,
+                            const int* top_ids, const float* top_logprobs, int top, int rest,
+                            const float* weight, float temperature, const float* by, long long step,
+                            void* grad, long long ldg, void* ws, hipStream_t stream);
+
 /* x [R, V] (dtype and rows as the gradient's above) times by[r * step] in place, row by row; rows whose factor
  * is 1 are not touched. Returns -1, -4 as those. */
 int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* by,

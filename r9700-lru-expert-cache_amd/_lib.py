@@ -44,6 +44,8 @@ SIGNATURES: dict[str, tuple] = {
     "rlu_loss_workspace": (_I, [_I] * 4 + [_P]),
     "rlu_policy_loss": (_I, [_P, _I, _LL, _I, _I, _P, _I] + [_P] * 4 + [_F] * 4 + [_P] * 3 + [_LL, _P, _P]),
     "rlu_distill_top": (_I, [_P, _I, _LL, _I, _I, _P, _P, _I, _I, _P, _F, _P, _P, _LL, _P, _P]),
+    "rlu_policy_grad_by": (_I, [_P, _I, _LL, _I, _I, _P, _I] + [_P] * 4 + [_F] * 4 + [_P, _LL, _P, _LL, _P, _P]),
+    "rlu_distill_top_grad_by": (_I, [_P, _I, _LL, _I, _I, _P, _P, _I, _I, _P, _F, _P, _LL, _P, _LL, _P, _P]),
     "rlu_scale_rows": (_I, [_P, _I, _LL, _I, _I, _P, _LL, _P]),
     "rlu_lora_plan": (_I, [_P] + [_I] * 5 + [_P] * 4),
     "rlu_lora_add": (_I, [_P, _LL, _P, _P, _P, _I, _P, _P, _P] + [_I] * 7 + [_P, _P, _LL, _P, _LL, _P]),

@@ -27,7 +27,6 @@ namespace rlu {
 namespace loss {
 
 using lp::Elem;
-using lp::L2E;
 using lp::lane_f;
 using lp::load_one;
 using lp::Max;
@@ -38,6 +37,7 @@ using lp::wave_max;
 
 constexpr int MAX_TOP = 32, MAX_V = 500000;
 constexpr int MOST_NW = 16;
+constexpr double LOG2_E = 1.44269504088896340736;
 
 // Threads of a workgroup, and the vectors of 16 bytes that each of them takes at a time.
 template <int THREADS, int VECTORS>
@@ -62,6 +62,8 @@ struct Args {
   float *loss, *logprob;
   uint8_t* grad;
   long long ldg;
+  const float* by;                         // null, or [R] step apart: the gradient alone, of rows whose factor is not 1
+  long long step;
 };
 
 // A row's workgroup (Wide: of long float32 rows), and a segment's. (4096 bf16 rows of 151936 with 256 threads 556 us, 517 with
@@ -289,7 +291,7 @@ __device__ __forceinline__ Coef policy(const Args& a, Part u, float x, int row, 
   }
   if (loss != loss) g = nan;
   const float f = none && !bad ? 0.f : weight * g * a.inv_t / z;
-  if (store && threadIdx.x == 0) {
+  if (store && a.loss && threadIdx.x == 0) {
     a.loss[row] = weight * loss;
     a.logprob[row] = lp;
   }
@@ -351,7 +353,7 @@ __device__ __forceinline__ Coef distill(const Args& a, Part u, float x, float v,
     loss += left * (logf(left) - ((u.m - m) * a.inv_t + logf(u.s) - ln_z));
   if (none) loss = wave_add(q) > 0.f ? inf : 0.f;
   if (bad) loss = nan;
-  if (store && threadIdx.x == 0) a.loss[row] = weight * loss;
+  if (store && a.loss && threadIdx.x == 0) a.loss[row] = weight * loss;
   const float w = (bad ? nan : weight) * a.inv_t;
   if (threadIdx.x < (unsigned)a.top) l.grad[lane] = none ? 0.f * w : w * (total * e / z - own);
   // relative to the unlisted logits' own maximum: their share of z may be below the smallest float
@@ -439,6 +441,12 @@ __device__ __forceinline__ void clear(const Args& a, const Row& r, int row, int 
   }
 }
 
+// A row whose gradient stays as it is. (A float32 gradient is multiplied: by is for 16 bits.)
+template <int DT>
+__device__ __forceinline__ bool done(const Args& a, int row) {
+  return Elem<DT>::SIZE == 2 && a.by && a.by[row * a.step] == 1.f;
+}
+
 // What the threads of a row know of what it lists.
 struct Own {
   float x, v, weight;                      // of the lane's listed token
@@ -454,6 +462,10 @@ __device__ __forceinline__ Own listed(const Args& a, const Row& r, int row, cons
                                     : (long long)((const int*)a.ids)[(size_t)row * top + lane];
   o.bad = __ballot(id >= a.V);
   o.skip = o.weight == 0.f || (OP == POLICY && __ballot(id >= 0) == 0);
+  if (Elem<DT>::SIZE == 2 && a.by) {       // (before the rounding to the logits' type)
+    o.weight *= a.by[row * a.step];
+    o.skip |= o.weight == 0.f;
+  }
   o.id = id >= 0 && id < a.V ? (int)id : -1;
   float v = 0.f;
   if (OP == DISTILL && lane < top) v = a.vals[(size_t)row * top + lane];
@@ -487,12 +499,13 @@ template <int DT, int OP, bool GRAD, class S>
 __global__ __launch_bounds__(S::NT, S::NT == Wide::NT ? 8 : 1) void row_k(Args a) {
   __shared__ Listed l;
   const int row = (int)blockIdx.x;
+  if (done<DT>(a, row)) return;
   const Row r = row_of<DT>(a, row);
   v4u raw[S::CV];
   load<DT, S, !GRAD>(raw, r, 0);
   const Own o = listed<DT, OP, S>(a, r, row, nullptr, l);
   if (o.skip) {
-    if (threadIdx.x == 0) {
+    if (a.loss && threadIdx.x == 0) {
       a.loss[row] = 0.f;
       if (OP == POLICY) a.logprob[row] = 0.f;
     }
@@ -513,6 +526,7 @@ __global__ __launch_bounds__(S::NT) void segment_k(Args a, Part* __restrict__ pa
                                                    float* __restrict__ xs) {
   __shared__ Listed l;
   const int row = (int)(blockIdx.x / (unsigned)a.nseg), seg = (int)(blockIdx.x % (unsigned)a.nseg);
+  if (done<DT>(a, row)) return;
   const Row r = row_of<DT>(a, row);
   const int len = ((r.nvec + S::CHUNK - 1) / S::CHUNK + a.nseg - 1) / a.nseg * S::CHUNK;
   const int v0 = min(seg * len, r.nvec), v1 = min(v0 + len, r.nvec);
@@ -532,6 +546,7 @@ __global__ __launch_bounds__(S::NT) void finish_k(Args a, const Part* __restrict
   __shared__ Listed l;
   const unsigned n = GRAD ? (unsigned)a.nseg : 1u;
   const int row = (int)(blockIdx.x / n), seg = (int)(blockIdx.x % n), lane = lane_id();
+  if (done<DT>(a, row)) return;
   const Row r = row_of<DT>(a, row);
   const int len = ((r.nvec + S::CHUNK - 1) / S::CHUNK + a.nseg - 1) / a.nseg * S::CHUNK;
   const int v0 = min(seg * len, r.nvec), v1 = min(v0 + len, r.nvec);
@@ -541,7 +556,7 @@ __global__ __launch_bounds__(S::NT) void finish_k(Args a, const Part* __restrict
   if (lane < a.nseg) u = parts[(size_t)row * a.nseg + lane];
   const Own o = listed<DT, OP, S>(a, r, row, xs, l);
   if (o.skip) {
-    if (seg == 0 && threadIdx.x == 0) {
+    if (a.loss && seg == 0 && threadIdx.x == 0) {
       a.loss[row] = 0.f;
       if (OP == POLICY) a.logprob[row] = 0.f;
     }
@@ -614,7 +629,8 @@ static int launch(Args a, int dtype, void* ws, hipStream_t stream) {
   long long bytes;
   if (check(a, dtype, &bytes) || a.ld < 0 || !(a.inv_t > 0.f) || !(a.k < __builtin_inff())) return -1;
   if (a.R == 0) return 0;
-  if (!a.logits || !a.loss || !ws) return -1;
+  if (a.by && dtype == 1) return -1;
+  if (!a.logits || !ws || !(a.by ? (const void*)a.grad : a.loss)) return -1;
   if (a.grad && a.R > 1 && a.ldg < a.V) return -1;
   if (((uintptr_t)a.logits | (uintptr_t)a.grad) % (dtype == 1 ? 4 : 2) || (uintptr_t)ws % 8) return -4;
   a.nseg = segments(dtype, a.R, a.V);
@@ -668,17 +684,12 @@ extern "C" int rlu_loss_workspace(int dtype, int R, int V, int top, long long* b
   return bytes ? rlu::loss::check(a, dtype, bytes) : -1;
 }
 
-extern "C" int rlu_policy_loss(const void* logits, int dtype, long long ld, int R, int V,
-                               const void* tokens, int wide, const float* old_logprobs,
-                               const float* advantages, const float* ref_logprobs,
-                               const float* weight, float clip_low, float clip_high, float kl,
-                               float temperature, float* loss, float* logprob, void* grad,
-                               long long ldg, void* ws, hipStream_t stream) {
-  using namespace rlu::loss;
+static int policy_args(rlu::loss::Args& a, const void* logits, long long ld, int R, int V, const void* tokens, int wide,
+                       const float* old_logprobs, const float* advantages, const float* ref_logprobs,
+                       const float* weight, float clip_low, float clip_high, float kl, float temperature) {
   if ((wide != 0 && wide != 1) || !(clip_low >= 0.f && clip_low <= 1.f) || !(clip_high >= 0.f)) return -1;
   if (!(temperature > 0.f) || !(kl >= 0.f && kl < __builtin_inff())) return -1;
-  if (R > 0 && (!tokens || !old_logprobs || !advantages || !logprob)) return -1;
-  Args a = {};
+  if (R > 0 && (!tokens || !old_logprobs || !advantages)) return -1;
   a.logits = (const uint8_t*)logits;
   a.ld = ld;
   a.R = R;
@@ -691,25 +702,50 @@ extern "C" int rlu_policy_loss(const void* logits, int dtype, long long ld, int 
   a.ref = kl != 0.f ? ref_logprobs : nullptr;
   a.weight = weight;
   a.inv_t = 1.f / temperature;
-  a.k = (float)(1.44269504088896340736 / temperature);
+  a.k = (float)(rlu::loss::LOG2_E / temperature);
   a.lo = 1.f - clip_low;
   a.hi = 1.f + clip_high;
   a.kl = kl;
+  return 0;
+}
+
+extern "C" int rlu_policy_loss(const void* logits, int dtype, long long ld, int R, int V,
+                               const void* tokens, int wide, const float* old_logprobs,
+                               const float* advantages, const float* ref_logprobs,
+                               const float* weight, float clip_low, float clip_high, float kl,
+                               float temperature, float* loss, float* logprob, void* grad,
+                               long long ldg, void* ws, hipStream_t stream) {
+  rlu::loss::Args a = {};
+  if (policy_args(a, logits, ld, R, V, tokens, wide, old_logprobs, advantages, ref_logprobs, weight, clip_low, clip_high,
+                  kl, temperature) || (R > 0 && !logprob))
+    return -1;
   a.loss = loss;
   a.logprob = logprob;
   a.grad = (uint8_t*)grad;
   a.ldg = ldg;
-  return launch<POLICY>(a, dtype, ws, stream);
+  return rlu::loss::launch<rlu::loss::POLICY>(a, dtype, ws, stream);
 }
 
-extern "C" int rlu_distill_top(const void* logits, int dtype, long long ld, int R, int V,
-                               const int* top_ids, const float* top_logprobs, int top, int rest,
-                               const float* weight, float temperature, float* loss, void* grad,
-                               long long ldg, void* ws, hipStream_t stream) {
-  using namespace rlu::loss;
+extern "C" int rlu_policy_grad_by(const void* logits, int dtype, long long ld, int R, int V, const void* tokens,
+                                  int wide, const float* old_logprobs, const float* advantages,
+                                  const float* ref_logprobs, const float* weight, float clip_low,
+                                  float clip_high, float kl, float temperature, const float* by,
+                                  long long step, void* grad, long long ldg, void* ws, hipStream_t stream) {
+  rlu::loss::Args a = {};
+  if (policy_args(a, logits, ld, R, V, tokens, wide, old_logprobs, advantages, ref_logprobs, weight, clip_low, clip_high,
+                  kl, temperature) || (R > 0 && !by))
+    return -1;
+  a.grad = (uint8_t*)grad;
+  a.ldg = ldg;
+  a.by = by;
+  a.step = step;
+  return rlu::loss::launch<rlu::loss::POLICY>(a, dtype, ws, stream);
+}
+
+static int distill_args(rlu::loss::Args& a, const void* logits, long long ld, int R, int V, const int* top_ids,
+                        const float* top_logprobs, int top, int rest, const float* weight, float temperature) {
   if ((rest != 0 && rest != 1) || !(temperature > 0.f)) return -1;
   if (R > 0 && (!top_ids || !top_logprobs)) return -1;
-  Args a = {};
   a.logits = (const uint8_t*)logits;
   a.ld = ld;
   a.R = R;
@@ -720,11 +756,34 @@ extern "C" int rlu_distill_top(const void* logits, int dtype, long long ld, int 
   a.rest = rest;
   a.weight = weight;
   a.inv_t = 1.f / temperature;
-  a.k = (float)(1.44269504088896340736 / temperature);
+  a.k = (float)(rlu::loss::LOG2_E / temperature);
+  return 0;
+}
+
+extern "C" int rlu_distill_top(const void* logits, int dtype, long long ld, int R, int V,
+                               const int* top_ids, const float* top_logprobs, int top, int rest,
+                               const float* weight, float temperature, float* loss, void* grad,
+                               long long ldg, void* ws, hipStream_t stream) {
+  rlu::loss::Args a = {};
+  if (distill_args(a, logits, ld, R, V, top_ids, top_logprobs, top, rest, weight, temperature)) return -1;
   a.loss = loss;
   a.grad = (uint8_t*)grad;
   a.ldg = ldg;
-  return launch<DISTILL>(a, dtype, ws, stream);
+  return rlu::loss::launch<rlu::loss::DISTILL>(a, dtype, ws, stream);
+}
+
+extern "C" int rlu_distill_top_grad_by(const void* logits, int dtype, long long ld, int R, int V, const int* top_ids,
+                                       const float* top_logprobs, int top, int rest, const float* weight,
+                                       float temperature, const float* by, long long step, void* grad,
+                                       long long ldg, void* ws, hipStream_t stream) {
+  rlu::loss::Args a = {};
+  if (distill_args(a, logits, ld, R, V, top_ids, top_logprobs, top, rest, weight, temperature) || (R > 0 && !by))
+    return -1;
+  a.grad = (uint8_t*)grad;
+  a.ldg = ldg;
+  a.by = by;
+  a.step = step;
+  return rlu::loss::launch<rlu::loss::DISTILL>(a, dtype, ws, stream);
 }
 
 extern "C" int rlu_scale_rows(void* x, int dtype, long long ld, int R, int V, const float* by,

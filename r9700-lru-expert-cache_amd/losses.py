@@ -84,23 +84,21 @@ def _check_out(name: str, out: torch.Tensor, logits: torch.Tensor) -> None:
         raise ValueError(f"{name}: out overlaps the logits (it may be the logits, or apart from them)")
 
 
-def _call(logits, grad, top, fn, before, after) -> torch.Tensor:
-    """Runs fn(logits ..., *before, loss, *after, grad ..., ws, stream); returns the loss."""
+def _call(logits, grad, top, fn, *args) -> None:
+    """Runs fn(logits ..., *args, grad ..., ws, stream)."""
     rows, vocab = logits.shape
     code, dev = _DTYPE_CODE[logits.dtype], logits.device
-    loss = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows == 0:
-        return loss
+        return
     # taken and given back on the current stream, as the outputs are: calls on two streams, or two
     # captured graphs, have their own
     ws = torch.empty(_workspace(code, rows, vocab, top), dtype=torch.uint8, device=dev)
     with on_device(dev):
         rc = getattr(lib(), fn)(
-            logits.data_ptr(), code, logits.stride()[0], rows, vocab, *before, loss.data_ptr(), *after,
+            logits.data_ptr(), code, logits.stride()[0], rows, vocab, *args,
             0 if grad is None else grad.data_ptr(),
             0 if grad is None else grad.stride()[0] if rows > 1 else vocab, ws.data_ptr(), stream_ptr())
     check(rc, fn)
-    return loss
 
 
 def _ptr(t) -> int:
@@ -108,20 +106,26 @@ def _ptr(t) -> int:
 
 
 def _policy(logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl, temperature,
-            grad) -> PolicyLoss:
-    logprob = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-    loss = _call(logits, grad, 1, "rlu_policy_loss",
-                 (tokens.data_ptr(), int(tokens.dtype == torch.int64), old_logprobs.data_ptr(),
-                  advantages.data_ptr(), _ptr(ref_logprobs), _ptr(weight), clip[0], clip[1], kl,
-                  temperature), (logprob.data_ptr(),))
+            grad, by=None) -> PolicyLoss | None:
+    """by: factors of rows whose gradient is in grad already; the others are written again, and nothing else."""
+    args = (tokens.data_ptr(), int(tokens.dtype == torch.int64), old_logprobs.data_ptr(), advantages.data_ptr(),
+            _ptr(ref_logprobs), _ptr(weight), clip[0], clip[1], kl, temperature)
+    if by is not None:
+        return _call(logits, grad, 1, "rlu_policy_grad_by", *args, by.data_ptr(), by.stride(0))
+    loss, logprob = (torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device) for _ in range(2))
+    _call(logits, grad, 1, "rlu_policy_loss", *args, loss.data_ptr(), logprob.data_ptr())
     return PolicyLoss(loss, logprob)
 
 
-def _distill(logits, top_ids, top_logprobs, weight, rest, temperature, grad) -> torch.Tensor:
+def _distill(logits, top_ids, top_logprobs, weight, rest, temperature, grad, by=None) -> torch.Tensor | None:
+    """by: as for _policy."""
     top = top_ids.shape[1]
-    return _call(logits, grad, top, "rlu_distill_top",
-                 (top_ids.data_ptr(), top_logprobs.data_ptr(), top, int(rest), _ptr(weight),
-                  temperature), ())
+    args = (top_ids.data_ptr(), top_logprobs.data_ptr(), top, int(rest), _ptr(weight), temperature)
+    if by is not None:
+        return _call(logits, grad, top, "rlu_distill_top_grad_by", *args, by.data_ptr(), by.stride(0))
+    loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+    _call(logits, grad, top, "rlu_distill_top", *args, loss.data_ptr())
+    return loss
 
 
 def _check_temperature(name: str, temperature) -> None:
@@ -206,13 +210,17 @@ def distill_top_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: 
 # ---- for autograd -------------------------------------------------------------------------------
 class _Rows(torch.autograd.Function):
     """The rows' losses. Their gradient is made in the forward pass, which has the logits in the cache, and
-    handed out once."""
+    handed out once. An incoming factor other than 1 belongs in front of the rounding to 16 bits (float16 has nothing
+    below 6e-8 for a loss scale to lift again): such rows are then worked out again from the logits. Float32's are
+    multiplied."""
 
     @staticmethod
-    def forward(ctx, logits, loss_of):
+    def forward(ctx, logits, op, beside, *how):
         grad = _grad_like(logits)
-        out = loss_of(logits, grad)
-        ctx.grad = grad
+        out = op(logits, *beside, *how, grad)
+        ctx.grad, ctx.op, ctx.how = grad, op, how
+        if grad.element_size() == 2:
+            ctx.save_for_backward(logits, *beside)
         if isinstance(out, PolicyLoss):
             ctx.mark_non_differentiable(out.logprob)
             return tuple(out)
@@ -227,14 +235,17 @@ class _Rows(torch.autograd.Function):
         if grad is None:
             raise RuntimeError("a loss's gradient is handed out once: compute the loss again for a "
                                "second backward pass")
-        if grad.numel():
+        none = (None,) * (2 + len(ctx.how))
+        if grad.element_size() == 2:
+            ctx.op(*ctx.saved_tensors, *ctx.how, grad, by)           # (refuses logits written to since)
+        elif grad.numel():
             rows, vocab = grad.shape
             with on_device(grad.device):
                 rc = lib().rlu_scale_rows(
                     grad.data_ptr(), _DTYPE_CODE[grad.dtype], grad.stride(0) if rows > 1 else vocab,
                     rows, vocab, by.data_ptr(), by.stride(0), stream_ptr())
             check(rc, "rlu_scale_rows")
-        return grad, None
+        return (grad, *none)
 
 
 def _differentiable(name: str, logits: torch.Tensor) -> bool:
@@ -258,15 +269,17 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: torch.
 
     A negative token (a padded row) or a weight of 0 gives 0 and no gradient; the logits of such a row may be
     anything. A token past the vocabulary, a NaN or +inf give NaN. A token at -inf has rho = 0, and with a KL term
-    an infinite loss. The factor of a mean belongs into weight: a gradient that comes in as 1 costs nothing, any
-    other one more pass. Backward runs once a loss."""
+    an infinite loss. A gradient that comes in as 1 (the factors of a mean in weight, the rows' sum) costs nothing; any other
+    one more pass, in which 16-bit rows are worked out again with it, so that a loss scale meets the gradient before its
+    rounding: autograd keeps 16-bit logits until then, and refuses a backward pass if they or the other inputs have been
+    written to. Backward runs once a loss."""
     _check_policy("policy_loss", logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip,
                   kl, temperature)
     if not _differentiable("policy_loss", logits):
         return _policy(logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
                        temperature, None)
-    return PolicyLoss(*_Rows.apply(logits, lambda x, grad: _policy(
-        x, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl, temperature, grad)))
+    return PolicyLoss(*_Rows.apply(logits, _policy, (tokens, old_logprobs, advantages, ref_logprobs, weight), clip, kl,
+                                   temperature))
 
 
 def distill_top(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch.Tensor,
@@ -288,5 +301,4 @@ def distill_top(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch
     _check_distill("distill_top", logits, top_ids, top_logprobs, weight, temperature)
     if not _differentiable("distill_top", logits):
         return _distill(logits, top_ids, top_logprobs, weight, rest, temperature, None)
-    return _Rows.apply(logits, lambda x, grad: _distill(x, top_ids, top_logprobs, weight, rest,
-                                                        temperature, grad))
+    return _Rows.apply(logits, _distill, (top_ids, top_logprobs, weight), rest, temperature)

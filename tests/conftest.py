@@ -27,7 +27,10 @@ def load_pkg():
 # they are and are expected to fail there; what is right is tested in the file that the reason names.
 NOTHING_LEFT = ("rows where no token is left for the teacher's rest: the expected gradient p - q is not that of the expected "
                 "loss, which lacks the rest's term (tests/test_gpu_losses_nothing_left.py)")
+ROUNDED_TWICE = ("a 16-bit gradient under an incoming factor: expected is the rounded gradient times the factor, rounded again, "
+                 "in place of the product rounded once (tests/test_gpu_losses_factor.py)")
 WRONG_VALUES = {
+    "test_gpu_losses.py::test_autograd": (lambda p: p["dtype"] != "f32", ROUNDED_TWICE),
     "test_gpu_losses.py::test_masked_rows": (lambda p: True, NOTHING_LEFT),
     "test_gpu_losses.py::test_distill": (lambda p: p["V"] in (1, 2, 5, 9), NOTHING_LEFT),
 }
