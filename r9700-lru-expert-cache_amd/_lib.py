@@ -125,6 +125,16 @@ def written(t) -> None:
     torch.autograd.graph.increment_version(t)
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether one of them is a dual tensor of forward-mode differentiation. It does not require a gradient and its
+    address reads as any other's, so a kernel's result would go without a tangent and say nothing."""
+    import torch
+    forward = torch.autograd.forward_ad
+    if getattr(forward, "_current_level", 0) < 0:      # (outside of every dual_level, as nearly always: 0.1 us)
+        return False
+    return any(t is not None and forward.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed rc={rc}")

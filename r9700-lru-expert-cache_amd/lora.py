@@ -16,7 +16,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, lib, on_device, stream_ptr, written
+from ._lib import check, has_tangent, lib, on_device, stream_ptr, written
 
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 2}
 MAX_RANK = 128
@@ -109,7 +109,8 @@ def _check_batch(name: str, w: LoraStack, rows: LoraRows) -> None:
 
 def _check_hidden(name: str, hidden: torch.Tensor, rows: int, w: LoraStack) -> None:
     if hidden.shape != (rows, w.rank) or hidden.dtype != torch.float32 or \
-            not hidden.is_contiguous() or hidden.device != w.a.device or hidden.requires_grad:
+            not hidden.is_contiguous() or hidden.device != w.a.device or hidden.requires_grad or \
+            has_tangent(hidden):
         raise ValueError(f"{name}: hidden must be contiguous float32 [{rows}, {w.rank}] beside the adapters")
 
 
@@ -155,6 +156,8 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
     _check_rows("add_lora", "y", y, M, b.shape[1], w)
     if hidden is not None:
         _check_hidden("add_lora", hidden, M, w)
+    if has_tangent(y, x, a, b, w.scale, out):
+        raise ValueError("add_lora has no forward-mode derivative")
     grad = (x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad) and \
         torch.is_grad_enabled()
     if grad and (out is not None or hidden is not None):
@@ -230,6 +233,8 @@ def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRow
     if (dy.requires_grad or x.requires_grad or w.a.requires_grad or w.b.requires_grad) and \
             torch.is_grad_enabled():
         raise ValueError("add_lora_grad returns the gradients itself: detach its operands")
+    if has_tangent(dy, x, w.a, w.b, w.scale):
+        raise ValueError("add_lora_grad has no forward-mode derivative")
     return _backward(dy, x, w, rows, hidden, need)
 
 

@@ -16,7 +16,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import check, lib, on_device, stream_ptr, written
+from ._lib import check, has_tangent, lib, on_device, stream_ptr, written
 from .logprobs import _DTYPE_CODE, MAX_VOCAB
 
 MAX_TOP = 32
@@ -42,13 +42,15 @@ def _check_logits(name: str, logits: torch.Tensor) -> None:
         raise ValueError(f"{name}: a vocabulary of {vocab} is outside 1..{MAX_VOCAB}")
     if vocab > 1 and logits.stride()[1] != 1:
         raise ValueError(f"{name}: a row's logits must lie next to each other")
+    if has_tangent(logits):
+        raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _check_beside(name: str, what: str, t, shape, dtypes, dev) -> None:
     if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{name}: {what} must be contiguous {' or '.join(str(d)[6:] for d in dtypes)} "
                          f"{list(shape)} beside the logits")
-    if t.requires_grad and torch.is_grad_enabled():
+    if (t.requires_grad and torch.is_grad_enabled()) or has_tangent(t):
         raise ValueError(f"{name} has no gradient of {what}: detach it")
 
 
@@ -73,7 +75,7 @@ def _check_out(name: str, out: torch.Tensor, logits: torch.Tensor) -> None:
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
             (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
         raise ValueError(f"{name}: out must be {logits.dtype} [{rows}, {vocab}] beside the logits, its rows apart")
-    if out.requires_grad and torch.is_grad_enabled():
+    if (out.requires_grad and torch.is_grad_enabled()) or has_tangent(out):
         raise ValueError(f"{name}: out asks for a gradient")
     a, b = logits.data_ptr(), out.data_ptr()
     if a == b and (rows < 2 or logits.stride(0) == out.stride(0)):
