@@ -114,15 +114,13 @@ def _check_hidden(name: str, hidden: torch.Tensor, rows: int, w: LoraStack) -> N
         raise ValueError(f"{name}: hidden must be contiguous float32 [{rows}, {w.rank}] beside the adapters")
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """The bytes that t's rows reach over."""
-    size, (rows, cols) = t.element_size(), t.shape
-    return t.data_ptr(), t.data_ptr() + ((rows - 1) * t.stride(0) + cols) * size if rows else t.data_ptr()
-
-
 def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
-    (a, b), (c, d) = _span(s), _span(t)
-    return a < d and c < b
+    """Whether the bytes that their rows reach over meet: the one that begins first ends behind the other's beginning."""
+    a, b = s.data_ptr(), t.data_ptr()
+    if a > b:
+        a, b, s, t = b, a, t, s
+    rows, cols = s.shape
+    return rows > 0 and t.shape[0] > 0 and a + ((rows - 1) * s.stride(0) + cols) * s.element_size() > b
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -172,12 +170,20 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
         same = out.data_ptr() == y.data_ptr() and _ld(out) == _ld(y)
         if (not same and _overlap(out, y)) or _overlap(out, x):
             raise ValueError("add_lora: out overlaps y or x (it may be y, or apart from both)")
+    if hidden is not None and M:
+        at = hidden.data_ptr()
+        for t in (x, y, out):                          # (_overlap, without asking for what is known: a small step's time)
+            if t is not None and t.data_ptr() < at + 4 * M * w.rank and \
+                    at < t.data_ptr() + 2 * ((M - 1) * t.stride()[0] + t.shape[1]):
+                raise ValueError("add_lora: hidden overlaps x, y or out")
     if grad:
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("add_lora: a captured graph takes add_lora_grad, without autograd")
         return _AddLora.apply(y, x, a, b, w, rows)
     if hidden is None:
         hidden = torch.empty(M * a.shape[1], dtype=torch.float32, device=x.device)
+    else:
+        written(hidden)
     if out is None:
         out = torch.empty(M, b.shape[1], dtype=y.dtype, device=y.device)
     else:
