@@ -130,7 +130,7 @@ def has_tangent(*tensors) -> bool:
     address reads as any other's, so a kernel's result would go without a tangent and say nothing."""
     import torch
     forward = torch.autograd.forward_ad
-    if getattr(forward, "_current_level", 0) < 0:      # (outside of every dual_level, as nearly always: 0.1 us)
+    if getattr(forward, "_current_level", 0) < 0:      # outside of every dual_level (a torch that lacks it: looks)
         return False
     return any(t is not None and forward.unpack_dual(t).tangent is not None for t in tensors)
 

@@ -109,8 +109,7 @@ def _check_batch(name: str, w: LoraStack, rows: LoraRows) -> None:
 
 def _check_hidden(name: str, hidden: torch.Tensor, rows: int, w: LoraStack) -> None:
     if hidden.shape != (rows, w.rank) or hidden.dtype != torch.float32 or \
-            not hidden.is_contiguous() or hidden.device != w.a.device or hidden.requires_grad or \
-            has_tangent(hidden):
+            not hidden.is_contiguous() or hidden.device != w.a.device or hidden.requires_grad:
         raise ValueError(f"{name}: hidden must be contiguous float32 [{rows}, {w.rank}] beside the adapters")
 
 
@@ -154,7 +153,7 @@ def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
     _check_rows("add_lora", "y", y, M, b.shape[1], w)
     if hidden is not None:
         _check_hidden("add_lora", hidden, M, w)
-    if has_tangent(y, x, a, b, w.scale, out):
+    if has_tangent(y, x, a, b, w.scale, out, hidden):
         raise ValueError("add_lora has no forward-mode derivative")
     grad = (x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad) and \
         torch.is_grad_enabled()
@@ -239,7 +238,7 @@ def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRow
     if (dy.requires_grad or x.requires_grad or w.a.requires_grad or w.b.requires_grad) and \
             torch.is_grad_enabled():
         raise ValueError("add_lora_grad returns the gradients itself: detach its operands")
-    if has_tangent(dy, x, w.a, w.b, w.scale):
+    if has_tangent(dy, x, w.a, w.b, w.scale, hidden):
         raise ValueError("add_lora_grad has no forward-mode derivative")
     return _backward(dy, x, w, rows, hidden, need)
 

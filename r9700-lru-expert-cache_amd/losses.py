@@ -42,15 +42,13 @@ def _check_logits(name: str, logits: torch.Tensor) -> None:
         raise ValueError(f"{name}: a vocabulary of {vocab} is outside 1..{MAX_VOCAB}")
     if vocab > 1 and logits.stride()[1] != 1:
         raise ValueError(f"{name}: a row's logits must lie next to each other")
-    if has_tangent(logits):
-        raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _check_beside(name: str, what: str, t, shape, dtypes, dev) -> None:
     if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous() or t.device != dev:
         raise ValueError(f"{name}: {what} must be contiguous {' or '.join(str(d)[6:] for d in dtypes)} "
                          f"{list(shape)} beside the logits")
-    if (t.requires_grad and torch.is_grad_enabled()) or has_tangent(t):
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient of {what}: detach it")
 
 
@@ -75,7 +73,7 @@ def _check_out(name: str, out: torch.Tensor, logits: torch.Tensor) -> None:
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device or \
             (vocab > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < vocab):
         raise ValueError(f"{name}: out must be {logits.dtype} [{rows}, {vocab}] beside the logits, its rows apart")
-    if (out.requires_grad and torch.is_grad_enabled()) or has_tangent(out):
+    if out.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name}: out asks for a gradient")
     a, b = logits.data_ptr(), out.data_ptr()
     if a == b and (rows < 2 or logits.stride(0) == out.stride(0)):
@@ -114,7 +112,9 @@ def _policy(logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip
             _ptr(ref_logprobs), _ptr(weight), clip[0], clip[1], kl, temperature)
     if by is not None:
         return _call(logits, grad, 1, "rlu_policy_grad_by", *args, by.data_ptr(), by.stride(0))
-    loss, logprob = (torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device) for _ in range(2))
+    rows, dev = logits.shape[0], logits.device
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
     _call(logits, grad, 1, "rlu_policy_loss", *args, loss.data_ptr(), logprob.data_ptr())
     return PolicyLoss(loss, logprob)
 
@@ -136,7 +136,7 @@ def _check_temperature(name: str, temperature) -> None:
 
 
 def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
-                  temperature) -> None:
+                  temperature, out=None) -> None:
     _check_logits(name, logits)
     rows, dev = (logits.shape[0],), logits.device
     _check_beside(name, "tokens", tokens, rows, _IDS, dev)
@@ -153,9 +153,11 @@ def _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, 
     if kl and ref_logprobs is None:
         raise ValueError(f"{name}: kl={kl} needs ref_logprobs")
     _check_temperature(name, temperature)
+    if has_tangent(logits, old_logprobs, advantages, ref_logprobs, weight, out):
+        raise ValueError(f"{name} has no forward-mode derivative")
 
 
-def _check_distill(name, logits, top_ids, top_logprobs, weight, temperature) -> None:
+def _check_distill(name, logits, top_ids, top_logprobs, weight, temperature, out=None) -> None:
     _check_logits(name, logits)
     rows, dev = logits.shape[0], logits.device
     if top_ids.ndim != 2 or top_ids.shape[0] != rows or not 1 <= top_ids.shape[1] <= MAX_TOP:
@@ -165,6 +167,8 @@ def _check_distill(name, logits, top_ids, top_logprobs, weight, temperature) -> 
     if weight is not None:
         _check_beside(name, "weight", weight, (rows,), _F32, dev)
     _check_temperature(name, temperature)
+    if has_tangent(logits, top_logprobs, weight, out):
+        raise ValueError(f"{name} has no forward-mode derivative")
 
 
 def _by_hand(name: str, logits: torch.Tensor) -> None:
@@ -181,7 +185,7 @@ def policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: t
     may be the logits themselves."""
     name = "policy_loss_grad"
     _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
-                  temperature)
+                  temperature, out)
     _by_hand(name, logits)
     if out is None:
         out = _grad_like(logits)
@@ -199,7 +203,7 @@ def distill_top_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: 
     """distill_top and the gradient of the rows' sum, [R, V] of the logits' type: into out where given, which
     may be the logits themselves."""
     name = "distill_top_grad"
-    _check_distill(name, logits, top_ids, top_logprobs, weight, temperature)
+    _check_distill(name, logits, top_ids, top_logprobs, weight, temperature, out)
     _by_hand(name, logits)
     if out is None:
         out = _grad_like(logits)
