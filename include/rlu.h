@@ -370,7 +370,8 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
  *     probability the last has no term. grad of a listed token: p - q, or sum(q) p - q in such a row and where the sum
  *     is over 1 + 2^-16.
  *     rest 0: q = softmax(top_logprobs / temperature) over the listed, which may be logits.
- *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf: NaN throughout.
+ *   -inf logits have probability 0. A row of nothing else: gradient 0; a row with a NaN or +inf, or a q that is not
+ *   finite: NaN throughout.
  * 0 <= clip_low <= 1, clip_high >= 0, 0 <= kl < inf, temperature > 0 and 1 / temperature finite, 1 <= top <= 32. ws:
  * what the first call says (top 1 for the policy loss), 8-byte aligned, used until the call's kernels end.
  * R = 0 launches nothing. Returns -1 (bad sizes or arguments, more than 2^22 - 1 workgroups, or a NULL pointer),

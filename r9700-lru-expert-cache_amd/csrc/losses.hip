@@ -340,7 +340,7 @@ __device__ __forceinline__ Coef distill(const Args& a, Part u, float x, float v,
     for (int j = 0; j < a.top; ++j) own += alike >> j & 1 && j != lane ? lane_f(q, j) : 0.f;
   }
   const float xm = wave_max(in ? x : -inf), m = fmaxf(u.m, xm);
-  bad |= m == inf || __ballot(in && q != q);
+  bad |= m == inf || __ballot(in && !(q < inf));
   const bool none = m == -inf;
   const float e = none || !in ? 0.f : __builtin_amdgcn_exp2f((x - m) * a.k);
   const float rest = join(u, m, a.k).s;

@@ -299,7 +299,8 @@ def distill_top(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: torch
                   loss = sum q_j ln(q_j / p_j) + q_rest ln(q_rest / p_rest)
       not rest    q = softmax(top_logprobs / temperature) over the listed (logits will do): sum q_j ln(q_j / p_j)
 
-    A negative id is none, with its value. One past the vocabulary, a NaN or +inf give a row of NaN. A weight of 0
+    A negative id is none, with its value. One past the vocabulary, a NaN or +inf among the logits or the values that
+    count, or (rest) a value whose exponential float32 does not hold, give a row of NaN. A weight of 0
     gives 0 and no gradient; the logits of such a row may be anything. An id listed twice has a term for each. Where
     probabilities sum to 1 or more there is no rest (and in the gradient an excess of up to 2^-16 is rounding). Where
     no token is left for the rest, as all are listed or those that are not are at -inf, its term is left out of the
