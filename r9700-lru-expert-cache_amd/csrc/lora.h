@@ -55,12 +55,7 @@ __device__ __forceinline__ uint32_t to_bits(float f) {
 // Two of them in one word.
 template <int DT>
 __device__ __forceinline__ uint32_t to_bits2(float a, float b) {
-  if (DT == 0) {
-    uint32_t r;
-    asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-  }
-  return to_bits<DT>(a) | to_bits<DT>(b) << 16;
+  return DT == 0 ? f32x2_to_bf16(a, b) : to_bits<DT>(a) | to_bits<DT>(b) << 16;
 }
 
 // n elements at p (8 or more: eight of them), zeros behind: p at any element's address. ONCE: nobody asks

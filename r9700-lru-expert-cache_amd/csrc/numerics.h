@@ -37,6 +37,13 @@ __device__ __forceinline__ uint16_t f32_to_bf16_hw(float f) {
   return (uint16_t)r;
 }
 
+// Two of them in one word, a the lower.
+__device__ __forceinline__ uint32_t f32x2_to_bf16(float a, float b) {
+  uint32_t r;
+  asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // two float32 -> two e4m3fn bytes (nearest-even), packed in the low 16 bits. Inputs are
 // already clamped to +-448 by every caller, so saturation behaviour never comes into play.
 __device__ __forceinline__ uint32_t f32x2_to_e4m3(float a, float b) {
