@@ -359,7 +359,8 @@ int rlu_token_logprobs(const void* logits, int dtype, long long ld, int R, int V
  * rlu_token_logprobs) a loss and, where grad is not NULL, the gradient of the losses' sum: [R, V] of the
  * logits' type, rows ldg elements apart (>= V), at any element's address, nothing written beside them; it may be
  * the logits themselves (same address and ld), but must not overlap them otherwise. p = softmax(x / temperature),
- * weight [R] f32 or NULL (1). A row of weight 0 is not read: loss, log probability and gradient are 0.
+ * weight [R] f32 or NULL (1). Of a row of weight 0 nothing that is read matters (its memory must be there all the
+ * same): loss, log probability and gradient are 0.
  *   policy_loss: lp = ln p of the row's token (int64 if wide 1, int32 if 0), rho = e^(lp - old), adv its advantage,
  *     loss = weight (-min(rho adv, clamp(rho, 1 - clip_low, 1 + clip_high) adv) + kl (e^(ref - lp) - (ref - lp) - 1)),
  *     without the last term where kl is 0 or ref_logprobs NULL. Also lp itself, [R]. A token below 0 is none (a

@@ -127,7 +127,10 @@ __device__ __forceinline__ float scale_to(float m) {
 }
 
 // f as the sum of 16-bit values, the largest first, for products with 16-bit ones: all of its 24 bits in three of bf16; in
-// two of float16 22, half a step of which is 2^-23 of f, no more than one addition of the float32 sums around it may lose.
+// two of float16 22, half a step of which is 2^-23 of f, no more than two additions of the float32 sums around it may lose.
+// (bf16 in two parts, 16 bits, left 1.2e-4 between lora_1's outputs and what float32 rounds to, 9e-8 in three. The third one's cost, us:
+// 8192 rows of [2560 -> 10240] in any order, R = 64 expand 81 -> 85, outer 95 -> 108, R = 128 121 -> 145 and 154 -> 175; R = 16
+// 1 to 2%, dx with dA 25 -> 28)
 template <int DT>
 struct Split {
   static constexpr int N = DT == 0 ? 3 : 2;
@@ -205,10 +208,11 @@ __device__ __forceinline__ void stage(Rows<DT, MT, KS>& s, int count, int R, At 
 // A workgroup a tile (or 16 MT of its rows) and a strip of columns, a wave 64 columns at a time: W's part of them as it
 // lies in memory through LDS into registers, then 16 rows after the other. Sums leave the matrix unit with a lane's
 // neighbour another row; through LDS they come in rows of 128 bytes, as y and out are read and written.
-// Bound by y read and out written: 8192 x 10240, R = 64 71 - 74 us, 4.6 TB/s; 1024 x 151936, R = 16 116 us, 5.4 TB/s; 160 x
-// 151936, R = 16, 32 adapters 51 - 52 us, 4.9 TB/s with their 156 MB. The matrix unit is busy for 12% of the cycles, LDS for
-// 25%. At 8192 x 10240: 150 us with h's eight values loaded one by one, 112 by 16 bytes, 97 with W through LDS, 77 with the sums
-// through it, 74 with y and out past the cache.
+// Bound by y read and out written: 8192 x 10240, R = 64 77 - 80 us, 4.4 TB/s; 1024 x 151936, R = 16 117 - 120 us, 5.3 TB/s; 160 x
+// 151936, R = 16, 32 adapters 53 - 54 us, 4.7 TB/s with their 156 MB. The matrix unit is busy for 17% of the cycles, LDS for
+// 28%. R over 64: 143 us at 8192 x 10240, as W's and h's 122 KB of LDS leave a CU one workgroup. At 8192 x 10240, R = 64, with h
+// in two parts: 150 us with h's eight values loaded one by one, 112 by 16 bytes, 97 with W through LDS, 77 with the sums through
+// it, 74 with y and out past the cache.
 struct Out {
   const uint16_t *w, *y;
   long long ldy;

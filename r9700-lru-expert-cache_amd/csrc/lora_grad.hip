@@ -4,9 +4,11 @@
 // they lie in memory: their tiles go through LDS as they are and are read transposed. h and u take part as sums of 16-bit
 // values each (Split).
 //
-// Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 79 - 83 us for u and dB, then 10 for u over the strips, 8 for dx,
-// dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 46 + 8 + 26 + 5, R = 64 83 - 91 + 16 + 48 + 7, where the
-// registers leave two workgroups a CU. 96 x 2560 x 2560 with one adapter: 7, 3, 4 us, each launch a chain of a few loads.
+// Bound by dy: 1024 x 151936, R = 16, 2 adapters (dy 311 MB) 79 - 83 us for u and dB, then 10 for u over the strips, 9 for dx,
+// dA and dB's parts, 4 for dA's. 8192 x [2560 -> 10240], 8 adapters: R = 16 48 + 8 + 28 + 5, R = 64 103 - 109 + 16 + 51 + 7, where the
+// registers leave two workgroups a CU, R = 128 175 + 33 + 43 + 55 + 8, where dy and x are read for 64 ranks at a time. u's parts, R
+// floats a row for each 256 columns, are R / 128 of dy's own bytes, written and read again. 96 x 2560 x 2560 with one adapter: 7, 3,
+// 5 us, each launch a chain of a few loads.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -442,7 +444,7 @@ static void backward(const Bwd& f, const Last& l, hipStream_t stream) {
       RLU_LAST(MT, 2, 1, l);                                                                    \
     } else if (f.R <= 64) {                                                                     \
       RLU_LAST(MT, 4, 2, l);                                                                    \
-    } else { /* (dx's 108 KB of LDS would leave dA one workgroup a CU: 531 us, 450 apart) */        \
+    } else { /* (dx's 123 KB of LDS would leave dA one workgroup a CU: 531 us, 450 apart) */        \
       Last dx = l, rest = l;                                                                    \
       dx.da = dx.joins = rest.dx = 0;                                                           \
       if (dx.dx) RLU_LAST(MT, 4, 4, dx);                                                        \

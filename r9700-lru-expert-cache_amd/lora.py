@@ -2,7 +2,9 @@
 adapter that its request asks for, out = y + s (x A^T) B^T, and the backward pass that trains them.
 
 No counterpart in the reference. The projection itself is whatever gave y: ops.gemm_fp8_dense, the heads, or
-any product of the caller's; rows, adapters and outputs are bf16 or f16.
+any product of the caller's; rows, adapters and outputs are bf16 or f16. The backward pass is the adapters' alone: what the
+frozen projection adds to dx, dy times its weight, is the caller's. ops.gemm_fp8_dense has no gradient and no product with
+the transposed weight, so in this package training reaches the adapters of a model's last product, the head.
 
   plan_rows      a batch's rows by adapter: once, for all the projections that the batch passes
   add_lora       for serving (in place or into another tensor), and for autograd in eager code
@@ -79,9 +81,11 @@ def plan_rows(ids: torch.Tensor, n: int) -> LoraRows:
     rows, dev = ids.shape[0], ids.device
     if rows > 1 << 24:
         raise ValueError(f"plan_rows: {rows} rows, at most {1 << 24}")
-    # few rows: tiles of 16 (most adapters have fewer); many: an adapter's factors are read once for 64. [2560 -> 10240], R =
+    # few rows: tiles of 16 (many adapters have fewer); many: an adapter's factors are read once for 64. [2560 -> 10240], R =
     # 16, 8 adapters, tiles of 16 / 64, us forward and backward: 256 rows 9.8 + 19.7 / 11.0 + 16.1, 1023 18.2 + 37.1 / 17.1
-    # + 33.9, 2048 30.9 + 50.4 / 25.8 + 44.5; 1023 rows of 64 adapters, [2560 -> 2560] 11.5 + 27.2 / 12.6 + 27.3
+    # + 33.9, 2048 30.9 + 50.4 / 25.8 + 44.5; 1023 rows of 64 adapters, [2560 -> 2560] 11.5 + 27.2 / 12.6 + 27.3. The rule goes by
+    # the rows alone: below 1024 the forward pass of few rows and batches of many adapters gain, the backward pass of few
+    # adapters loses, 8% of a step with 8.
     size = 16 if rows < 1024 else 64
     cap = rows // size + min(rows, n + 2)
     order = torch.empty(rows, dtype=torch.int32, device=dev)
@@ -144,8 +148,10 @@ def _forward(y, x, w, rows, hidden, out) -> None:
 def add_lora(y: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
              out: torch.Tensor | None = None, hidden: torch.Tensor | None = None) -> torch.Tensor:
     """y [rows, N] + scale (x [rows, K] a^T) b^T with each row's adapter, all of the stack's type; sums and
-    x a^T in float32 (of which float16's second product takes 22 bits), rounded once. Rows may be apart (x, y and out of any stride). A row without an adapter is y's.
-    out: where the result goes, y itself among others; a new tensor without it.
+    x a^T in float32 (of which float16's second product takes 22 bits), rounded once. Rows may be apart (x, y and out of any
+    stride). A row without an adapter is y's.
+    out: where the result goes, y itself among others; a new tensor without it. What out's rows reach over from the first to
+    the last must not meet x's, nor y's unless it is y: not columns of one buffer side by side.
     hidden: float32 [rows, rank] that receives scale x a^T, for add_lora_grad."""
     a, b, M = w.a, w.b, rows.rows
     _check_batch("add_lora", w, rows)
@@ -227,8 +233,9 @@ def _backward(dy, x, w, rows, hidden, need):
 def add_lora_grad(dy: torch.Tensor, x: torch.Tensor, w: LoraStack, rows: LoraRows,
                   hidden: torch.Tensor, need: tuple[bool, bool, bool] = (True, True, True)):
     """From the gradient dy [rows, N] of add_lora's output, its x, rows and the hidden that it filled: the gradients
-    (dx [rows, K], da [n, rank, K], db [n, N, rank]) of the stack's type, None where need says no. That of y is
-    dy itself. Sums in float32, in an order that the sizes and the rows' ids decide."""
+    (dx [rows, K], da [n, rank, K], db [n, N, rank]) of the stack's type, None where need says no (the pass
+    over dy that db comes out of is dx's and da's too). That of y is dy itself. Sums in float32, in an order that the sizes
+    and the rows' ids decide."""
     _check_batch("add_lora_grad", w, rows)
     _check_rows("add_lora_grad", "x", x, rows.rows, w.a.shape[2], w)
     _check_rows("add_lora_grad", "dy", dy, rows.rows, w.b.shape[1], w)

@@ -182,7 +182,7 @@ def policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logprobs: t
                      kl: float = 0.0, temperature: float = 1.0,
                      out: torch.Tensor | None = None) -> tuple[PolicyLoss, torch.Tensor]:
     """policy_loss and the gradient of the rows' sum, [R, V] of the logits' type: into out where given, which
-    may be the logits themselves."""
+    may be the logits themselves or lie apart from them as a whole (not columns of one buffer side by side)."""
     name = "policy_loss_grad"
     _check_policy(name, logits, tokens, old_logprobs, advantages, ref_logprobs, weight, clip, kl,
                   temperature, out)
@@ -201,7 +201,7 @@ def distill_top_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_logprobs: 
                      temperature: float = 1.0,
                      out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """distill_top and the gradient of the rows' sum, [R, V] of the logits' type: into out where given, which
-    may be the logits themselves."""
+    may be the logits themselves or lie apart from them as a whole (not columns of one buffer side by side)."""
     name = "distill_top_grad"
     _check_distill(name, logits, top_ids, top_logprobs, weight, temperature, out)
     _by_hand(name, logits)
